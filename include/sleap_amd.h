@@ -710,6 +710,59 @@ int sa_h264_decode_slice(const sa_h264_slice* s, const uint8_t* rbsp, int64_t n_
 int sa_yuv420_to_bgr(const uint8_t* y, const uint8_t* cb, const uint8_t* cr, int width, int height, int y_stride, int c_stride,
                      uint8_t* out, int channels);
 
+/* ------------------------------------------------------------------------------------------------
+ * Token operators -- layers of networks that read feature maps and clips as sets of tokens, and the step that fits them. The reference
+ * has none (its networks are convolutional, its optimizer is tf.keras.optimizers.Adam, sleap/nn/training.py); they stand beside the layer
+ * entry points above. Unlike those, the element type is an argument of the call; both library builds hold every type.
+ * Strides are in ELEMENTS, HOST arrays, and may be zero (a broadcast input); the last dimension is contiguous.
+ * ---------------------------------------------------------------------------------------------- */
+#define SA_F32 0
+#define SA_F16 1
+#define SA_BF16 2
+#define SA_POS_I32 0
+#define SA_POS_I64 1
+#define SA_POS_F32 2
+
+/* Rotary positions with several axes. x [B,T,H,D] (x_strides: B, T, H) -> y [B,T,H,D] contiguous, same type; D even.
+ *   positions  [B,T,n_axes] of pos_type (pos_strides: B, T, axis; B stride 0 where the batch shares them)
+ *   sections   HOST, pairs of each axis; P = their sum, 1 <= P <= 128, 2P <= D; values from 2P on pass
+ *   angle of pair i of axis a: position[a] * theta^-(i / sections[a]), or with shared_ladder theta^-(j / P) over all pairs j
+ *   pairs are (j, j + P), or (2j, 2j + 1) if `interleaved` (then addresses and strides are multiples of 2 elements)
+ *   inverse    turns by -angle: the gradient of x from the gradient of y
+ * Angles are accurate to 32 bits up to |position| of about 1e8. */
+int sa_rotary_axes(const void* x, int dtype, int B, int T, int H, int D, const int64_t* x_strides, const void* positions,
+                   int pos_type, const int64_t* pos_strides, int n_axes, const int* sections, double theta, int shared_ladder,
+                   int interleaved, int inverse, void* y, sa_stream_t stream);
+
+/* Cross attention: out[b,t,h] = sum_j w_j v[b,j,h'], w = softmax over the visible keys j of scale * q[b,t,h] . k[b,j,h'], h' = h / (Hq / Hkv).
+ *   q [B,Tq,Hq,D], k and v [B,Tk,Hkv,D] of `dtype` (SA_F16, SA_BF16); D a multiple of 8, at most 128; Hq a multiple of Hkv
+ *   strides      HOST, 9: batch, token, head of q, k, v; multiples of 8; addresses multiples of 16
+ *   key_lengths  [B] or NULL: keys j >= key_lengths[b] are hidden (values outside 0 .. Tk count as the nearer of the two)
+ *   key_mask     [B,Tk] bytes or NULL, 0 hides a key (mask_strides: HOST, batch, token); what hidden keys and values hold is not read
+ *                into a result, NaN and infinities included
+ *   out          [B,Tq,Hq,D] contiguous; zeros where no key is visible
+ *   lse          [B,Hq,Tq] natural logarithm of the softmax's denominator (-inf where no key is visible), or NULL
+ *   workspace    sa_cross_attention_workspace bytes (0: none): runs of keys that several workgroups work on */
+size_t sa_cross_attention_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D);
+int sa_cross_attention(const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D,
+                       const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, const int64_t* mask_strides,
+                       float scale, void* out, float* lse, void* workspace, size_t workspace_bytes, sa_stream_t stream);
+
+/* One AdamW step over n tensors of one type, in place (decoupled decay; 32-bit states and arithmetic; a 16-bit parameter is rounded once):
+ *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  [vmax = max(vmax, v)];  p = p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v | vmax)/sqrt(1-b2^t) + eps)
+ *   tensors    HOST array; its addresses travel in the launches' arguments (64 tensors a launch): nothing is kept after the call
+ *   step       t >= 1, or step_dev: DEVICE counter that already holds t (a captured step); lr_dev: DEVICE learning rate or NULL */
+typedef struct {
+  void* param;             /* dtype, n contiguous values */
+  const void* grad;        /* dtype */
+  float* exp_avg;
+  float* exp_avg_sq;
+  float* max_exp_avg_sq;   /* with amsgrad, else NULL */
+  int64_t n;
+} sa_adamw_tensor;
+int sa_adamw_step(const sa_adamw_tensor* tensors, int n, int dtype, int amsgrad, double lr, const float* lr_dev, double beta1,
+                  double beta2, double eps, double weight_decay, int64_t step, const int64_t* step_dev, sa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,169 @@
+// Pieces that the cross attention kernels (attention.hip, attention_bwd.hip) share.
+//
+// Layout of the work. All query heads that share a key head are one matrix: row r = t * G + g is token t of the g-th of those heads,
+// so a single token of 8 heads on 2 key heads is a tile of 4 rows and shared heads sum their gradients by themselves.
+//
+// Matrix products are v_mfma_f32_32x32x16 (fp16 / bf16 operands, float32 sums): A [32 x 16] gives lane l the eight k-values
+// 8 (l >> 5) .. + 7 of row l & 31, B [16 x 32] the same of column l & 31, and C [32 x 32] holds column l & 31 in lane l, its
+// register i being row 8 (i >> 2) + 4 (l >> 5) + (i & 3). Every product here is arranged so that the 32 columns are rows r of the
+// softmax (or keys, for the gradients of k and v): one lane then owns one softmax row (shared with lane ^ 32), maxima and sums need one
+// exchange, and registers 8s .. 8s + 7 of a C are, rounded to 16 bits, the B operand of the next product -- for the k order
+// {4h .. 4h + 3, 8 + 4h .. 8 + 4h + 3}, h = l >> 5. The A operand in that order is two transposed reads from LDS
+// (ds_read_b64_tr_b16: 16 lanes read four rows of 16 values and lane i gets column i), so no value of a softmax passes through LDS.
+//
+// Tiles in LDS are rows of DP 16-bit values (DP = 32, 64 or 128). Pieces of 16 bytes are exchanged within a row, piece c to
+// c ^ swizzle(row), in steps of 32 bytes, so that eight rows read at one piece (A operand) and four rows read at 32 neighbouring
+// bytes (transposed) fall into different banks. Tiles come by buffer_load ... lds: the swizzle is applied to the source offset,
+// and a lane whose key is hidden or whose piece lies behind D gets an offset out of range, which writes zeros: what hidden
+// keys hold (NaN, infinities) never enters a product.
+#pragma once
+#include "sa_common.h"
+#include "token_types.h"
+
+namespace sa {
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int TILE = 64;                   // rows of a tile in LDS
+constexpr uint32_t OUT_OF_RANGE = 0xFFFFFFF0u;
+
+template <typename E>
+struct Mfma;
+template <>
+struct Mfma<_Float16> {
+  typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+  typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+  __device__ static __forceinline__ f32x16 run(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mfma<__bf16> {
+  typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+  typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+  __device__ static __forceinline__ f32x16 run(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+};
+
+template <typename E>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const f32x2 v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, typename Mfma<E>::v2));
+}
+// registers 8s .. 8s + 7 of a C as a B operand
+template <typename E>
+__device__ __forceinline__ s16x8 pack8(const f32x16& c, int s) {
+  const u32x4 v = {pack2<E>(c[8 * s], c[8 * s + 1]), pack2<E>(c[8 * s + 2], c[8 * s + 3]), pack2<E>(c[8 * s + 4], c[8 * s + 5]),
+                   pack2<E>(c[8 * s + 6], c[8 * s + 7])};
+  return __builtin_bit_cast(s16x8, v);
+}
+
+// the other half-wave's value of the same column
+__device__ __forceinline__ float other_half(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // lanes < 32: {own, upper}; lanes >= 32: {lower, own}
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float max_halves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <int DP>
+__device__ __forceinline__ int swizzle(int row) {
+  constexpr int PER_LINE = 128 / DP, PAIRS = DP / 16;  // rows of 256 bytes, 32-byte pairs of a row
+  return ((row / PER_LINE) & (PAIRS - 1)) << 1;
+}
+
+// one 16-bit [TILE][DP] tile in LDS
+template <int DP>
+struct Tile {
+  static constexpr int ROW = DP * 2, BYTES = TILE * ROW, PIECES = BYTES / 1024;
+  // byte address of the A operand's eight values at k-step ks, row m of a 32-row block: off_a(m, h, ks) + block * 32 * ROW
+  __device__ static __forceinline__ int off_a(int m, int h, int ks) { return m * ROW + (((ks * 2 + h) ^ swizzle<DP>(m)) << 4); }
+  // transposed read: rows 16 kk + 8 u + 4 h .. + 3, columns of block db: off_t(lane, db) + (16 kk + 8 u) * ROW
+  __device__ static __forceinline__ int off_t(int lane, int db) {
+    const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), c = db * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    return row * ROW + ((c ^ swizzle<DP>(row)) << 4) + (lane & 1) * 8;
+  }
+};
+
+__device__ __forceinline__ s16x8 read_a(const char* lds, int off) { return *reinterpret_cast<const s16x8*>(lds + off); }
+__device__ __forceinline__ s16x8 read_t(const char* lds, int off, int step) {
+  typedef __attribute__((address_space(3))) s16x4* p4;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lds + off)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lds + off + step));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// every wave's copies have landed, every wave's reads are done
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Copies of a tile's rows into LDS by NW waves. `rows` is the 64-bit word of the rows that exist (all others become zeros).
+template <int DP, int NW>
+struct TileCopy {
+  static constexpr int N = (Tile<DP>::PIECES + NW - 1) / NW;
+  uint32_t off[N];
+  int row[N];
+  __device__ __forceinline__ void init(int wave, int lane, int64_t stride_bytes, int D) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int at = (wave + j * NW) * 1024 + lane * 16;
+      row[j] = at / Tile<DP>::ROW;
+      const int c = ((at >> 4) & (DP / 8 - 1)) ^ swizzle<DP>(row[j]);
+      off[j] = c * 8 < D ? (uint32_t)(row[j] * stride_bytes) + c * 16 : OUT_OF_RANGE;
+    }
+  }
+  __device__ __forceinline__ void issue(char* lds, const void* base, uint64_t rows, int wave) const {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (Tile<DP>::PIECES % NW != 0 && wave + j * NW >= Tile<DP>::PIECES) break;
+      const uint32_t o = rows == ~0ull ? off[j] : ((rows >> row[j]) & 1) ? off[j] : OUT_OF_RANGE;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(lds + (wave + j * NW) * 1024), 16, o, 0, 0, 0);
+    }
+  }
+};
+
+// hides the scores of keys whose bit in `seen` (32 keys of a block) is not set
+__device__ __forceinline__ void hide(f32x16& s, uint32_t seen, int h, float with) {
+  const uint32_t w = seen >> (4 * h);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = (w >> (8 * (i >> 2) + (i & 3))) & 1 ? s[i] : with;
+}
+
+// workgroups that read the same keys are neighbours in `id`: give each of the eight XCDs (workgroups go round them) a run of ids
+__device__ __forceinline__ uint32_t xcd_run(uint32_t block, uint32_t n) {
+  const uint32_t x = block & 7, q = n >> 3, r = n & 7;
+  return x * q + min(x, r) + (block >> 3);
+}
+
+// what forward and backward know of a call
+struct AttnShape {
+  const void *q, *k, *v;
+  int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh;  // strides in elements
+  int Tq, Tk, G, Hq, Hkv, D;
+  uint32_t R;                                  // rows of a key head: Tq * G
+  FastDiv div_g;
+  const int32_t* lengths;                      // keys of each batch entry, or NULL
+  const uint8_t* mask;                         // [B, Tk], 0 hides a key, or NULL
+  int64_t mb, mt;
+  float c;                                     // scale * log2(e)
+  float scale;
+};
+
+}  // namespace sa

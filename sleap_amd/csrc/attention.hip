@@ -1,0 +1,322 @@
+// Cross attention to an encoder's states: out = softmax(scale q k^T over the visible keys) v, rows without a visible key are zero.
+// One pass over the keys with a running maximum and sum per row (in 32 bits); the layout of the products is in attention.h:
+//     S^T [keys x rows] = k q^T        P^T = exp2(c S^T - m)        O^T [d x rows] += v^T P^T
+#include "attention.h"
+
+namespace {
+
+using namespace sa;
+
+struct FwdParams {
+  AttnShape a;
+  void* out;              // [B, Tq, Hq, D] contiguous
+  float* lse;             // [B, Hq, Tq] natural logarithm of the softmax's denominator, or NULL
+  float* part;            // splits > 1: [B * Hkv][splits][R][D] of each run of keys, normalised
+  float* part_lse;        // and their base-2 logarithms [B * Hkv][splits][R]
+  uint32_t blocks, row_tiles, splits;
+  FastDiv div_tiles, div_splits, div_heads;
+  int split_keys;         // keys of a run: a multiple of TILE
+};
+
+// P is rounded to 16 bits. Its maximum is 2^GROW at most (the running maximum is only followed when it has grown by 2^GROW: most tiles
+// then skip the rescaling of O). fp16 moves all of P up by a power of two, so that weights down to 2^-31 of the largest are held.
+template <typename E>
+struct Range {
+  static constexpr float LIFT = 0.0f;
+};
+template <>
+struct Range<_Float16> {
+  static constexpr float LIFT = 7.0f;
+};
+constexpr float GROW = 8.0f;
+
+template <typename E, int DB, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p) {
+  constexpr int DP = DB == 3 ? 128 : DB * 32, KS = DB * 2;
+  using T = Tile<DP>;
+  extern __shared__ __align__(1024) char lds[];  // [2 stages][k tile, v tile]
+  const AttnShape& a = p.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+  const uint32_t id = xcd_run(blockIdx.x, p.blocks);
+  const uint32_t bhs = div_by(id, p.div_tiles), tile = id - bhs * p.row_tiles;
+  const uint32_t bh = div_by(bhs, p.div_splits), split = bhs - bh * p.splits;
+  const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv;
+
+  const uint32_t row = tile * (NW * 32) + wave * 32 + n;
+  const bool real = row < a.R;
+  const uint32_t rr = real ? row : a.R - 1, t = div_by(rr, a.div_g), g = rr - t * a.G;
+  s16x8 q[KS];
+  {
+    const E* src = static_cast<const E*>(a.q) + (int64_t)b * a.qb + (int64_t)t * a.qt + (int64_t)(hk * a.G + g) * a.qh;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = ks * 16 + h * 8;
+      q[ks] = d < a.D ? *reinterpret_cast<const s16x8*>(src + d) : s16x8{};
+    }
+  }
+  int length = a.Tk;
+  if (a.lengths) length = min(max(a.lengths[b], 0), a.Tk);
+  const int first = (int)split * p.split_keys, end = min(first + p.split_keys, length);
+  const int tiles = end > first ? (end - first + TILE - 1) / TILE : 0;
+  const E* kbase = static_cast<const E*>(a.k) + (int64_t)b * a.kb + (int64_t)hk * a.kh;
+  const E* vbase = static_cast<const E*>(a.v) + (int64_t)b * a.vb + (int64_t)hk * a.vh;
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mb : nullptr;
+  TileCopy<DP, NW> ck, cv;
+  ck.init(wave, lane, a.kt * 2, a.D);
+  cv.init(wave, lane, a.vt * 2, a.D);
+
+  auto load_mask = [&](int i) -> uint8_t {
+    const int key = first + i * TILE + lane;
+    return mask && key < end ? mask[(int64_t)key * a.mt] : 1;
+  };
+  auto seen_of = [&](int i, uint8_t m) { return __ballot(first + i * TILE + lane < end && m); };
+  auto copy = [&](int i, uint64_t seen) {
+    char* s = lds + (i & 1) * 2 * T::BYTES;
+    const int64_t key = first + (int64_t)i * TILE;
+    ck.issue(s, kbase + key * a.kt, seen, wave);
+    cv.issue(s + T::BYTES, vbase + key * a.vt, seen, wave);
+  };
+
+  int oa[KS], ot[DB];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) oa[ks] = T::off_a(n, h, ks);
+#pragma unroll
+  for (int db = 0; db < DB; ++db) ot[db] = T::off_t(lane, db);
+
+  f32x16 o[DB] = {};
+  float m = -INFINITY, l = 0.0f, shift = -Range<E>::LIFT;  // shift = c m - LIFT, of a maximum that is not -inf
+  uint64_t seen = 0;
+  uint8_t next_mask = 1;
+  if (tiles) {
+    seen = seen_of(0, load_mask(0));
+    copy(0, seen);
+    next_mask = load_mask(1);
+  }
+  for (int i = 0; i < tiles; ++i) {
+    tile_barrier();
+    const uint64_t now = seen;
+    if (i + 1 < tiles) {
+      seen = seen_of(i + 1, next_mask);
+      copy(i + 1, seen);
+      next_mask = load_mask(i + 2);
+    }
+    if (now == 0) continue;
+    const char* kt = lds + (i & 1) * 2 * T::BYTES;
+    const char* vt = kt + T::BYTES;
+    f32x16 s0 = {}, s1 = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      s0 = Mfma<E>::run(read_a(kt, oa[ks]), q[ks], s0);
+      s1 = Mfma<E>::run(read_a(kt, oa[ks] + 32 * T::ROW), q[ks], s1);
+    }
+    if (now != ~0ull) {
+      hide(s0, (uint32_t)now, h, -INFINITY);
+      hide(s1, (uint32_t)(now >> 32), h, -INFINITY);
+    }
+    float top = fmaxf(s0[0], s1[0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s0[i], s1[i]));
+    top = max_halves(top);
+    if (__any((top - m) * a.c > GROW)) {
+      const float grown = fmaxf(m, top), at = grown == -INFINITY ? 0.0f : grown;
+      const float keep = __builtin_amdgcn_exp2f((m - at) * a.c);
+      m = grown;
+      shift = at * a.c - Range<E>::LIFT;
+      l *= keep;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] *= keep;
+    }
+    float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s0[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s0[i], a.c, -shift));
+      s1[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[i], a.c, -shift));
+      l0 += s0[i];
+      l1 += s1[i];
+    }
+    l += l0 + l1;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      const s16x8 w = pack8<E>(kk < 2 ? s0 : s1, kk & 1);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = Mfma<E>::run(read_t(vt, ot[db] + kk * 16 * T::ROW, 8 * T::ROW), w, o[db]);
+    }
+  }
+
+  l = sum_halves(l);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (!real) return;
+  if (p.splits > 1) {
+    const int64_t at = ((int64_t)bh * p.splits + split) * a.R + row;
+    if (h == 0) p.part_lse[at] = l == 0.0f ? -INFINITY : shift + __log2f(l);
+    float* dst = p.part + at * a.D;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = db * 32 + j * 8 + h * 4;
+        if (d < a.D) *reinterpret_cast<f32x4*>(dst + d) = f32x4{o[db][4 * j] * inv, o[db][4 * j + 1] * inv, o[db][4 * j + 2] * inv, o[db][4 * j + 3] * inv};
+      }
+    return;
+  }
+  if (p.lse && h == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = l == 0.0f ? -INFINITY : (shift + __log2f(l)) * LN2;
+  E* dst = static_cast<E*>(p.out) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = db * 32 + j * 8 + h * 4;
+      if (d < a.D) *reinterpret_cast<u32x2*>(dst + d) = u32x2{pack2<E>(o[db][4 * j] * inv, o[db][4 * j + 1] * inv), pack2<E>(o[db][4 * j + 2] * inv, o[db][4 * j + 3] * inv)};
+    }
+}
+
+// joins the runs of keys: out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max); a thread has 8 values of a row
+template <typename E>
+__global__ __launch_bounds__(256) void attention_join_kernel(const FwdParams p, FastDiv div_pieces, FastDiv div_rows, uint32_t pieces, uint32_t total) {
+  const AttnShape& a = p.a;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const uint32_t br = div_by(i, div_pieces), d = (i - br * pieces) * 8;
+  const uint32_t bh = div_by(br, div_rows), row = br - bh * a.R;
+  const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv, t = div_by(row, a.div_g), g = row - t * a.G;
+  const float* lse = p.part_lse + (int64_t)bh * p.splits * a.R + row;
+  float top = -INFINITY;
+  for (uint32_t s = 0; s < p.splits; ++s) top = fmaxf(top, lse[(int64_t)s * a.R]);
+  const float at = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f, acc[8] = {};
+  for (uint32_t s = 0; s < p.splits; ++s) {
+    const float w = __builtin_amdgcn_exp2f(lse[(int64_t)s * a.R] - at);
+    const f32x4* src = reinterpret_cast<const f32x4*>(p.part + (((int64_t)bh * p.splits + s) * a.R + row) * a.D + d);
+    const f32x4 x = src[0], y = src[1];
+    sum += w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc[e] += w * x[e];
+      acc[4 + e] += w * y[e];
+    }
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  if (p.lse && d == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = sum == 0.0f ? -INFINITY : (at + __log2f(sum)) * LN2;
+  E* dst = static_cast<E*>(p.out) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D + d;
+  *reinterpret_cast<u32x4*>(dst) = u32x4{pack2<E>(acc[0] * inv, acc[1] * inv), pack2<E>(acc[2] * inv, acc[3] * inv),
+                                         pack2<E>(acc[4] * inv, acc[5] * inv), pack2<E>(acc[6] * inv, acc[7] * inv)};
+}
+
+// How a call is cut: waves of a workgroup (32 rows each) and runs of keys.
+struct Cut {
+  int waves;
+  uint32_t row_tiles, splits;
+  int split_keys;
+};
+Cut cut(int B, int Tq, int Tk, int Hq, int Hkv) {
+  const uint64_t R = (uint64_t)Tq * (Hq / Hkv);
+  Cut c;
+  c.waves = R <= 32 ? 1 : R <= 64 ? 2 : 4;
+  c.row_tiles = (uint32_t)((R + c.waves * 32 - 1) / (c.waves * 32));
+  const uint64_t blocks = (uint64_t)c.row_tiles * B * Hkv;
+  const uint64_t want = 2048 / c.waves;  // eight waves a CU
+  const uint32_t key_tiles = (uint32_t)((Tk + TILE - 1) / TILE);
+  uint64_t splits = blocks ? want / blocks : 1;
+  const uint64_t most = key_tiles / 4;   // a run of at least four tiles
+  if (splits > most) splits = most;
+  if (splits < 1) splits = 1;
+  const uint32_t per = key_tiles ? (uint32_t)((key_tiles + splits - 1) / splits) : 1;
+  c.split_keys = (int)per * TILE;
+  c.splits = key_tiles ? (key_tiles + per - 1) / per : 1;
+  return c;
+}
+
+template <typename E, int DB>
+void launch(const FwdParams& p, int waves, hipStream_t s) {
+  constexpr size_t lds = 4 * Tile<DB == 3 ? 128 : DB * 32>::BYTES;
+  if (waves == 1) attention_kernel<E, DB, 1><<<dim3(p.blocks), dim3(64), lds, s>>>(p);
+  else if (waves == 2) attention_kernel<E, DB, 2><<<dim3(p.blocks), dim3(128), lds, s>>>(p);
+  else attention_kernel<E, DB, 4><<<dim3(p.blocks), dim3(256), lds, s>>>(p);
+}
+
+template <typename E>
+void launch_e(const FwdParams& p, int waves, hipStream_t s) {
+  const int db = (p.a.D + 31) / 32;
+  if (db == 1) launch<E, 1>(p, waves, s);
+  else if (db == 2) launch<E, 2>(p, waves, s);
+  else if (db == 3) launch<E, 3>(p, waves, s);
+  else launch<E, 4>(p, waves, s);
+  if (p.splits > 1) {
+    const uint32_t pieces = p.a.D / 8, total = (uint32_t)(p.blocks / p.row_tiles / p.splits) * p.a.R * pieces;
+    attention_join_kernel<E><<<dim3((total + 255) / 256), dim3(256), 0, s>>>(p, fast_div(pieces), fast_div(p.a.R), pieces, total);
+  }
+}
+
+}  // namespace
+
+namespace sa {
+
+int attention_shape(const char* who, AttnShape* a, const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq,
+                    int Hkv, int D, const int64_t* strides, const int32_t* lengths, const uint8_t* mask, const int64_t* mask_strides, float scale) {
+  SA_REQUIRE(B >= 0 && Tq >= 0 && Tk >= 0 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0, "%s: bad shape B=%d Tq=%d Tk=%d Hq=%d Hkv=%d", who, B, Tq, Tk, Hq, Hkv);
+  SA_REQUIRE(D >= 8 && D <= 128 && D % 8 == 0, "%s: head size %d (a multiple of 8, at most 128)", who, D);
+  SA_REQUIRE(dtype == SA_F16 || dtype == SA_BF16, "%s: 16-bit types only (%d)", who, dtype);
+  SA_REQUIRE(scale > 0 && scale <= 1e30f, "%s: scale must be positive and finite", who);
+  SA_REQUIRE(Tk <= (1 << 30) && (uint64_t)Tq * (Hq / Hkv) < (1ull << 31) - 1024 && (uint64_t)B * Hq < (1ull << 31), "%s: too many rows", who);
+  for (int i = 0; i < 9; ++i) SA_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, "%s: strides are multiples of 8 elements", who);
+  for (int i = 3; i < 9; i += 3) SA_REQUIRE(strides[i + 1] < (1ll << 23), "%s: token strides of keys and values are below 2^23 elements", who);
+  SA_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0, "%s: addresses are multiples of 16", who);
+  a->q = q;
+  a->k = k;
+  a->v = v;
+  a->qb = strides[0]; a->qt = strides[1]; a->qh = strides[2];
+  a->kb = strides[3]; a->kt = strides[4]; a->kh = strides[5];
+  a->vb = strides[6]; a->vt = strides[7]; a->vh = strides[8];
+  a->Tq = Tq;
+  a->Tk = Tk;
+  a->Hq = Hq;
+  a->Hkv = Hkv;
+  a->G = Hq / Hkv;
+  a->D = D;
+  a->R = (uint32_t)Tq * a->G;
+  a->div_g = fast_div(a->G);
+  a->lengths = lengths;
+  a->mask = mask;
+  a->mb = mask ? mask_strides[0] : 0;
+  a->mt = mask ? mask_strides[1] : 0;
+  a->scale = scale;
+  a->c = scale * LOG2E;
+  return SA_OK;
+}
+
+}  // namespace sa
+
+extern "C" size_t sa_cross_attention_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
+  if (B < 1 || Tq < 1 || Tk < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1) return 0;
+  const Cut c = cut(B, Tq, Tk, Hq, Hkv);
+  return c.splits > 1 ? (size_t)B * Hq * Tq * c.splits * (D + 1) * sizeof(float) : 0;
+}
+
+extern "C" int sa_cross_attention(const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D,
+                                  const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, const int64_t* mask_strides,
+                                  float scale, void* out, float* lse, void* workspace, size_t workspace_bytes, sa_stream_t stream) {
+  FwdParams p;
+  if (int rc = attention_shape("sa_cross_attention", &p.a, q, k, v, dtype, B, Tq, Tk, Hq, Hkv, D, strides, key_lengths, key_mask, mask_strides, scale)) return rc;
+  if (B == 0 || Tq == 0) return SA_OK;
+  SA_REQUIRE(((uintptr_t)out & 15) == 0, "sa_cross_attention: addresses are multiples of 16");
+  const Cut c = cut(B, Tq, Tk, Hq, Hkv);
+  const uint64_t blocks = (uint64_t)c.row_tiles * c.splits * B * Hkv;
+  SA_REQUIRE(blocks < (1ull << 31) && (uint64_t)B * Hq * Tq * D / 8 < (1ull << 31), "sa_cross_attention: too many rows");
+  if (c.splits > 1 && workspace_bytes < sa_cross_attention_workspace(B, Tq, Tk, Hq, Hkv, D))
+    return fail(SA_ERR_WORKSPACE, "sa_cross_attention: workspace of %zu bytes is too small", workspace_bytes);
+  p.out = out;
+  p.lse = lse;
+  p.part = static_cast<float*>(workspace);
+  p.part_lse = p.part + (size_t)B * Hq * Tq * c.splits * D;
+  p.blocks = (uint32_t)blocks;
+  p.row_tiles = c.row_tiles;
+  p.splits = c.splits;
+  p.split_keys = c.split_keys;
+  p.div_tiles = fast_div(c.row_tiles);
+  p.div_splits = fast_div(c.splits);
+  p.div_heads = fast_div(Hkv);
+  if (dtype == SA_F16) launch_e<_Float16>(p, c.waves, (hipStream_t)stream);
+  else launch_e<__bf16>(p, c.waves, (hipStream_t)stream);
+  SA_LAUNCH_CHECK();
+  return SA_OK;
+}

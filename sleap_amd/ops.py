@@ -5,6 +5,7 @@ torch stream. Shapes and meanings follow include/sleap_amd.h.
 """
 import collections
 import ctypes as C
+import math
 
 import numpy as np
 import torch
@@ -397,3 +398,261 @@ def optical_flow_pyr_lk(prev: "FlowPyramid", nxt: "FlowPyramid", points, max_cou
     check(_lib.lib().sa_flow_lk(_ptr(ptrs), _ptr(nxt.buf), nxt.H, nxt.W, nxt.win, nxt.max_level, n, _ptr(pts), _ptr(out),
                                 _ptr(status), _ptr(err), int(max_count), float(epsilon), _stream()), "sa_flow_lk")
     return out, status, err
+
+
+# --------------------------------------------------------------------------------------------------
+# token operators (csrc/rotary.hip, attention.hip, attention_bwd.hip, adamw.hip): keypoint queries and feature-map tokens. Unlike the
+# layer wrappers above they take any torch layout, check their arguments, run on the device of their tensors and have gradients.
+# --------------------------------------------------------------------------------------------------
+_TOKEN_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # SA_F32, SA_F16, SA_BF16
+_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}     # SA_POS_*
+
+
+def _launch(name, device, *args):
+    """One C call on the tensors' own device and its current stream."""
+    fn = getattr(_lib.lib(), name)
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, C.c_void_p(torch.cuda.current_stream(device).cuda_stream)), name)
+        return
+    with torch.cuda.device(device):
+        check(fn(*args, C.c_void_p(torch.cuda.current_stream(device).cuda_stream)), name)
+
+
+def _cuda_tensors(who, **tensors):
+    device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError(f"{who}: {name} must be a CUDA tensor (there is no CPU fallback)")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f"{who}: {name} is on {t.device}, not on {device}")
+    return device
+
+
+def _strides(t, dims):
+    """Strides of the first `dims` dimensions in elements; 0 where there is nothing to step over."""
+    return [s if n > 1 else 0 for n, s in zip(t.shape[:dims], t.stride()[:dims])]
+
+
+def _laid_out(t, elements, limit=None):
+    """`t` itself if its last dimension is contiguous and every other stride and the address are whole multiples of `elements`
+    values (and, with `limit`, the second dimension's stride is below it), else a contiguous copy."""
+    s = _strides(t, 3)
+    if t.numel() and ((t.shape[3] > 1 and t.stride(3) != 1) or any(v % elements for v in s) or t.data_ptr() % (elements * t.element_size())
+                      or (limit is not None and s[1] >= limit)):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _i64(values):
+    return (C.c_int64 * len(values))(*values)
+
+
+def _rotary_call(x, positions, sections, theta, ladder, interleaved, inverse):
+    x = _laid_out(x, 2 if interleaved else 1)
+    B, T, H, D = x.shape
+    y = torch.empty((B, T, H, D), dtype=x.dtype, device=x.device)
+    if y.numel():
+        p = positions if positions.dim() == 3 else positions[None]
+        ps = list(p.stride())
+        if p.shape[0] == 1:
+            ps[0] = 0
+        _launch("sa_rotary_axes", x.device, x.data_ptr(), _TOKEN_TYPES[x.dtype], B, T, H, D, _i64(_strides(x, 3)), p.data_ptr(),
+                _POSITION_TYPES[p.dtype], _i64(ps), len(sections), (C.c_int * len(sections))(*sections), float(theta), int(ladder == "shared"),
+                int(interleaved), int(inverse), y.data_ptr())
+    return y
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, sections, theta, ladder, interleaved, inverse):
+        ctx.save_for_backward(positions)
+        ctx.how = (sections, theta, ladder, interleaved, inverse)
+        return _rotary_call(x, positions, *ctx.how)
+
+    @staticmethod
+    def backward(ctx, dy):
+        (positions,) = ctx.saved_tensors
+        sections, theta, ladder, interleaved, inverse = ctx.how
+        # linear in x: its gradient is the turn the other way, which has a gradient again
+        return rotary_axes(dy, positions, sections, theta, ladder, interleaved, not inverse), None, None, None, None, None, None
+
+
+def rotary_axes(x, positions, sections, theta=10000.0, ladder="axis", interleaved=False, inverse=False):
+    """Rotary positions with several axes (time, row, column of a clip; x, y of a keypoint) -> tensor like `x`, contiguous.
+
+    x           (B, T, H, D) float32 / float16 / bfloat16, D even
+    positions   (T, A) or (B, T, A) int32, int64 or float32: the A coordinates of every token (32-bit accurate angles up to |position| 1e8)
+    sections    A counts of pairs: the first sections[0] pairs turn with axis 0, the next sections[1] with axis 1, ...; their sum P <= D / 2
+                (and <= 128); values from 2 P on pass
+    ladder      "axis": pair i of an axis with n pairs has frequency theta^(-i / n); "shared": pair j of all P has theta^(-j / P)
+    interleaved pairs are (2j, 2j + 1) instead of (j, j + P)
+    inverse     turn the other way
+    Differentiable in x."""
+    _cuda_tensors("rotary_axes", x=x, positions=positions)
+    if x.dim() != 4 or x.shape[3] % 2 or x.shape[3] < 2 or x.shape[3] > 4096 or not 1 <= x.shape[2] <= 4096:
+        raise ValueError(f"rotary_axes: x must be (B, T, heads, even size): got {tuple(x.shape)}")
+    if x.dtype not in _TOKEN_TYPES:
+        raise TypeError(f"rotary_axes: x must be float32, float16 or bfloat16: got {x.dtype}")
+    if positions.dtype not in _POSITION_TYPES:
+        raise TypeError(f"rotary_axes: positions must be int32, int64 or float32: got {positions.dtype}")
+    sections = tuple(int(n) for n in sections)
+    B, T, _, D = x.shape
+    if not 1 <= len(sections) <= 8 or min(sections) < 0 or not 1 <= sum(sections) <= min(D // 2, 128):
+        raise ValueError(f"rotary_axes: sections {sections} do not fit a head of {D} (at most 8 axes and 128 pairs of two values)")
+    if tuple(positions.shape) not in ((T, len(sections)), (B, T, len(sections)), (1, T, len(sections))):
+        raise ValueError(f"rotary_axes: positions {tuple(positions.shape)} for {B} x {T} tokens and {len(sections)} axes")
+    if ladder not in ("axis", "shared"):
+        raise ValueError(f"rotary_axes: ladder {ladder!r}: 'axis' or 'shared'")
+    if not 0 < theta < 1e30:
+        raise ValueError(f"rotary_axes: theta {theta}")
+    if positions.requires_grad:
+        raise ValueError("rotary_axes: there is no gradient for positions")
+    how = (sections, float(theta), ladder, bool(interleaved), bool(inverse))
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Rotary.apply(x, positions, *how)
+    return _rotary_call(x, positions, *how)
+
+
+_KEY_STRIDE = 1 << 23  # token strides of keys and values, in elements: a tile of 64 tokens spans less than 2 GiB
+
+
+class _Keys:
+    """Which keys are visible, as the C calls take it."""
+
+    def __init__(self, lengths, mask, B, Tk):
+        if lengths is not None:
+            if lengths.dtype not in (torch.int32, torch.int64) or tuple(lengths.shape) != (B,):
+                raise ValueError(f"cross_attention: key_lengths must be ({B},) int32 or int64: got {tuple(lengths.shape)} {lengths.dtype}")
+            lengths = lengths.clamp(0, Tk).to(torch.int32).contiguous() if lengths.dtype == torch.int64 else lengths.contiguous()
+        if mask is not None:
+            if mask.dtype != torch.bool or tuple(mask.shape) not in ((B, Tk), (1, Tk)):
+                raise ValueError(f"cross_attention: key_mask must be ({B}, {Tk}) bool, True where a key is visible: got {tuple(mask.shape)} {mask.dtype}")
+        self.lengths, self.mask = lengths, mask
+
+    def args(self):
+        return (self.lengths.data_ptr() if self.lengths is not None else None, self.mask.data_ptr() if self.mask is not None else None,
+                _i64(_strides(self.mask, 2)) if self.mask is not None else None)
+
+
+def _attention_args(q, k, v):
+    B, Tq, H, D = q.shape
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), _TOKEN_TYPES[q.dtype], B, Tq, k.shape[1], H, k.shape[2], D,
+            _i64(_strides(q, 3) + _strides(k, 3) + _strides(v, 3)))
+
+
+def _workspace(name, device, *args):
+    n = getattr(_lib.lib(), name)(*args)
+    t = torch.empty((n,), dtype=torch.uint8, device=device) if n else None  # of this call alone: the allocator orders its next use
+    return t, (t.data_ptr() if n else None, n)
+
+
+def _attention_forward(q, k, v, keys, scale, want_lse):
+    q, k, v = _laid_out(q, 8), _laid_out(k, 8, _KEY_STRIDE), _laid_out(v, 8, _KEY_STRIDE)
+    B, Tq, H, D = q.shape
+    out = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
+    if out.numel():
+        ws, ws_args = _workspace("sa_cross_attention_workspace", q.device, B, Tq, k.shape[1], H, k.shape[2], D)
+        _launch("sa_cross_attention", q.device, *_attention_args(q, k, v), *keys.args(), scale, out.data_ptr(),
+                lse.data_ptr() if want_lse else None, *ws_args)
+    return out, lse
+
+
+def _attention_checks(who, q, k, v, key_lengths, key_mask, scale):
+    _cuda_tensors(who, q=q, k=k, v=v, key_lengths=key_lengths, key_mask=key_mask)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"{who}: q (B, Tq, heads, D), k and v (B, Tk, key heads, D): got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"{who}: q, k and v must all be float16 or all bfloat16: got {q.dtype}, {k.dtype}, {v.dtype}")
+    D = q.shape[3]
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"{who}: head size {D}: a multiple of 8, at most 128")
+    if q.shape[2] < 1 or k.shape[2] < 1 or q.shape[2] % k.shape[2]:
+        raise ValueError(f"{who}: {q.shape[2]} query heads do not share {k.shape[2]} key heads evenly")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0 < scale <= 1e30:
+        raise ValueError(f"{who}: scale {scale} must be positive and finite")
+    return _Keys(key_lengths, key_mask, q.shape[0], k.shape[1]), scale
+
+
+def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, return_lse=False):
+    """softmax(scale q k^T) v of queries over the tokens of an encoder's states (a feature map, a clip) -> (B, Tq, H, D) like q, contiguous.
+
+    q            (B, Tq, H, D) float16 or bfloat16; D a multiple of 8, at most 128; any strides (unaligned ones cost a copy)
+    k, v         (B, Tk, K, D) of q's type; H a multiple of K: head h reads key head h // (H // K)
+    key_lengths  (B,) int32 / int64: keys from key_lengths[b] on are hidden (padding)
+    key_mask     (B, Tk) or (1, Tk) bool: False hides a key. What hidden keys and values hold (NaN, infinities) reaches no result
+    scale        positive; default 1 / sqrt(D)
+    return_lse   also the natural logarithm of the softmax's denominators, (B, H, Tq) float32, without a gradient
+    A query that sees no key gives zeros (lse: -inf) and passes no gradient. Softmax and sums are float32, weights are rounded to q's
+    type before the product with v; results do not depend on the order in which workgroups run. Differentiable in q, k and v, once."""
+    keys, scale = _attention_checks("cross_attention", q, k, v, key_lengths, key_mask, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise NotImplementedError("cross_attention: no gradient yet; call it under torch.no_grad()")
+    out, lse = _attention_forward(q, k, v, keys, scale, return_lse)
+    return (out, lse) if return_lse else out
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_exp_avg_sqs=None):
+    """One AdamW step over many tensors, in place, in as few launches as there are 64 tensors of one type and device:
+
+        m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  [vmax = max(vmax, v)]
+        p = p (1 - lr wd) - lr / (1-b1^t) m / (sqrt(v or vmax) / sqrt(1-b2^t) + eps)
+
+    params, grads   lists of contiguous float32 / float16 / bfloat16 CUDA tensors, pairwise of one type and size; arithmetic is float32, a
+                    16-bit parameter is rounded to nearest once a step (steps below half its spacing are lost)
+    exp_avgs, exp_avg_sqs, max_exp_avg_sqs (amsgrad, or None)   float32 tensors of the same sizes
+    step            t >= 1, or a one-element int64 CUDA tensor that already holds it; lr likewise a number or a one-element float32 CUDA
+                    tensor: a captured graph needs both as tensors, or it repeats the numbers of its capture"""
+    lists = [params, grads, exp_avgs, exp_avg_sqs] + ([max_exp_avg_sqs] if max_exp_avg_sqs is not None else [])
+    lists = [list(x) for x in lists]
+    n = len(lists[0])
+    if any(len(x) != n for x in lists):
+        raise ValueError(f"adamw_step: lists of {[len(x) for x in lists]} tensors")
+    if n == 0:
+        return
+    dev_step, dev_lr = isinstance(step, torch.Tensor), isinstance(lr, torch.Tensor)
+    if dev_step and (step.dtype != torch.int64 or step.numel() != 1) or dev_lr and (lr.dtype != torch.float32 or lr.numel() != 1):
+        raise ValueError("adamw_step: a step tensor is one int64, a learning rate tensor one float32")
+    if not dev_step and int(step) < 1:
+        raise ValueError(f"adamw_step: step {step}: the first is 1")
+    b1, b2 = (float(b) for b in betas)
+    if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0 and weight_decay >= 0 and (dev_lr or lr >= 0)):
+        raise ValueError(f"adamw_step: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
+    sizes = [t.numel() for t in lists[0]]
+    types = [t.dtype for t in lists[0]]
+    for x, kind in zip(lists, ("params", "grads", "exp_avgs", "exp_avg_sqs", "max_exp_avg_sqs")):
+        if [t.numel() for t in x] != sizes:
+            raise ValueError(f"adamw_step: {kind} differ in size from params")
+        if not all([t.is_contiguous() for t in x]):
+            raise ValueError(f"adamw_step: {kind} must be contiguous")
+    if [t.dtype for t in lists[1]] != types or any(t not in _TOKEN_TYPES for t in set(types)):
+        raise TypeError("adamw_step: params and grads must be pairs of one type: float32, float16 or bfloat16")
+    if {t.dtype for x in lists[2:] for t in x} != {torch.float32}:
+        raise TypeError("adamw_step: the states must be float32")
+    where = [t.get_device() for t in lists[0]]
+    if min(where) < 0 or any([t.get_device() for t in x] != where for x in lists[1:]):
+        raise ValueError("adamw_step: a parameter, its gradient and its states must be on one GPU (there is no CPU fallback)")
+    if dev_step and step.get_device() not in where or dev_lr and lr.get_device() not in where or (dev_step or dev_lr) and len(set(where)) > 1:
+        raise ValueError("adamw_step: step and learning rate tensors must be on the GPU of the parameters")
+    table = np.zeros((n, 6), np.int64)  # sa_adamw_tensor
+    for j, x in enumerate(lists):
+        table[:, j] = [t.data_ptr() for t in x]
+    table[:, 5] = sizes
+    if len(set(table[table[:, 5] > 0, 0].tolist())) != int((table[:, 5] > 0).sum()):
+        raise ValueError("adamw_step: the same parameter twice")
+    groups = {}
+    if len(set(types)) == 1 and len(set(where)) == 1:
+        groups[types[0], where[0]] = table
+    else:
+        for i, key in enumerate(zip(types, where)):
+            groups.setdefault(key, []).append(i)
+        groups = {key: np.ascontiguousarray(table[rows]) for key, rows in groups.items()}
+    for (dtype, index), t in groups.items():
+        _launch("sa_adamw_step", torch.device("cuda", index), t.ctypes.data, len(t), _TOKEN_TYPES[dtype], int(len(lists) == 5),
+                0.0 if dev_lr else float(lr), lr.data_ptr() if dev_lr else None, b1, b2, float(eps), float(weight_decay),
+                1 if dev_step else int(step), step.data_ptr() if dev_step else None)
