@@ -748,6 +748,15 @@ int sa_cross_attention(const void* q, const void* k, const void* v, int dtype, i
                        const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, const int64_t* mask_strides,
                        float scale, void* out, float* lse, void* workspace, size_t workspace_bytes, sa_stream_t stream);
 
+/* Gradients of sa_cross_attention from its out and lse and from dout [B,Tq,Hq,D] (dout_strides: HOST, batch, token, head) ->
+ * dq [B,Tq,Hq,D], dk and dv [B,Tk,Hkv,D], contiguous; shared heads are summed; hidden keys and rows that see none get zeros. No
+ * atomics: the same call gives the same bits. workspace: sa_cross_attention_backward_workspace bytes. */
+size_t sa_cross_attention_backward_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D);
+int sa_cross_attention_backward(const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D,
+                                const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, const int64_t* mask_strides,
+                                float scale, const void* out, const float* lse, const void* dout, const int64_t* dout_strides, void* dq,
+                                void* dk, void* dv, void* workspace, size_t workspace_bytes, sa_stream_t stream);
+
 /* One AdamW step over n tensors of one type, in place (decoupled decay; 32-bit states and arithmetic; a 16-bit parameter is rounded once):
  *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  [vmax = max(vmax, v)];  p = p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v | vmax)/sqrt(1-b2^t) + eps)
  *   tensors    HOST array; its addresses travel in the launches' arguments (64 tensors a launch): nothing is kept after the call

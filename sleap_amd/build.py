@@ -42,6 +42,7 @@ SOURCES = [
     ("rotary.hip", NO_PACKED_F32),
     # -fno-honor-nans: a maximum is one instruction (else each carries two that quiet signalling NaNs); NaNs still pass the arithmetic
     ("attention.hip", ["-fno-honor-nans"] + NO_PACKED_F32),
+    ("attention_bwd.hip", ["-fno-honor-nans"] + NO_PACKED_F32),
     ("adamw.hip", NO_PACKED_F32),
 ]
 COMMON = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function"]

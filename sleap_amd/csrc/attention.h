@@ -20,6 +20,8 @@
 #include "sa_common.h"
 #include "token_types.h"
 
+#include <algorithm>
+
 namespace sa {
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -165,5 +167,9 @@ struct AttnShape {
   float c;                                     // scale * log2(e)
   float scale;
 };
+
+// checks a call's shape and fills `a` (attention.hip)
+int attention_shape(const char* who, AttnShape* a, const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq,
+                    int Hkv, int D, const int64_t* strides, const int32_t* lengths, const uint8_t* mask, const int64_t* mask_strides, float scale);
 
 }  // namespace sa

@@ -1,0 +1,511 @@
+// Gradients of cross attention. With w = softmax (from the stored logarithms of its denominators, not kept), dw = do v^T,
+// ds = w (dw - rowsum(do * out)):
+//     dv = w^T do        dk = scale ds^T q        dq = scale ds k
+// Two kernels, both without atomics, so that sums have one order: one whose waves own keys and walk the rows (dk, dv: four products),
+// one whose waves own rows and walk the keys (dq: three). A combined kernel would save two of the seven products and need
+// atomics or a float32 dq read and written once per run of keys. Shared heads are rows like any others (attention.h): dk and dv sum
+// over them by themselves. Few rows or few keys: runs of the walked side go to several workgroups, and a last kernel adds them in order.
+#include "attention.h"
+
+namespace {
+
+using namespace sa;
+
+struct BwdParams {
+  AttnShape a;
+  const void *out, *dout;
+  int64_t ob, ot, oh;       // strides of dout
+  const float* lse;         // [B, Hq, Tq]
+  float *lse2, *delta;      // [B * Hkv][R]: log2 of the denominator less LIFT; rowsum(do * out)
+  void *dq, *dk, *dv;       // contiguous
+  float *part_dq, *part_dk, *part_dv;  // [splits] of the whole gradient each, or NULL
+  uint32_t blocks, tiles, splits;      // tiles: workgroups along the owned side
+  int run;                  // rows (keys) of a run: a multiple of TILE
+  FastDiv div_tiles, div_splits, div_heads, div_hq;
+};
+
+// w is rounded to 16 bits for w^T do, ds for the other two. bf16 has the range of float32. fp16 has not: w moves up by 2^14 (held down to
+// 2^-38), and ds by a power of two of each column that follows its largest value so far (Range16 below).
+template <typename E>
+struct Lift {
+  static constexpr float LOG = 0.0f, BACK = 1.0f;
+};
+template <>
+struct Lift<_Float16> {
+  static constexpr float LOG = 14.0f, BACK = 1.0f / 16384.0f;
+};
+
+// power of two that a column's ds is multiplied with before it is rounded; never grows, so sums are rescaled a few times at most
+template <typename E>
+struct Range16 {
+  __device__ __forceinline__ void follow(f32x16&, f32x16*, int) {}
+  __device__ __forceinline__ float back() const { return 1.0f; }
+};
+template <>
+struct Range16<_Float16> {
+  float up = 0x1p100f;
+  __device__ __forceinline__ void follow(f32x16& ds, f32x16* acc, int n) {
+    float top = fabsf(ds[0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, fabsf(ds[i]));
+    top = max_halves(top);
+    if (__any(top * up > 0x1p15f)) {
+      const int e = __builtin_amdgcn_frexp_expf(top);  // top < 2^e
+      const float to = top * up > 0x1p15f ? __builtin_amdgcn_ldexpf(1.0f, min(13 - e, 100)) : up;
+      const float r = to / up;
+      up = to;
+      for (int db = 0; db < n; ++db) acc[db] *= r;
+    }
+    ds *= up;
+  }
+  __device__ __forceinline__ float back() const { return 1.0f / up; }
+};
+
+template <typename E>
+__global__ __launch_bounds__(256) void attention_stats_kernel(const BwdParams p, uint32_t total) {
+  const AttnShape& a = p.a;
+  const uint32_t i = blockIdx.x * 16 + (threadIdx.x >> 4);  // 16 lanes of 8 values a row
+  const uint32_t ic = min(i, total - 1);
+  const uint32_t bt = div_by(ic, p.div_hq), hh = ic - bt * a.Hq;
+  const uint32_t b = bt / a.Tq, t = bt - b * a.Tq;
+  const int d = (threadIdx.x & 15) * 8;
+  float sum = 0.0f;
+  if (d < a.D) {
+    union {
+      s16x8 v;
+      E e[8];
+    } x, y;
+    x.v = *reinterpret_cast<const s16x8*>(static_cast<const E*>(p.out) + (int64_t)ic * a.D + d);
+    y.v = *reinterpret_cast<const s16x8*>(static_cast<const E*>(p.dout) + (int64_t)b * p.ob + (int64_t)t * p.ot + (int64_t)hh * p.oh + d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += to_f32(x.e[e]) * to_f32(y.e[e]);
+  }
+#pragma unroll
+  for (int w = 8; w; w >>= 1) sum += __shfl_xor(sum, w);
+  if (i < total && (threadIdx.x & 15) == 0) {
+    const float l = p.lse[((int64_t)b * a.Hq + hh) * a.Tq + t];
+    const int64_t at = ((int64_t)b * a.Hkv + hh / a.G) * a.R + (int64_t)t * a.G + hh % a.G;
+    p.lse2[at] = l == -INFINITY ? INFINITY : l * LOG2E - Lift<E>::LOG;
+    p.delta[at] = sum;
+  }
+}
+
+// rows r0 .. r0 + 63 of q and dout into two tiles
+template <int DP, int NW>
+struct RowCopy {
+  static constexpr int N = (Tile<DP>::PIECES + NW - 1) / NW;
+  int row[N];
+  uint32_t col[N];
+  __device__ __forceinline__ void init(int wave, int lane, int D) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int at = (wave + j * NW) * 1024 + lane * 16;
+      row[j] = at / Tile<DP>::ROW;
+      const int c = ((at >> 4) & (DP / 8 - 1)) ^ swizzle<DP>(row[j]);
+      col[j] = c * 8 < D ? c * 16 : OUT_OF_RANGE;
+    }
+  }
+  template <typename E>
+  __device__ __forceinline__ void issue(char* lds, const BwdParams& p, const E* q, const E* dout, uint32_t r0, uint32_t end, int wave) const {
+    const AttnShape& a = p.a;
+    const uint32_t t0 = __builtin_amdgcn_readfirstlane(div_by(r0, a.div_g));
+    const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(q + (int64_t)t0 * a.qt), 0, 0x7FFFFFFF, 0x00020000);
+    const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(dout + (int64_t)t0 * p.ot), 0, 0x7FFFFFFF, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (Tile<DP>::PIECES % NW != 0 && wave + j * NW >= Tile<DP>::PIECES) break;
+      const uint32_t r = r0 + row[j], t = div_by(r, a.div_g), g = r - t * a.G;
+      const bool in = r < end && col[j] != OUT_OF_RANGE;
+      const uint32_t oq = in ? 2 * ((t - t0) * (uint32_t)a.qt + g * (uint32_t)a.qh) + col[j] : OUT_OF_RANGE;
+      const uint32_t oo = in ? 2 * ((t - t0) * (uint32_t)p.ot + g * (uint32_t)p.oh) + col[j] : OUT_OF_RANGE;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (lds_ptr)(lds + (wave + j * NW) * 1024), 16, oq, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ro, (lds_ptr)(lds + Tile<DP>::BYTES + (wave + j * NW) * 1024), 16, oo, 0, 0, 0);
+    }
+  }
+};
+
+template <typename E>
+__device__ __forceinline__ void store_column(E* dst, float* part, const f32x16* acc, int n, int D, int h, float by) {
+  for (int db = 0; db < n; ++db)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = db * 32 + j * 8 + h * 4;
+      if (d >= D) continue;
+      const f32x4 v = {acc[db][4 * j] * by, acc[db][4 * j + 1] * by, acc[db][4 * j + 2] * by, acc[db][4 * j + 3] * by};
+      if (part) *reinterpret_cast<f32x4*>(part + d) = v;
+      else *reinterpret_cast<u32x2*>(dst + d) = u32x2{pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3])};
+    }
+}
+
+// dk, dv: a wave owns 32 keys (k and v in registers) and walks rows in tiles of 64
+template <typename E, int DB, int NW>
+__global__ __launch_bounds__(NW * 64, DB == 4 ? 1 : 2) void attention_dkv_kernel(const BwdParams p) {
+  constexpr int DP = DB == 3 ? 128 : DB * 32, KS = DB * 2;
+  using T = Tile<DP>;
+  constexpr int STAGE = 2 * T::BYTES + 2 * TILE * 4;  // q, dout, lse2, delta
+  extern __shared__ __align__(1024) char lds[];
+  const AttnShape& a = p.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+  const uint32_t id = xcd_run(blockIdx.x, p.blocks);
+  const uint32_t bhs = div_by(id, p.div_tiles), tile = id - bhs * p.tiles;
+  const uint32_t bh = div_by(bhs, p.div_splits), split = bhs - bh * p.splits;
+  const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv;
+
+  int length = a.Tk;
+  if (a.lengths) length = min(max(a.lengths[b], 0), a.Tk);
+  const int key0 = (int)tile * (NW * 32), key = key0 + wave * 32 + n;
+  bool seen = key < length;
+  if (seen && a.mask) seen = a.mask[(int64_t)b * a.mb + (int64_t)key * a.mt] != 0;
+  s16x8 kf[KS], vf[KS];
+  {
+    const E* ks_ = static_cast<const E*>(a.k) + (int64_t)b * a.kb + (int64_t)hk * a.kh + (int64_t)key * a.kt;
+    const E* vs_ = static_cast<const E*>(a.v) + (int64_t)b * a.vb + (int64_t)hk * a.vh + (int64_t)key * a.vt;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = ks * 16 + h * 8;
+      const bool in = seen && d < a.D;
+      kf[ks] = in ? *reinterpret_cast<const s16x8*>(ks_ + d) : s16x8{};
+      vf[ks] = in ? *reinterpret_cast<const s16x8*>(vs_ + d) : s16x8{};
+    }
+  }
+  const uint32_t first = split * (uint32_t)p.run, end = min(first + (uint32_t)p.run, a.R);
+  const int tiles = key0 < length && first < end ? (int)((end - first + TILE - 1) / TILE) : 0;  // no visible key in this tile: nothing to walk
+  const E* qbase = static_cast<const E*>(a.q) + (int64_t)b * a.qb + (int64_t)(hk * a.G) * a.qh;
+  const E* obase = static_cast<const E*>(p.dout) + (int64_t)b * p.ob + (int64_t)(hk * a.G) * p.oh;
+  RowCopy<DP, NW> rc;
+  rc.init(wave, lane, a.D);
+  auto copy = [&](int i) {
+    char* s = lds + (i & 1) * STAGE;
+    const uint32_t r0 = first + (uint32_t)i * TILE;
+    rc.template issue<E>(s, p, qbase, obase, r0, end, wave);
+    if (wave == 0) {
+      const int64_t at = (int64_t)bh * a.R + r0;
+      const uint32_t o = r0 + lane < end ? lane * 4 : OUT_OF_RANGE;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(p.lse2 + at, 0, 0x7FFFFFFF, 0x00020000), (lds_ptr)(s + 2 * T::BYTES), 4, o, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(p.delta + at, 0, 0x7FFFFFFF, 0x00020000), (lds_ptr)(s + 2 * T::BYTES + TILE * 4), 4, o, 0, 0, 0);
+    }
+  };
+  int oa[KS], ot[DB];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) oa[ks] = T::off_a(n, h, ks);
+#pragma unroll
+  for (int db = 0; db < DB; ++db) ot[db] = T::off_t(lane, db);
+
+  f32x16 dk[DB] = {}, dv[DB] = {};
+  Range16<E> range;
+  if (tiles) copy(0);
+  for (int i = 0; i < tiles; ++i) {
+    tile_barrier();
+    if (i + 1 < tiles) copy(i + 1);
+    const char* qt = lds + (i & 1) * STAGE;
+    const char* dt = qt + T::BYTES;
+    const float* stat = reinterpret_cast<const float*>(qt + 2 * T::BYTES) + 4 * h;
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s = Mfma<E>::run(read_a(qt, oa[ks] + blk * 32 * T::ROW), kf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) dp = Mfma<E>::run(read_a(dt, oa[ks] + blk * 32 * T::ROW), vf[ks], dp);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 l = *reinterpret_cast<const f32x4*>(stat + blk * 32 + 8 * j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * j + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], a.c, -l[e]));
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        const s16x8 w = pack8<E>(s, s2);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) dv[db] = Mfma<E>::run(read_t(dt, ot[db] + (blk * 2 + s2) * 16 * T::ROW, 8 * T::ROW), w, dv[db]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 l = *reinterpret_cast<const f32x4*>(stat + TILE + blk * 32 + 8 * j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * j + e] = s[4 * j + e] * (dp[4 * j + e] - l[e]);
+      }
+      range.follow(dp, dk, DB);
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        const s16x8 w = pack8<E>(dp, s2);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) dk[db] = Mfma<E>::run(read_t(qt, ot[db] + (blk * 2 + s2) * 16 * T::ROW, 8 * T::ROW), w, dk[db]);
+      }
+    }
+  }
+  if (key >= a.Tk) return;
+  if (!seen) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
+  }
+  const int64_t at = (((int64_t)b * a.Tk + key) * a.Hkv + hk) * a.D;
+  const int64_t whole = (int64_t)(p.blocks / (p.tiles * p.splits)) * a.Tk * a.D;
+  store_column<E>(static_cast<E*>(p.dk) + at, p.part_dk ? p.part_dk + split * whole + at : nullptr, dk, DB, a.D, h, a.scale * Lift<E>::BACK * range.back());
+  store_column<E>(static_cast<E*>(p.dv) + at, p.part_dv ? p.part_dv + split * whole + at : nullptr, dv, DB, a.D, h, Lift<E>::BACK);
+}
+
+// dq: a wave owns 32 rows (q and dout in registers) and walks keys in tiles of 64
+template <typename E, int DB, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void attention_dq_kernel(const BwdParams p) {
+  constexpr int DP = DB == 3 ? 128 : DB * 32, KS = DB * 2;
+  using T = Tile<DP>;
+  extern __shared__ __align__(1024) char lds[];
+  const AttnShape& a = p.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+  const uint32_t id = xcd_run(blockIdx.x, p.blocks);
+  const uint32_t bhs = div_by(id, p.div_tiles), tile = id - bhs * p.tiles;
+  const uint32_t bh = div_by(bhs, p.div_splits), split = bhs - bh * p.splits;
+  const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv;
+
+  const uint32_t row = tile * (NW * 32) + wave * 32 + n;
+  const bool real = row < a.R;
+  const uint32_t rr = real ? row : a.R - 1, t = div_by(rr, a.div_g), g = rr - t * a.G;
+  s16x8 qf[KS], df[KS];
+  {
+    const E* q = static_cast<const E*>(a.q) + (int64_t)b * a.qb + (int64_t)t * a.qt + (int64_t)(hk * a.G + g) * a.qh;
+    const E* o = static_cast<const E*>(p.dout) + (int64_t)b * p.ob + (int64_t)t * p.ot + (int64_t)(hk * a.G + g) * p.oh;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = ks * 16 + h * 8;
+      qf[ks] = d < a.D ? *reinterpret_cast<const s16x8*>(q + d) : s16x8{};
+      df[ks] = d < a.D ? *reinterpret_cast<const s16x8*>(o + d) : s16x8{};
+    }
+  }
+  const float lse2 = p.lse2[(int64_t)bh * a.R + rr], delta = p.delta[(int64_t)bh * a.R + rr];
+  int length = a.Tk;
+  if (a.lengths) length = min(max(a.lengths[b], 0), a.Tk);
+  const int first = (int)split * p.run, end = min(first + p.run, length);
+  const int tiles = end > first ? (end - first + TILE - 1) / TILE : 0;
+  const E* kbase = static_cast<const E*>(a.k) + (int64_t)b * a.kb + (int64_t)hk * a.kh;
+  const E* vbase = static_cast<const E*>(a.v) + (int64_t)b * a.vb + (int64_t)hk * a.vh;
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mb : nullptr;
+  TileCopy<DP, NW> ck, cv;
+  ck.init(wave, lane, a.kt * 2, a.D);
+  cv.init(wave, lane, a.vt * 2, a.D);
+  auto load_mask = [&](int i) -> uint8_t {
+    const int key = first + i * TILE + lane;
+    return mask && key < end ? mask[(int64_t)key * a.mt] : 1;
+  };
+  auto seen_of = [&](int i, uint8_t m) { return __ballot(first + i * TILE + lane < end && m); };
+  auto copy = [&](int i, uint64_t seen) {
+    char* s = lds + (i & 1) * 2 * T::BYTES;
+    const int64_t key = first + (int64_t)i * TILE;
+    ck.issue(s, kbase + key * a.kt, seen, wave);
+    cv.issue(s + T::BYTES, vbase + key * a.vt, seen, wave);
+  };
+  int oa[KS], ot[DB];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) oa[ks] = T::off_a(n, h, ks);
+#pragma unroll
+  for (int db = 0; db < DB; ++db) ot[db] = T::off_t(lane, db);
+
+  f32x16 dq[DB] = {};
+  Range16<E> range;
+  uint64_t seen = 0;
+  uint8_t next_mask = 1;
+  if (tiles) {
+    seen = seen_of(0, load_mask(0));
+    copy(0, seen);
+    next_mask = load_mask(1);
+  }
+  for (int i = 0; i < tiles; ++i) {
+    tile_barrier();
+    const uint64_t now = seen;
+    if (i + 1 < tiles) {
+      seen = seen_of(i + 1, next_mask);
+      copy(i + 1, seen);
+      next_mask = load_mask(i + 2);
+    }
+    if (now == 0) continue;
+    const char* kt = lds + (i & 1) * 2 * T::BYTES;
+    const char* vt = kt + T::BYTES;
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s = Mfma<E>::run(read_a(kt, oa[ks] + blk * 32 * T::ROW), qf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) dp = Mfma<E>::run(read_a(vt, oa[ks] + blk * 32 * T::ROW), df[ks], dp);
+      if (now != ~0ull) hide(s, (uint32_t)(now >> (32 * blk)), h, -INFINITY);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dp[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.c, -lse2)) * (dp[e] - delta);
+      range.follow(dp, dq, DB);
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        const s16x8 w = pack8<E>(dp, s2);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) dq[db] = Mfma<E>::run(read_t(kt, ot[db] + (blk * 2 + s2) * 16 * T::ROW, 8 * T::ROW), w, dq[db]);
+      }
+    }
+  }
+  if (!real) return;
+  const int64_t at = (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D;
+  const int64_t whole = (int64_t)(p.blocks / (p.tiles * p.splits)) * a.R * a.D;
+  store_column<E>(static_cast<E*>(p.dq) + at, p.part_dq ? p.part_dq + split * whole + at : nullptr, dq, DB, a.D, h, a.scale * Lift<E>::BACK * range.back());
+}
+
+// adds the runs' gradients, in their order; a thread has 8 values
+template <typename E>
+__global__ __launch_bounds__(256) void attention_add_kernel(const float* part, E* dst, int64_t n, int splits) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (i >= n) return;
+  f32x4 x = {}, y = {};
+  for (int s = 0; s < splits; ++s) {
+    const f32x4* src = reinterpret_cast<const f32x4*>(part + s * n + i);
+    x += src[0];
+    y += src[1];
+  }
+  *reinterpret_cast<u32x4*>(dst + i) = u32x4{pack2<E>(x[0], x[1]), pack2<E>(x[2], x[3]), pack2<E>(y[0], y[1]), pack2<E>(y[2], y[3])};
+}
+
+// How one of the two kernels is cut: `own` rows (keys) among waves of 32, `walk` keys (rows) among runs.
+struct Cut {
+  int waves;
+  uint32_t tiles, splits;
+  int run;
+};
+Cut cut(uint64_t heads, uint64_t own, uint64_t walk) {
+  Cut c;
+  c.waves = own <= 32 ? 1 : own <= 64 ? 2 : 4;
+  c.tiles = (uint32_t)((own + c.waves * 32 - 1) / (c.waves * 32));
+  const uint64_t blocks = c.tiles * heads, want = 2048 / c.waves, walked = (walk + TILE - 1) / TILE;
+  uint64_t splits = blocks ? want / blocks : 1;
+  splits = std::max<uint64_t>(1, std::min(splits, walked / 4));
+  const uint64_t per = std::max<uint64_t>(1, (walked + splits - 1) / splits);
+  c.run = (int)(per * TILE);
+  c.splits = (uint32_t)std::max<uint64_t>(1, (walked + per - 1) / per);
+  return c;
+}
+
+struct Layout {
+  Cut kv, q;
+  size_t stats, dq, dkv;  // floats of each part of the workspace
+  size_t total() const { return 2 * stats + dq + 2 * dkv; }
+};
+Layout layout(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
+  Layout l;
+  const uint64_t R = (uint64_t)Tq * (Hq / Hkv);
+  l.kv = cut((uint64_t)B * Hkv, Tk, R);
+  l.q = cut((uint64_t)B * Hkv, R, Tk);
+  l.stats = ((size_t)B * Hq * Tq + 3) / 4 * 4;
+  l.dq = l.q.splits > 1 ? (size_t)l.q.splits * B * Hq * Tq * D : 0;
+  l.dkv = l.kv.splits > 1 ? (size_t)l.kv.splits * B * Hkv * Tk * D : 0;
+  return l;
+}
+
+void set(BwdParams& p, const Cut& c, uint64_t heads) {
+  p.blocks = (uint32_t)(c.tiles * c.splits * heads);
+  p.tiles = c.tiles;
+  p.splits = c.splits;
+  p.run = c.run;
+  p.div_tiles = fast_div(c.tiles);
+  p.div_splits = fast_div(c.splits);
+}
+
+template <typename E, int DB>
+void launch_kv(const BwdParams& p, int waves, hipStream_t s) {
+  constexpr size_t lds = 2 * (2 * Tile<DB == 3 ? 128 : DB * 32>::BYTES + 2 * TILE * 4);
+  auto go = [&](auto kernel) {
+    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    kernel<<<dim3(p.blocks), dim3(waves * 64), lds, s>>>(p);
+  };
+  if (waves == 1) go(attention_dkv_kernel<E, DB, 1>);
+  else if (waves == 2) go(attention_dkv_kernel<E, DB, 2>);
+  else go(attention_dkv_kernel<E, DB, 4>);
+}
+
+template <typename E, int DB>
+void launch_q(const BwdParams& p, int waves, hipStream_t s) {
+  constexpr size_t lds = 4 * Tile<DB == 3 ? 128 : DB * 32>::BYTES;
+  if (waves == 1) attention_dq_kernel<E, DB, 1><<<dim3(p.blocks), dim3(64), lds, s>>>(p);
+  else if (waves == 2) attention_dq_kernel<E, DB, 2><<<dim3(p.blocks), dim3(128), lds, s>>>(p);
+  else attention_dq_kernel<E, DB, 4><<<dim3(p.blocks), dim3(256), lds, s>>>(p);
+}
+
+template <typename E>
+int launch(BwdParams& p, const Layout& l, int B, hipStream_t s) {
+  const AttnShape& a = p.a;
+  const uint64_t heads = (uint64_t)B * a.Hkv;
+  const int db = (a.D + 31) / 32;
+  if (a.R) {
+    const uint32_t rows = (uint32_t)B * a.Hq * a.Tq;
+    attention_stats_kernel<E><<<dim3((rows + 15) / 16), dim3(256), 0, s>>>(p, rows);
+    SA_LAUNCH_CHECK();
+  }
+  if (a.Tk) {
+    set(p, l.kv, heads);
+    if (db == 1) launch_kv<E, 1>(p, l.kv.waves, s);
+    else if (db == 2) launch_kv<E, 2>(p, l.kv.waves, s);
+    else if (db == 3) launch_kv<E, 3>(p, l.kv.waves, s);
+    else launch_kv<E, 4>(p, l.kv.waves, s);
+    SA_LAUNCH_CHECK();
+    if (p.part_dk) {
+      const int64_t n = (int64_t)heads * a.Tk * a.D;
+      const dim3 grid((uint32_t)((n / 8 + 255) / 256));
+      attention_add_kernel<E><<<grid, dim3(256), 0, s>>>(p.part_dk, static_cast<E*>(p.dk), n, (int)l.kv.splits);
+      attention_add_kernel<E><<<grid, dim3(256), 0, s>>>(p.part_dv, static_cast<E*>(p.dv), n, (int)l.kv.splits);
+      SA_LAUNCH_CHECK();
+    }
+  }
+  if (a.R) {
+    set(p, l.q, heads);
+    if (db == 1) launch_q<E, 1>(p, l.q.waves, s);
+    else if (db == 2) launch_q<E, 2>(p, l.q.waves, s);
+    else if (db == 3) launch_q<E, 3>(p, l.q.waves, s);
+    else launch_q<E, 4>(p, l.q.waves, s);
+    SA_LAUNCH_CHECK();
+    if (p.part_dq) {
+      const int64_t n = (int64_t)heads * a.R * a.D;
+      attention_add_kernel<E><<<dim3((uint32_t)((n / 8 + 255) / 256)), dim3(256), 0, s>>>(p.part_dq, static_cast<E*>(p.dq), n, (int)l.q.splits);
+      SA_LAUNCH_CHECK();
+    }
+  }
+  return SA_OK;
+}
+
+}  // namespace
+
+extern "C" size_t sa_cross_attention_backward_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
+  if (B < 1 || Tq < 0 || Tk < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1) return 0;
+  return layout(B, Tq, Tk, Hq, Hkv, D).total() * sizeof(float);
+}
+
+extern "C" int sa_cross_attention_backward(const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq, int Hkv,
+                                           int D, const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask,
+                                           const int64_t* mask_strides, float scale, const void* out, const float* lse, const void* dout,
+                                           const int64_t* dout_strides, void* dq, void* dk, void* dv, void* workspace,
+                                           size_t workspace_bytes, sa_stream_t stream) {
+  const char* who = "sa_cross_attention_backward";
+  BwdParams p;
+  if (int rc = attention_shape(who, &p.a, q, k, v, dtype, B, Tq, Tk, Hq, Hkv, D, strides, key_lengths, key_mask, mask_strides, scale)) return rc;
+  if (B == 0) return SA_OK;
+  SA_REQUIRE((((uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) & 15) == 0, "%s: addresses are multiples of 16", who);
+  for (int i = 0; i < 3; ++i) SA_REQUIRE(dout_strides[i] >= 0 && dout_strides[i] % 8 == 0, "%s: strides are multiples of 8 elements", who);
+  const int64_t G = Hq / Hkv, far = 1ll << 30;
+  SA_REQUIRE(TILE * strides[1] + G * strides[2] < far && TILE * dout_strides[1] + G * dout_strides[2] < far,
+             "%s: 64 tokens and the heads on one key head span less than 2^30 elements of q and of dout", who);
+  const Layout l = layout(B, Tq, Tk, Hq, Hkv, D);
+  const uint64_t heads = (uint64_t)B * Hkv, most = 1ull << 31;
+  SA_REQUIRE((uint64_t)l.kv.tiles * l.kv.splits * heads < most && (uint64_t)l.q.tiles * l.q.splits * heads < most && (uint64_t)B * Hq * Tq < most - 1024,
+             "%s: too many rows", who);
+  if (workspace_bytes < l.total() * sizeof(float)) return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", who, workspace_bytes);
+  p.out = out;
+  p.dout = dout;
+  p.ob = dout_strides[0];
+  p.ot = dout_strides[1];
+  p.oh = dout_strides[2];
+  p.lse = lse;
+  p.dq = dq;
+  p.dk = dk;
+  p.dv = dv;
+  float* w = static_cast<float*>(workspace);
+  p.lse2 = w;
+  p.delta = w + l.stats;
+  p.part_dq = l.dq ? w + 2 * l.stats : nullptr;
+  p.part_dk = l.dkv ? w + 2 * l.stats + l.dq : nullptr;
+  p.part_dv = l.dkv ? w + 2 * l.stats + l.dq + l.dkv : nullptr;
+  p.div_heads = fast_div(Hkv);
+  p.div_hq = fast_div(Hq);
+  return dtype == SA_F16 ? launch<_Float16>(p, l, B, (hipStream_t)stream) : launch<__bf16>(p, l, B, (hipStream_t)stream);
+}

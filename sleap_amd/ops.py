@@ -562,6 +562,47 @@ def _attention_forward(q, k, v, keys, scale, want_lse):
     return out, lse
 
 
+_SPAN = 1 << 30  # elements that 64 tokens and the heads on one key head of q (and of dout) may span in the backward kernels
+
+
+def _spans(t, group):
+    s = _strides(t, 3)
+    return t if 64 * s[1] + group * s[2] < _SPAN else t.clone(memory_format=torch.contiguous_format)
+
+
+def _attention_backward(dout, q, k, v, out, lse, keys, scale):
+    group = q.shape[2] // k.shape[2]
+    q, k, v = _spans(_laid_out(q, 8), group), _laid_out(k, 8, _KEY_STRIDE), _laid_out(v, 8, _KEY_STRIDE)
+    dout, out, lse = _spans(_laid_out(dout, 8), group), _laid_out(out.contiguous(), 8), lse.contiguous()
+    B, Tq, H, D = q.shape
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    if dq.numel() or dk.numel():
+        ws, ws_args = _workspace("sa_cross_attention_backward_workspace", q.device, B, Tq, k.shape[1], H, k.shape[2], D)
+        _launch("sa_cross_attention_backward", q.device, *_attention_args(q, k, v), *keys.args(), scale, out.data_ptr(), lse.data_ptr(),
+                dout.data_ptr(), _i64(_strides(dout, 3)), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *ws_args)
+    return dq, dk, dv
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, mask, scale):
+        keys = _Keys.__new__(_Keys)
+        keys.lengths, keys.mask = lengths, mask
+        out, lse = _attention_forward(q, k, v, keys, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, lengths, mask)
+        ctx.scale = scale
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _):
+        q, k, v, out, lse, lengths, mask = ctx.saved_tensors
+        keys = _Keys.__new__(_Keys)
+        keys.lengths, keys.mask = lengths, mask
+        return (*_attention_backward(dout, q, k, v, out, lse, keys, ctx.scale), None, None, None)
+
+
 def _attention_checks(who, q, k, v, key_lengths, key_mask, scale):
     _cuda_tensors(who, q=q, k=k, v=v, key_lengths=key_lengths, key_mask=key_mask)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
@@ -592,7 +633,8 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, return
     type before the product with v; results do not depend on the order in which workgroups run. Differentiable in q, k and v, once."""
     keys, scale = _attention_checks("cross_attention", q, k, v, key_lengths, key_mask, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        raise NotImplementedError("cross_attention: no gradient yet; call it under torch.no_grad()")
+        out, lse = _CrossAttention.apply(q, k, v, keys.lengths, keys.mask, scale)
+        return (out, lse) if return_lse else out
     out, lse = _attention_forward(q, k, v, keys, scale, return_lse)
     return (out, lse) if return_lse else out
 
