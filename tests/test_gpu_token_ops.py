@@ -1,0 +1,538 @@
+"""Rotary positions, cross attention and AdamW on the device against their 64-bit definitions (tests/token_oracle.py)."""
+import math
+
+import pytest
+import torch
+
+from tests import token_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def rng(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def normal(g, *shape, dtype=torch.float16, scale=1.0):
+    return (torch.randn(shape, generator=g, device=DEV) * scale).to(dtype)
+
+
+# --------------------------------------------------------------------------------------------------
+# rotary positions
+# --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("B,T,H,D,sections,ladder", [
+    (1, 1, 1, 2, (1,), "axis"), (1, 52, 8, 64, (16, 16), "axis"), (2, 333, 3, 80, (8, 15, 13), "shared"), (3, 17, 5, 34, (4, 0, 3), "axis"),
+    (2, 100, 2, 128, (24, 20, 20), "axis"), (1, 2050, 1, 50, (2, 3, 5), "shared"), (2, 65, 7, 256, (128,), "axis"), (1, 31, 4, 300, (1, 1, 1, 1), "axis")])
+def test_rotary_matches_its_definition(dtype, interleaved, B, T, H, D, sections, ladder):
+    from sleap_amd import ops
+
+    g = rng(T * D)
+    x = normal(g, B, T, H, D, dtype=dtype)
+    for positions in (torch.randint(-50, 2_000_000, (T, len(sections)), generator=g, device=DEV, dtype=torch.int32),
+                      torch.randint(0, 100_000_000, (B, T, len(sections)), generator=g, device=DEV),
+                      torch.rand((B, T, len(sections)), generator=g, device=DEV) * 1024):
+        y = ops.rotary_axes(x, positions, sections, ladder=ladder, interleaved=interleaved)
+        assert y.dtype == dtype and y.is_contiguous()
+        assert oracle.worst(y, oracle.rotary(x, positions, sections, ladder=ladder, interleaved=interleaved)) <= 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_takes_any_layout(dtype, interleaved):
+    from sleap_amd import ops
+
+    g = rng(3)
+    B, T, H, D, sections = 2, 37, 4, 48, (8, 8)
+    p = torch.rand((T, 2, 2), generator=g, device=DEV)[..., 1] * 300  # strided positions
+    base = normal(g, B, H, T + 3, D + 9, dtype=dtype)
+    for x in (base[..., :T, :D].transpose(1, 2), base[..., 3:, 9:].transpose(1, 2), base[..., 1:T + 1, 1:D + 1].transpose(1, 2),
+              base[..., :T, :D].transpose(1, 2)[:, :, :1].expand(B, T, H, D), base[:1, :, :T, :D].transpose(1, 2).expand(B, T, H, D),
+              normal(g, B, T, D, H, dtype=dtype).transpose(2, 3), normal(g, B * T * H * D + 1, dtype=dtype)[1:].view(B, T, H, D)):
+        y = ops.rotary_axes(x, p, sections, theta=500.0, interleaved=interleaved)
+        assert oracle.worst(y, oracle.rotary(x, p, sections, 500.0, interleaved=interleaved)) <= 1
+
+
+def test_rotary_gradient_is_the_inverse_turn():
+    from sleap_amd import ops
+
+    g = rng(4)
+    x = normal(g, 2, 45, 3, 40, dtype=torch.float32).requires_grad_(True)
+    p = torch.randint(0, 5000, (2, 45, 3), generator=g, device=DEV)
+    dy = normal(g, 2, 45, 3, 40, dtype=torch.float32)
+    y = ops.rotary_axes(x, p, (5, 6, 4))
+    (dx,) = torch.autograd.grad(y, x, dy, create_graph=True)
+    assert oracle.worst(dx, oracle.rotary(dy, p, (5, 6, 4), inverse=True)) <= 1
+    back = ops.rotary_axes(y.detach(), p, (5, 6, 4), inverse=True)
+    assert torch.allclose(back, x, atol=4e-6)  # two turns of 1e-6 (|a| + |b|)
+    # differences: <dx, d> against (y(x + h d) - y(x - h d)) . dy / 2h in 64 bits; linear in x, so any h does
+    d = normal(g, *x.shape, dtype=torch.float32)
+    plus, minus = (oracle.rotary(x.detach() + s * d, p, (5, 6, 4))[0] for s in (1, -1))
+    want = ((plus - minus) * dy.double()).sum() / 2
+    assert abs((dx.double() * d.double()).sum() - want) <= 2e-6 * (dy.double().abs() * d.double().abs()).sum() * 2
+    # a second gradient: d/d(dy) of <dx, d>
+    dy2 = dy.clone().requires_grad_(True)
+    (dx2,) = torch.autograd.grad(ops.rotary_axes(x, p, (5, 6, 4)), x, dy2, create_graph=True)
+    (again,) = torch.autograd.grad((dx2 * d).sum(), dy2)
+    assert oracle.worst(again, oracle.rotary(d, p, (5, 6, 4))) <= 1
+
+
+@pytest.mark.parametrize("B,T", [(0, 5), (3, 0)])
+def test_rotary_of_nothing(B, T):
+    from sleap_amd import ops
+
+    assert ops.rotary_axes(torch.empty((B, T, 2, 8), device=DEV), torch.empty((T, 1), device=DEV), (4,)).shape == (B, T, 2, 8)
+
+
+def test_rotary_of_a_bad_position_stays_in_its_token():
+    from sleap_amd import ops
+
+    x = normal(rng(5), 1, 9, 2, 16, dtype=torch.float32)
+    p = torch.arange(9, device=DEV, dtype=torch.float32)[:, None].clone()
+    p[4] = float("nan")
+    y = ops.rotary_axes(x, p, (4,))
+    assert torch.isnan(y[:, 4, :, :8]).all() and torch.equal(y[:, 4, :, 8:], x[:, 4, :, 8:])
+    assert torch.isfinite(y[:, [0, 1, 2, 3, 5, 6, 7, 8]]).all()
+
+
+# --------------------------------------------------------------------------------------------------
+# cross attention
+# --------------------------------------------------------------------------------------------------
+def make(g, B, Tq, Tk, H, K, D, dtype, ragged="none", scale=1.0):
+    q, k, v, dout = (normal(g, B, n, h, D, dtype=dtype, scale=s) for n, h, s in ((Tq, H, scale), (Tk, K, 1.0), (Tk, K, 1.0), (Tq, H, 1.0)))
+    lengths = mask = None
+    if "lengths" in ragged:
+        lengths = torch.randint(0, Tk + 1, (B,), generator=g, device=DEV, dtype=torch.int32)
+        lengths[:1] = Tk + 5  # counts as Tk
+        if B > 1:
+            lengths[1] = -3  # counts as 0
+    if "mask" in ragged:
+        mask = torch.rand((B, Tk), generator=g, device=DEV) < 0.6
+        if B > 2:
+            mask[2] = False
+    hidden = ~oracle.visible(B, Tk, lengths, mask, DEV)[:, :, None, None]
+    k.masked_fill_(hidden, float("nan"))
+    v.masked_fill_(hidden, float("inf"))
+    return q, k, v, dout, lengths, mask
+
+
+def check(q, k, v, dout, lengths=None, mask=None, scale=None):
+    from sleap_amd import ops
+
+    want = oracle.attention(q, k, v, lengths, mask, scale, dout)
+    out, lse = ops.cross_attention(q, k, v, key_lengths=lengths, key_mask=mask, scale=scale, return_lse=True)
+    assert out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()
+    far = {"out": oracle.worst(out, want["out"]), "lse": oracle.worst(lse, want["lse"])}
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    again = ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask, scale=scale)
+    assert torch.equal(again, out)
+    grads = torch.autograd.grad(again, leaves, dout)
+    for name, x in zip(("dq", "dk", "dv"), grads):
+        assert x.dtype == q.dtype
+        far[name] = oracle.worst(x, want[name])
+    assert max(far.values()) <= 1, far
+    return out, grads
+
+
+SHAPES = [(1, 1, 1, 1, 1, 8), (2, 1, 64, 2, 2, 16), (1, 7, 63, 4, 1, 24), (2, 33, 65, 3, 3, 32), (3, 64, 129, 2, 1, 40), (1, 65, 200, 6, 2, 64),
+          (2, 130, 97, 4, 4, 72), (1, 257, 300, 2, 2, 96), (2, 100, 130, 8, 2, 104), (1, 140, 333, 2, 1, 128), (3, 1, 1029, 8, 2, 128),
+          (1, 5, 2500, 2, 2, 64), (1, 1500, 40, 1, 1, 56), (4, 31, 31, 5, 5, 120), (2, 1, 0, 2, 2, 32), (2, 0, 9, 2, 2, 32), (0, 4, 9, 2, 2, 32)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ragged", ["none", "lengths", "mask", "lengths+mask"])
+@pytest.mark.parametrize("B,Tq,Tk,H,K,D", SHAPES)
+def test_attention_matches_its_definition(dtype, ragged, B, Tq, Tk, H, K, D):
+    check(*make(rng(B + Tq * Tk + D), B, Tq, Tk, H, K, D, dtype, ragged))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,Tq,Tk,H,K,D", [(2, 1000, 1100, 4, 2, 64), (1, 300, 5000, 2, 2, 128), (1, 3000, 320, 4, 1, 80), (16, 1, 4096, 8, 1, 128)])
+def test_attention_of_many_tiles(dtype, B, Tq, Tk, H, K, D):
+    check(*make(rng(7), B, Tq, Tk, H, K, D, dtype, "lengths+mask"))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("spread", [0.0, 8.0, 40.0])
+def test_attention_of_flat_and_of_steep_scores(dtype, spread):
+    """From uniform weights to a weight of one; the largest score comes first, last and in the middle of the keys."""
+    g = rng(8)
+    q, k, v, dout, _, _ = make(g, 1, 70, 700, 2, 2, 64, dtype, scale=spread)
+    check(q, k, v, dout)
+    at = torch.linspace(-1, 1, 700, device=DEV)[None, :, None, None]
+    for slope in (at, -at, 1 - at.abs()):
+        check(q, (k * 0.1 + slope).to(dtype), v, dout, scale=0.3)
+
+
+def test_half_precision_gradients_of_far_sizes():
+    """fp16 gradients of outputs scaled by 2^-14 and by 2^12, and of values that are large: ds leaves fp16's range both ways."""
+    q, k, v, dout, lengths, mask = make(rng(9), 2, 90, 1200, 4, 2, 64, torch.float16, "lengths")
+    for scale in (2.0 ** -10, 1.0, 2.0 ** 9):
+        check(q, k, v, (dout * scale).to(torch.float16), lengths, mask)
+    rows = torch.logspace(-4, 3, 90, device=DEV)[None, :, None, None]
+    check(q, k, v, (dout * rows).to(torch.float16), lengths, mask)
+    check(q, k, v, (dout * rows.flip(1)).to(torch.float16), lengths, mask)
+
+
+def test_attention_takes_any_layout():
+    g = rng(10)
+    B, Tq, Tk, H, K, D = 2, 50, 90, 4, 2, 40
+    dtype = torch.bfloat16
+    packed = normal(g, B, Tk, 2, K, D, dtype=dtype)
+    q = normal(g, B, H, Tq, D, dtype=dtype).transpose(1, 2)  # heads first
+    dout = normal(g, B, 1, H, D, dtype=dtype).expand(B, Tq, H, D)
+    check(q, packed[:, :, 0], packed[:, :, 1], dout)
+    wide = normal(g, B, Tk, K, D + 3, dtype=dtype)
+    check(q, wide[..., 3:], wide[..., :D], dout)                                # addresses and strides of odd values
+    check(q, packed[:1, :, 0].expand(B, Tk, K, D), packed[:, :1, 1].expand(B, Tk, K, D), dout)  # one image for all, one value for all
+    last = normal(g, B, Tk, D, K, dtype=dtype).transpose(2, 3)
+    check(normal(g, B, Tq, D, H, dtype=dtype).transpose(2, 3), last, last, dout)
+    mask = torch.rand((Tk, 2, B), generator=g, device=DEV) < 0.5
+    check(q, packed[:, :, 0], packed[:, :, 1], dout, mask=mask[:, 0].T)          # a strided mask
+    check(q, packed[:, :, 0], packed[:, :, 1], dout, mask=mask[:, 1, :1].T)      # one mask for all
+    check(q, packed[:, :, 0], packed[:, :, 1], dout, lengths=torch.tensor([[90, 1], [17, 1]], device=DEV)[:, 0])  # int64, strided
+
+
+def test_gradients_of_broadcast_inputs_are_summed():
+    from sleap_amd import ops
+
+    g = rng(11)
+    q, k, v, dout, _, _ = make(g, 3, 20, 40, 2, 2, 32, torch.bfloat16)
+    one = k[:1].clone().requires_grad_(True)
+    (d,) = torch.autograd.grad(ops.cross_attention(q, one.expand(3, -1, -1, -1), v), one, dout)
+    whole = k[:1].expand(3, -1, -1, -1).contiguous().requires_grad_(True)
+    (e,) = torch.autograd.grad(ops.cross_attention(q, whole, v), whole, dout)
+    assert torch.equal(d, e.sum(0, keepdim=True))
+
+
+def test_gradients_against_differences():
+    """The 64-bit loss along a direction, by central differences, against the kernels' gradients along it."""
+    from sleap_amd import ops
+
+    g = rng(12)
+    q, k, v, dout, lengths, mask = make(g, 2, 40, 100, 4, 2, 48, torch.float16, "lengths+mask")
+    k, v = (t.nan_to_num(0, 0, 0) for t in (k, v))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask), leaves, dout)
+    want = oracle.attention(q, k, v, lengths, mask, dout=dout)
+    for i, name in enumerate(("dq", "dk", "dv")):
+        d = torch.randn(leaves[i].shape, generator=g, device=DEV, dtype=torch.float64)
+        h, loss = 1e-4, []
+        for s in (1, -1):
+            x = [t.detach().double() for t in (q, k, v)]
+            x[i] = x[i] + s * h * d
+            y = torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+            seen = oracle.visible(2, 100, lengths, mask, DEV)
+            for b in range(2):
+                at = seen[b].nonzero()[:, 0]
+                for n in range(4 if len(at) else 0):
+                    y[b, :, n] = torch.softmax(x[0][b, :, n] @ x[1][b, at, n // 2].T / math.sqrt(48), -1) @ x[2][b, at, n // 2]
+            loss.append((y * dout.double()).sum())
+        slope = (loss[0] - loss[1]) / (2 * h)
+        assert abs((grads[i].double() * d).sum() - slope) <= (want[name][1] * d.abs()).sum() + 1e-5 * abs(slope)
+
+
+def test_what_a_visible_key_holds_is_seen():
+    """A NaN value reaches its head's outputs and no other's; an infinite key its rows."""
+    from sleap_amd import ops
+
+    q, k, v, _, _, _ = make(rng(13), 2, 40, 100, 4, 2, 32, torch.bfloat16)
+    v[1, 70, 1, 5] = float("nan")
+    out = ops.cross_attention(q, k, v)
+    bad = torch.isnan(out)
+    assert bad[1, :, 2:, 5].all() and bad.sum() == 40 * 2
+    k[0, 3, 0] = float("nan")
+    out, lse = ops.cross_attention(q, k, v, return_lse=True)
+    assert torch.isnan(out[0, :, :2]).all() and torch.isfinite(out[0, :, 2:]).all() and torch.isnan(lse[0, :2]).all()
+
+
+def test_rows_without_a_visible_key():
+    from sleap_amd import ops
+
+    q, k, v, dout, _, _ = make(rng(14), 3, 17, 130, 2, 1, 64, torch.float16)
+    lengths = torch.tensor([0, 130, 0], dtype=torch.int32, device=DEV)
+    k[0], v[0], k[2], v[2] = (float("nan"),) * 4
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out, lse = ops.cross_attention(*leaves, key_lengths=lengths, return_lse=True)
+    assert (out[[0, 2]] == 0).all() and (lse[[0, 2]] == -math.inf).all() and not lse.requires_grad
+    dout[0] = float("inf")
+    for x in torch.autograd.grad(out, leaves, dout):
+        assert (x[[0, 2]] == 0).all() and torch.isfinite(x).all() and x[1].abs().sum() > 0
+
+
+def test_the_same_call_gives_the_same_bits():
+    from sleap_amd import ops
+
+    for shape in ((1, 5, 9000, 2, 2, 64), (1, 9000, 70, 4, 1, 64)):  # runs of keys and of rows, joined
+        q, k, v, dout, _, _ = make(rng(15), *shape, torch.bfloat16)
+        leaves = [t.requires_grad_(True) for t in (q, k, v)]
+        first = None
+        for _ in range(3):
+            out = ops.cross_attention(*leaves)
+            got = [out, *torch.autograd.grad(out, leaves, dout)]
+            assert first is None or all(torch.equal(a, b) for a, b in zip(first, got))
+            first = got
+
+
+def test_keys_beyond_32_bit_offsets():
+    """Keys 128 Ki elements apart: the last lie 4.3 GB behind the first."""
+    from sleap_amd import ops
+
+    g, Tk, step = rng(16), 16500, 1 << 17
+    held = torch.empty((Tk, step), dtype=torch.bfloat16, device=DEV)
+    held[:, :64] = normal(g, Tk, 64, dtype=torch.bfloat16)
+    k = held[:, :32].view(1, Tk, 1, 32)
+    v = held[:, 32:64].view(1, Tk, 1, 32)
+    q = normal(g, 1, 3, 2, 32, dtype=torch.bfloat16)
+    near = ops.cross_attention(q, k.contiguous(), v.contiguous())
+    far = ops.cross_attention(q, k, v)
+    assert torch.equal(near, far)
+
+
+def test_attention_on_another_stream():
+    from sleap_amd import ops
+
+    q, k, v, dout, lengths, mask = make(rng(17), 2, 30, 700, 4, 2, 64, torch.float16, "lengths+mask")
+    want = oracle.attention(q, k, v, lengths, mask, dout=dout)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        leaves = [t.requires_grad_(True) for t in (q, k, v)]
+        out = ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask)
+        got = [out, *torch.autograd.grad(out, leaves, dout)]
+    torch.cuda.current_stream().wait_stream(side)
+    for name, x in zip(("out", "dq", "dk", "dv"), got):
+        assert oracle.worst(x.detach(), want[name]) <= 1
+
+
+def test_captured_calls_follow_their_inputs():
+    """Forward and backward in a graph each, replayed on new inputs with eager work between; each graph has its own scratch."""
+    from sleap_amd import ops
+
+    shape = (2, 24, 1300, 4, 2, 64)
+    graphs = []
+    for seed in (18, 19):
+        q, k, v, dout, _, _ = make(rng(seed), *shape, torch.bfloat16)
+        p = torch.randint(0, 1000, (24, 2), generator=rng(seed), device=DEV)
+
+        def step(q=q, k=k, v=v, dout=dout, p=p):
+            leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+            out = ops.cross_attention(ops.rotary_axes(leaves[0], p, (16, 16)), leaves[1], leaves[2])
+            return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step()
+        graphs.append((graph, held, step, (q, k, v, dout)))
+    for turn in range(3):
+        for graph, held, step, inputs in graphs:
+            for t in inputs:
+                t.copy_(torch.randn(t.shape, generator=rng(100 + turn), device=DEV).to(t.dtype))
+        for graph, *_ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, held, step, _ in graphs:
+            for a, b in zip(held, step()):
+                assert torch.equal(a, b)
+
+
+# --------------------------------------------------------------------------------------------------
+# AdamW
+# --------------------------------------------------------------------------------------------------
+def tensors(g, sizes, dtype, amsgrad, offset=0):
+    def some(scale, kind=torch.float32):
+        return [normal(g, n + offset, dtype=kind, scale=scale)[offset:] for n in sizes]
+
+    p, gr, m = some(0.05, dtype), some(1e-2, dtype), some(2e-3)
+    v = [t.square() for t in some(1e-2)]
+    return p, gr, m, v, [t * 1.5 for t in v] if amsgrad else None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("amsgrad", [False, True])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_adamw_matches_its_definition(dtype, amsgrad, offset):
+    from sleap_amd import ops
+
+    sizes = [1, 3, 4096, 4097, 0, 12289, 16, 5000] + [7 * i + 1 for i in range(130)]
+    p, gr, m, v, w = tensors(rng(20), sizes, dtype, amsgrad, offset)
+    if amsgrad:
+        w = [t * f for t, f in zip(w, torch.rand(len(w)).tolist())]
+    gr[5][17], v[3][0] = float("nan"), float("inf")
+    how = dict(step=7, lr=3e-3, betas=(0.8, 0.95), eps=1e-6, weight_decay=0.1)
+    want = [oracle.adamw(*[x[i] for x in (p, gr, m, v)], w[i] if amsgrad else None, **how) for i in range(len(sizes))]
+    ops.adamw_step(p, gr, m, v, max_exp_avg_sqs=w, **how)
+    for i, o in enumerate(want):
+        for name, got in (("param", p), ("exp_avg", m), ("exp_avg_sq", v), ("max_exp_avg_sq", w)):
+            if name in o:
+                assert oracle.worst(got[i], o[name]) <= 1, (i, name)
+
+
+def test_adamw_of_mixed_types_and_of_its_corners():
+    from sleap_amd import ops
+
+    g = rng(21)
+    sets = [tensors(g, [100, 5000], dtype, False) for dtype in (torch.float32, torch.bfloat16, torch.float16)]
+    p, gr, m, v = ([t for s in sets for t in s[j]] for j in range(4))
+    for t in gr + m + v:
+        t.zero_()  # no gradient so far: only the decay moves
+    before = [t.double() for t in p]
+    ops.adamw_step(p, gr, m, v, step=1, lr=0.5, weight_decay=0.5)
+    for a, b in zip(p, before):
+        assert oracle.worst(a, (b * 0.75, b.abs() * 1.01 * oracle.UNIT[a.dtype] + oracle.TINY[a.dtype])) <= 1
+    ops.adamw_step([], [], [], [], step=1, lr=1.0)
+
+
+def test_a_captured_adamw_step_counts_on():
+    from sleap_amd import ops
+
+    p, gr, m, v, _ = tensors(rng(22), [300, 70], torch.float32, False)
+    q, mm, vv = ([t.clone() for t in x] for x in (p, m, v))
+    step, lr = torch.zeros(1, dtype=torch.int64, device=DEV), torch.full((1,), 1e-2, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step.add_(1)
+        ops.adamw_step(p, gr, m, v, step=step, lr=lr)
+        with pytest.raises(RuntimeError, match="count as a tensor"):
+            ops.adamw_step(p, gr, m, v, step=1, lr=lr)
+    for t in range(1, 4):
+        lr.fill_(1e-2 / t)
+        graph.replay()
+        ops.adamw_step(q, gr, mm, vv, step=t, lr=1e-2 / t)
+        torch.cuda.synchronize()
+        for a, b in zip(p + m + v, q + mm + vv):
+            assert torch.allclose(a, b, rtol=4 * oracle.F32, atol=1e-9)  # lr and its decay once rounded more
+
+
+def test_the_optimizer_follows_the_definition_over_steps():
+    """Eight steps with a schedule against the 64-bit step, allowances added up; a state that was saved and loaded goes on."""
+    from sleap_amd.nn.optim import AdamW
+
+    g = rng(23)
+    start = [normal(g, *s, dtype=torch.float32, scale=0.1) for s in ((16, 3, 3, 3), (16,), (33, 16), (7,))]
+    params = [torch.nn.Parameter(t.clone()) for t in start]
+    opt = AdamW([dict(params=params[:2], lr=1e-2), dict(params=params[2:], weight_decay=0.0)], lr=3e-3, amsgrad=True)
+    sched = torch.optim.lr_scheduler.LambdaLR(opt, lambda t: 1 / (1 + t))
+    state = [[t.double(), torch.zeros_like(t).double(), torch.zeros_like(t).double(), torch.zeros_like(t).double(), torch.zeros_like(t).double()] for t in start]
+    for t in range(1, 9):
+        for i, p in enumerate(params):
+            p.grad = None if i == 3 else normal(g, *p.shape, dtype=torch.float32, scale=10.0 ** (i - 2))
+            if i == 3:
+                continue
+            group = opt.param_groups[i // 2]
+            x, m, v, w, e = state[i]
+            o = oracle.adamw(x.float(), p.grad, m, v, w, step=t, lr=group["lr"], weight_decay=group["weight_decay"])
+            moved = x - x.float().double()
+            state[i] = [o["param"][0] + moved, o["exp_avg"][0], o["exp_avg_sq"][0], o["max_exp_avg_sq"][0], e + o["param"][1] * 4 * t]
+        opt.step()
+        sched.step()
+        if t == 4:
+            saved = opt.state_dict()
+            opt = AdamW([dict(params=params[:2]), dict(params=params[2:])], amsgrad=True)
+            opt.load_state_dict(saved)
+            sched.optimizer = opt
+            assert all(s["exp_avg"].dtype == torch.float32 for s in opt.state.values())
+    for p, (x, *_, e) in zip(params, state):
+        assert oracle.worst(p.detach(), (x, e + 1e-30)) <= 1
+    assert torch.equal(params[3].detach(), start[3])
+
+
+def test_the_optimizer_keeps_float32_states_of_16_bit_parameters():
+    from sleap_amd.nn.optim import AdamW
+
+    p = torch.nn.Parameter(normal(rng(24), 50, dtype=torch.bfloat16))
+    p.grad = torch.full_like(p, 1e-3)
+    opt = AdamW([p], lr=1e-2)
+    opt.step()
+    saved = opt.state_dict()
+    m = opt.state[p]["exp_avg"].clone()
+    opt.load_state_dict(saved)
+    assert opt.state[p]["exp_avg"].dtype == torch.float32 and torch.equal(opt.state[p]["exp_avg"], m)
+    opt.step()
+    assert opt.state[p]["step"] == 2
+    p.grad = torch.ones((5, 10), device=DEV, dtype=torch.bfloat16).T.reshape(50)  # any layout of gradient
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.zeros(1, device=DEV)
+        with pytest.raises(RuntimeError, match="counts on the host"):
+            opt.step()
+
+
+def test_the_fitting_commands_step_on_the_gpu():
+    """tools/train_benchmark_model.py as it is started, three small steps of it: the fit runs and its losses stay finite."""
+    import os
+    import subprocess
+    import sys
+    import tempfile
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with tempfile.TemporaryDirectory() as d:
+        run = subprocess.run([sys.executable, os.path.join(root, "tools", "train_benchmark_model.py"), "--steps", "3", "--batch", "2", "--crop", "128", "--pool", "1",
+                              "--out", os.path.join(d, "w.npz")], capture_output=True, text=True, timeout=110)
+        assert run.returncode == 0 and os.path.exists(os.path.join(d, "w.npz")), run.stderr[-2000:]
+    losses = [float(line.split("loss")[1].split()[0]) for line in run.stdout.splitlines() if line.startswith("step")]
+    assert len(losses) == 2 and all(math.isfinite(v) for v in losses) and "on cuda" in run.stdout
+
+
+# --------------------------------------------------------------------------------------------------
+# together
+# --------------------------------------------------------------------------------------------------
+def test_keypoint_queries_read_a_padded_clip_and_are_fitted():
+    """Queries with sub-pixel places read the tokens of clips of different lengths: rotary -> attention -> loss -> gradients -> AdamW,
+    three steps of a whole model, each step's gradients against the same graph in 64 bits."""
+    from sleap_amd import ops
+    from sleap_amd.nn.optim import AdamW
+
+    g = rng(25)
+    B, frames, side, N, H, D = 3, 3, 7, 26, 4, 32
+    Tk = frames * side * side
+    feats = normal(g, B, Tk, H * D, dtype=torch.bfloat16)
+    grid = torch.stack(torch.meshgrid(torch.arange(frames, device=DEV), torch.arange(side, device=DEV), torch.arange(side, device=DEV), indexing="ij"), -1).reshape(Tk, 3)
+    places = torch.rand((B, N, 3), generator=g, device=DEV) * side
+    lengths = torch.tensor([Tk, 2 * side * side, 0], dtype=torch.int32, device=DEV)
+    target = normal(g, B, N, 2, dtype=torch.float32)
+    params = [torch.nn.Parameter(normal(g, *s, dtype=torch.float32, scale=0.2)) for s in ((N, H * D), (H * D, H * D), (H * D, H * D), (H * D, 2))]
+    opt = AdamW(params, lr=1e-3)
+
+    def loss_of(ps, rotary, attend, kind):
+        q0, wk, wv, wo = ps
+        q = rotary(q0.to(kind).expand(B, N, H * D).reshape(B, N, H, D), places)
+        k = rotary((feats.to(kind) @ wk.to(kind)).reshape(B, Tk, H, D), grid)
+        v = (feats.to(kind) @ wv.to(kind)).reshape(B, Tk, H, D)
+        y = attend(q, k, v).reshape(B, N, H * D).to(wo.dtype) @ wo
+        return ((y - target.to(y.dtype)) ** 2).mean()
+
+    def rotary64(x, p):
+        axis = [0] * 4 + [1] * 6 + [2] * 6
+        f = torch.tensor([10000.0 ** -(i / n) for n in (4, 6, 6) for i in range(n)], device=DEV, dtype=torch.float64)
+        a = p.double()[..., axis] * f
+        c, s = a.cos()[..., None, :], a.sin()[..., None, :]
+        u, w = x[..., :16], x[..., 16:]
+        return torch.cat([u * c - w * s, w * c + u * s], -1)
+
+    def attend64(q, k, v):
+        s = (q.transpose(1, 2) @ k.permute(0, 2, 3, 1).contiguous()) / math.sqrt(D)
+        s = s.masked_fill((torch.arange(Tk, device=DEV)[None] >= lengths[:, None])[:, None, None], -1e300)
+        w = torch.softmax(s, -1) * (lengths > 0)[:, None, None, None]
+        return (w @ v.transpose(1, 2).contiguous()).transpose(1, 2)
+
+    for _ in range(3):
+        opt.zero_grad()
+        loss = loss_of(params, lambda x, p: ops.rotary_axes(x, p, (4, 6, 6)), lambda q, k, v: ops.cross_attention(q, k, v, key_lengths=lengths), torch.bfloat16)
+        loss.backward()
+        twins = [p.detach().double().requires_grad_(True) for p in params]
+        wants = torch.autograd.grad(loss_of(twins, rotary64, attend64, torch.float64), twins)
+        for p, want in zip(params, wants):
+            # bf16 along the way: inputs, products, turns, weights and outputs are rounded, about ten roundings of 2^-9 each that
+            # add up along sums of hundreds of terms of either sign; held to ten of them over the whole gradient
+            assert (p.grad.double() - want).norm() <= 10 * 2.0 ** -8 * want.norm()
+        opt.step()
+    assert all(torch.isfinite(p).all() for p in params)

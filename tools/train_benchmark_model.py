@@ -5,7 +5,7 @@ upsampling; 13-node confidence maps @ stride 4 + 12-edge part-affinity fields @ 
 that DETECTS the rendered animals (4 instances x 13 nodes per frame, peaks far above the 0.2 threshold, PAF scores far above
 the 0.25 cut) instead of on the noise-like maps of a random-init network.
 
-TOOLING, not product: plain torch autograd on whatever device torch offers (CPU here; a few hundred steps on 256 x 256 crops
+TOOLING, not product: plain torch autograd on whatever device torch offers (on a GPU with the package's optimizer step; CPU here; a few hundred steps on 256 x 256 crops
 are enough because node identity and limb direction are locally decodable in the rendering). Seeded and reproducible on one
 machine/torch build. The targets are the reference's own training targets for this profile, re-stated in torch:
 
@@ -35,6 +35,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
 
 from sleap_amd.nn.architectures import build_unet_model_config, he_normal_weights  # noqa: E402  (plain data, no GPU)
+from sleap_amd.nn.optim import adam  # noqa: E402
 from sleap_amd.synth import FLIES13_EDGES, FLIES13_NODES, render_flies  # noqa: E402
 
 EDGE_IDX = [(FLIES13_NODES.index(a), FLIES13_NODES.index(b)) for a, b in FLIES13_EDGES]
@@ -161,7 +162,7 @@ def main():
     net = TorchGraph(mc, weights).to(dev)
     print(f"{sum(p.numel() for p in net.parameters())} parameters on {dev}", flush=True)
     frames, insts = render_flies(args.pool, 1024, 1024, 4, seed=10_000 + args.seed + (1000 if args.resume else 0))  # training seeds are disjoint from bench/test seeds (< 10000)
-    opt = torch.optim.Adam(net.parameters(), lr=args.lr)
+    opt = adam(net.parameters(), args.lr)
     sched = torch.optim.lr_scheduler.OneCycleLR(opt, max_lr=args.lr, total_steps=args.steps, pct_start=0.1)
     margin = 24  # crop borders see zero padding where the full frame has context: keep them out of the loss
     t0 = time.time()

@@ -38,6 +38,7 @@ sys.path.insert(0, os.path.join(ROOT, "tests"))  # config_models.py: test infras
 
 from sleap_amd.nn import architectures as A  # noqa: E402  (plain data, no GPU)
 from sleap_amd import synth  # noqa: E402
+from sleap_amd.nn.optim import adam  # noqa: E402
 
 from config_models import ANCHOR, DATA_DIR as OUT_DIR, TASKS, load_task_weights, task_graph  # noqa: E402
 
@@ -228,7 +229,7 @@ def make_targets(t, skel, insts, crop):
 
 def fit(task, steps=None, threads=0, seed=0, lr=2e-3, resume=False, device="cpu", out_dir=None, batch=0, hard_neg=0.0,
         bn_inference=False, crop=0):
-    """`device="cuda"`: the same fit on a GPU (plain torch; used for the ResNet-50 task, 45 minutes on 8 CPU cores). The stored
+    """`device="cuda"`: the same fit on a GPU (plain torch but for the optimizer step; used for the ResNet-50 task, 45 minutes on 8 CPU cores). The stored
     weights then depend on the GPU's convolution algorithms: reproducible in distribution, not bit for bit."""
     t = dict(TASKS[task])
     steps = steps or t["steps"]
@@ -261,7 +262,7 @@ def fit(task, steps=None, threads=0, seed=0, lr=2e-3, resume=False, device="cpu"
     net = TorchGraph(mc, weights, freeze=t.get("freeze")).to(device)
     n_fit = sum(p.numel() for p in net.parameters())
     print(f"[{task}] {n_fit} fitted parameters ({len(net.frozen)} frozen tensors), crop {crop}, {steps} steps", flush=True)
-    opt = torch.optim.Adam(net.parameters(), lr=lr)
+    opt = adam(net.parameters(), lr)
     sched = torch.optim.lr_scheduler.OneCycleLR(opt, max_lr=lr, total_steps=steps, pct_start=0.1)
     # pixels of a crop's border ring left out of the loss. 0 for tasks whose network sees whole frames at inference with a large
     # receptive field (the ResNet: with a free border ring its confidence maps reached 4.0 along the frame edges -- 1100 false
