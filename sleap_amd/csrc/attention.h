@@ -87,7 +87,7 @@ __device__ __forceinline__ float sum_halves(float v) {
 }
 
 template <int DP>
-__device__ __forceinline__ int swizzle(int row) {
+__device__ __host__ constexpr int swizzle(int row) {
   constexpr int PER_LINE = 128 / DP, PAIRS = DP / 16;  // rows of 256 bytes, 32-byte pairs of a row
   return ((row / PER_LINE) & (PAIRS - 1)) << 1;
 }
@@ -96,11 +96,11 @@ __device__ __forceinline__ int swizzle(int row) {
 template <int DP>
 struct Tile {
   static constexpr int ROW = DP * 2, BYTES = TILE * ROW, PIECES = BYTES / 1024;
-  // byte address of the A operand's eight values at k-step ks, row m of a 32-row block: off_a(m, h, ks) + block * 32 * ROW
-  __device__ static __forceinline__ int off_a(int m, int h, int ks) { return m * ROW + (((ks * 2 + h) ^ swizzle<DP>(m)) << 4); }
-  // transposed read: rows 16 kk + 8 u + 4 h .. + 3, columns of block db: off_t(lane, db) + (16 kk + 8 u) * ROW
-  __device__ static __forceinline__ int off_t(int lane, int db) {
-    const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), c = db * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+  // A operand: eight values of k-step ks of row m of a 32-row block at (at_a(m, h) ^ (ks << 5)) + block * 32 * ROW
+  __device__ static __forceinline__ int at_a(int m, int h) { return m * ROW + ((h ^ swizzle<DP>(m)) << 4); }
+  // transposed read: rows 16 kk + 8 u + 4 h .. + 3, columns of block db at (at_t(lane) ^ (db << 6)) + (16 kk + 8 u) * ROW
+  __device__ static __forceinline__ int at_t(int lane) {
+    const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), c = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
     return row * ROW + ((c ^ swizzle<DP>(row)) << 4) + (lane & 1) * 8;
   }
 };
@@ -115,27 +115,38 @@ __device__ __forceinline__ s16x8 read_t(const char* lds, int off, int step) {
 // every wave's copies have landed, every wave's reads are done
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Which 16 bytes of a tile each lane copies: piece (wave + j NW) of 1 KB holds rows row0 + j STEP. A lane's place in its row is the same
+// for every j (swizzle(row) repeats with STEP), but for a single wave on rows of 256 bytes, where odd j differ in one bit.
+template <int DP, int NW>
+struct Pieces {
+  static constexpr int N = (Tile<DP>::PIECES + NW - 1) / NW, STEP = NW * 1024 / Tile<DP>::ROW;
+  int row0, c0;
+  __device__ __forceinline__ void init(int wave, int lane) {
+    const int at = wave * 1024 + lane * 16;
+    row0 = at / Tile<DP>::ROW;
+    c0 = ((at >> 4) & (DP / 8 - 1)) ^ swizzle<DP>(row0);
+  }
+  __device__ __forceinline__ int row(int j) const { return row0 + j * STEP; }
+  __device__ __forceinline__ int piece(int j) const { return c0 ^ swizzle<DP>(j * STEP); }
+  __device__ static __forceinline__ bool any(int wave, int j) { return Tile<DP>::PIECES % NW == 0 || wave + j * NW < Tile<DP>::PIECES; }
+};
+
 // Copies of a tile's rows into LDS by NW waves. `rows` is the 64-bit word of the rows that exist (all others become zeros).
 template <int DP, int NW>
 struct TileCopy {
-  static constexpr int N = (Tile<DP>::PIECES + NW - 1) / NW;
-  uint32_t off[N];
-  int row[N];
+  Pieces<DP, NW> at;
+  uint32_t off[Pieces<DP, NW>::N];  // kept: computing them in every tile costs the forward kernel 5 %
   __device__ __forceinline__ void init(int wave, int lane, int64_t stride_bytes, int D) {
+    at.init(wave, lane);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int at = (wave + j * NW) * 1024 + lane * 16;
-      row[j] = at / Tile<DP>::ROW;
-      const int c = ((at >> 4) & (DP / 8 - 1)) ^ swizzle<DP>(row[j]);
-      off[j] = c * 8 < D ? (uint32_t)(row[j] * stride_bytes) + c * 16 : OUT_OF_RANGE;
-    }
+    for (int j = 0; j < at.N; ++j) off[j] = at.piece(j) * 8 < D ? at.row(j) * (uint32_t)stride_bytes + at.piece(j) * 16 : OUT_OF_RANGE;
   }
   __device__ __forceinline__ void issue(char* lds, const void* base, uint64_t rows, int wave) const {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (Tile<DP>::PIECES % NW != 0 && wave + j * NW >= Tile<DP>::PIECES) break;
-      const uint32_t o = rows == ~0ull ? off[j] : ((rows >> row[j]) & 1) ? off[j] : OUT_OF_RANGE;
+    for (int j = 0; j < at.N; ++j) {
+      if (!at.any(wave, j)) break;
+      const uint32_t o = rows == ~0ull || ((rows >> at.row(j)) & 1) ? off[j] : OUT_OF_RANGE;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(lds + (wave + j * NW) * 1024), 16, o, 0, 0, 0);
     }
   }

@@ -79,9 +79,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
 
   int oa[KS], ot[DB];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) oa[ks] = T::off_a(n, h, ks);
+  for (int ks = 0; ks < KS; ++ks) oa[ks] = T::at_a(n, h) ^ (ks << 5);
 #pragma unroll
-  for (int db = 0; db < DB; ++db) ot[db] = T::off_t(lane, db);
+  for (int db = 0; db < DB; ++db) ot[db] = T::at_t(lane) ^ (db << 6);
 
   f32x16 o[DB] = {};
   float m = -INFINITY, l = 0.0f, shift = -Range<E>::LIFT;  // shift = c m - LIFT, of a maximum that is not -inf

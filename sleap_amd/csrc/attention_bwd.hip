@@ -91,38 +91,24 @@ __global__ __launch_bounds__(256) void attention_stats_kernel(const BwdParams p,
 }
 
 // rows r0 .. r0 + 63 of q and dout into two tiles
-template <int DP, int NW>
-struct RowCopy {
-  static constexpr int N = (Tile<DP>::PIECES + NW - 1) / NW;
-  int row[N];
-  uint32_t col[N];
-  __device__ __forceinline__ void init(int wave, int lane, int D) {
+template <int DP, int NW, typename E>
+__device__ __forceinline__ void copy_rows(char* lds, const Pieces<DP, NW>& at, const BwdParams& p, const E* q, const E* dout, uint32_t r0, uint32_t end, int wave) {
+  const AttnShape& a = p.a;
+  const uint32_t t0 = __builtin_amdgcn_readfirstlane(div_by(r0, a.div_g));
+  const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(q + (int64_t)t0 * a.qt), 0, 0x7FFFFFFF, 0x00020000);
+  const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(dout + (int64_t)t0 * p.ot), 0, 0x7FFFFFFF, 0x00020000);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int at = (wave + j * NW) * 1024 + lane * 16;
-      row[j] = at / Tile<DP>::ROW;
-      const int c = ((at >> 4) & (DP / 8 - 1)) ^ swizzle<DP>(row[j]);
-      col[j] = c * 8 < D ? c * 16 : OUT_OF_RANGE;
-    }
+  for (int j = 0; j < at.N; ++j) {
+    if (!at.any(wave, j)) break;
+    const int c = at.piece(j);
+    const uint32_t r = r0 + at.row(j), t = div_by(r, a.div_g), g = r - t * a.G;
+    const bool in = r < end && c * 8 < a.D;
+    const uint32_t oq = in ? 2 * ((t - t0) * (uint32_t)a.qt + g * (uint32_t)a.qh) + c * 16 : OUT_OF_RANGE;
+    const uint32_t oo = in ? 2 * ((t - t0) * (uint32_t)p.ot + g * (uint32_t)p.oh) + c * 16 : OUT_OF_RANGE;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (lds_ptr)(lds + (wave + j * NW) * 1024), 16, oq, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(ro, (lds_ptr)(lds + Tile<DP>::BYTES + (wave + j * NW) * 1024), 16, oo, 0, 0, 0);
   }
-  template <typename E>
-  __device__ __forceinline__ void issue(char* lds, const BwdParams& p, const E* q, const E* dout, uint32_t r0, uint32_t end, int wave) const {
-    const AttnShape& a = p.a;
-    const uint32_t t0 = __builtin_amdgcn_readfirstlane(div_by(r0, a.div_g));
-    const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(q + (int64_t)t0 * a.qt), 0, 0x7FFFFFFF, 0x00020000);
-    const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(dout + (int64_t)t0 * p.ot), 0, 0x7FFFFFFF, 0x00020000);
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (Tile<DP>::PIECES % NW != 0 && wave + j * NW >= Tile<DP>::PIECES) break;
-      const uint32_t r = r0 + row[j], t = div_by(r, a.div_g), g = r - t * a.G;
-      const bool in = r < end && col[j] != OUT_OF_RANGE;
-      const uint32_t oq = in ? 2 * ((t - t0) * (uint32_t)a.qt + g * (uint32_t)a.qh) + col[j] : OUT_OF_RANGE;
-      const uint32_t oo = in ? 2 * ((t - t0) * (uint32_t)p.ot + g * (uint32_t)p.oh) + col[j] : OUT_OF_RANGE;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (lds_ptr)(lds + (wave + j * NW) * 1024), 16, oq, 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ro, (lds_ptr)(lds + Tile<DP>::BYTES + (wave + j * NW) * 1024), 16, oo, 0, 0, 0);
-    }
-  }
-};
+}
 
 template <typename E>
 __device__ __forceinline__ void store_column(E* dst, float* part, const f32x16* acc, int n, int D, int h, float by) {
@@ -139,7 +125,7 @@ __device__ __forceinline__ void store_column(E* dst, float* part, const f32x16* 
 
 // dk, dv: a wave owns 32 keys (k and v in registers) and walks rows in tiles of 64
 template <typename E, int DB, int NW>
-__global__ __launch_bounds__(NW * 64, DB == 4 ? 1 : 2) void attention_dkv_kernel(const BwdParams p) {
+__global__ __launch_bounds__(NW * 64, 2) void attention_dkv_kernel(const BwdParams p) {
   constexpr int DP = DB == 3 ? 128 : DB * 32, KS = DB * 2;
   using T = Tile<DP>;
   constexpr int STAGE = 2 * T::BYTES + 2 * TILE * 4;  // q, dout, lse2, delta
@@ -172,12 +158,12 @@ __global__ __launch_bounds__(NW * 64, DB == 4 ? 1 : 2) void attention_dkv_kernel
   const int tiles = key0 < length && first < end ? (int)((end - first + TILE - 1) / TILE) : 0;  // no visible key in this tile: nothing to walk
   const E* qbase = static_cast<const E*>(a.q) + (int64_t)b * a.qb + (int64_t)(hk * a.G) * a.qh;
   const E* obase = static_cast<const E*>(p.dout) + (int64_t)b * p.ob + (int64_t)(hk * a.G) * p.oh;
-  RowCopy<DP, NW> rc;
-  rc.init(wave, lane, a.D);
+  Pieces<DP, NW> pieces;
+  pieces.init(wave, lane);
   auto copy = [&](int i) {
     char* s = lds + (i & 1) * STAGE;
     const uint32_t r0 = first + (uint32_t)i * TILE;
-    rc.template issue<E>(s, p, qbase, obase, r0, end, wave);
+    copy_rows<DP, NW, E>(s, pieces, p, qbase, obase, r0, end, wave);
     if (wave == 0) {
       const int64_t at = (int64_t)bh * a.R + r0;
       const uint32_t o = r0 + lane < end ? lane * 4 : OUT_OF_RANGE;
@@ -185,43 +171,40 @@ __global__ __launch_bounds__(NW * 64, DB == 4 ? 1 : 2) void attention_dkv_kernel
       __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(p.delta + at, 0, 0x7FFFFFFF, 0x00020000), (lds_ptr)(s + 2 * T::BYTES + TILE * 4), 4, o, 0, 0, 0);
     }
   };
-  int oa[KS], ot[DB];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) oa[ks] = T::off_a(n, h, ks);
-#pragma unroll
-  for (int db = 0; db < DB; ++db) ot[db] = T::off_t(lane, db);
-
+  const int aa = T::at_a(n, h), at_ = T::at_t(lane);
   f32x16 dk[DB] = {}, dv[DB] = {};
   Range16<E> range;
   if (tiles) copy(0);
   for (int i = 0; i < tiles; ++i) {
     tile_barrier();
     if (i + 1 < tiles) copy(i + 1);
-    const char* qt = lds + (i & 1) * STAGE;
-    const char* dt = qt + T::BYTES;
-    const float* stat = reinterpret_cast<const float*>(qt + 2 * T::BYTES) + 4 * h;
-#pragma unroll
+    // one block of 32 rows after the other, not unrolled: its scores are out of the registers before the next one's come in, which
+    // leaves room for a second wave on each SIMD
+#pragma unroll 1
     for (int blk = 0; blk < 2; ++blk) {
+      const char* qt = lds + (i & 1) * STAGE + blk * 32 * T::ROW;
+      const char* dt = qt + T::BYTES;
+      const float* stat = reinterpret_cast<const float*>(lds + (i & 1) * STAGE + 2 * T::BYTES) + 4 * h + blk * 32;
       f32x16 s = {}, dp = {};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = Mfma<E>::run(read_a(qt, oa[ks] + blk * 32 * T::ROW), kf[ks], s);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) dp = Mfma<E>::run(read_a(dt, oa[ks] + blk * 32 * T::ROW), vf[ks], dp);
+      for (int ks = 0; ks < KS; ++ks) s = Mfma<E>::run(read_a(qt, aa ^ (ks << 5)), kf[ks], s);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const f32x4 l = *reinterpret_cast<const f32x4*>(stat + blk * 32 + 8 * j);
+        const f32x4 l = *reinterpret_cast<const f32x4*>(stat + 8 * j);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[4 * j + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], a.c, -l[e]));
       }
 #pragma unroll
+      for (int ks = 0; ks < KS; ++ks) dp = Mfma<E>::run(read_a(dt, aa ^ (ks << 5)), vf[ks], dp);
+#pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const s16x8 w = pack8<E>(s, s2);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) dv[db] = Mfma<E>::run(read_t(dt, ot[db] + (blk * 2 + s2) * 16 * T::ROW, 8 * T::ROW), w, dv[db]);
+        for (int db = 0; db < DB; ++db) dv[db] = Mfma<E>::run(read_t(dt, (at_ ^ (db << 6)) + s2 * 16 * T::ROW, 8 * T::ROW), w, dv[db]);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const f32x4 l = *reinterpret_cast<const f32x4*>(stat + TILE + blk * 32 + 8 * j);
+        const f32x4 l = *reinterpret_cast<const f32x4*>(stat + TILE + 8 * j);
 #pragma unroll
         for (int e = 0; e < 4; ++e) dp[4 * j + e] = s[4 * j + e] * (dp[4 * j + e] - l[e]);
       }
@@ -230,7 +213,7 @@ __global__ __launch_bounds__(NW * 64, DB == 4 ? 1 : 2) void attention_dkv_kernel
       for (int s2 = 0; s2 < 2; ++s2) {
         const s16x8 w = pack8<E>(dp, s2);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) dk[db] = Mfma<E>::run(read_t(qt, ot[db] + (blk * 2 + s2) * 16 * T::ROW, 8 * T::ROW), w, dk[db]);
+        for (int db = 0; db < DB; ++db) dk[db] = Mfma<E>::run(read_t(qt, (at_ ^ (db << 6)) + s2 * 16 * T::ROW, 8 * T::ROW), w, dk[db]);
       }
     }
   }
@@ -296,9 +279,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_dq_kernel(const BwdParam
   };
   int oa[KS], ot[DB];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) oa[ks] = T::off_a(n, h, ks);
+  for (int ks = 0; ks < KS; ++ks) oa[ks] = T::at_a(n, h) ^ (ks << 5);
 #pragma unroll
-  for (int db = 0; db < DB; ++db) ot[db] = T::off_t(lane, db);
+  for (int db = 0; db < DB; ++db) ot[db] = T::at_t(lane) ^ (db << 6);
 
   f32x16 dq[DB] = {};
   Range16<E> range;
