@@ -152,11 +152,17 @@ struct TileCopy {
   }
 };
 
-// hides the scores of keys whose bit in `seen` (32 keys of a block) is not set
-__device__ __forceinline__ void hide(f32x16& s, uint32_t seen, int h, float with) {
-  const uint32_t w = seen >> (4 * h);
+// Hides the scores of keys whose bit in `seen` (32 keys of a block) is not set: minus infinity in two instructions a score. Behind a
+// branch: the barrier keeps the compiler from doing this in every tile (it would take the select for cheaper than the jump).
+__device__ __forceinline__ void hide(f32x16& s, uint32_t seen, int h) {
+  __builtin_amdgcn_sched_barrier(0);
+  const int w = (int)(seen >> (4 * h));
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] = (w >> (8 * (i >> 2) + (i & 3))) & 1 ? s[i] : with;
+  for (int i = 0; i < 16; ++i) {
+    const int bit = 8 * (i >> 2) + (i & 3);
+    const uint32_t keep = (uint32_t)((w << (31 - bit)) >> 31);
+    s[i] = __uint_as_float((__float_as_uint(s[i]) & keep) | (0xFF800000u & ~keep));
+  }
 }
 
 // workgroups that read the same keys are neighbours in `id`: give each of the eight XCDs (workgroups go round them) a run of ids

@@ -85,6 +85,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
 
   f32x16 o[DB] = {};
   float m = -INFINITY, l = 0.0f, shift = -Range<E>::LIFT;  // shift = c m - LIFT, of a maximum that is not -inf
+  // A tile is copied while the one before is multiplied; the mask's bytes come one tile earlier still. (Three stages: slower by 5 to 15 %
+  // at every head size, and workgroups of eight waves gain nothing either.)
   uint64_t seen = 0;
   uint8_t next_mask = 1;
   if (tiles) {
@@ -110,12 +112,12 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
       s1 = Mfma<E>::run(read_a(kt, oa[ks] + 32 * T::ROW), q[ks], s1);
     }
     if (now != ~0ull) {
-      hide(s0, (uint32_t)now, h, -INFINITY);
-      hide(s1, (uint32_t)(now >> 32), h, -INFINITY);
+      hide(s0, (uint32_t)now, h);
+      hide(s1, (uint32_t)(now >> 32), h);
     }
     float top = fmaxf(s0[0], s1[0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s0[i], s1[i]));
+    for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, s0[i]), s1[i]);
     top = max_halves(top);
     if (__any((top - m) * a.c > GROW)) {
       const float grown = fmaxf(m, top), at = grown == -INFINITY ? 0.0f : grown;
@@ -170,33 +172,67 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
     }
 }
 
-// joins the runs of keys: out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max); a thread has 8 values of a row
+// Joins the runs of keys: out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max). A row has 16 lanes of 8 values and `groups` of
+// them: group j takes runs j, j + groups, ..., four loads of both kinds in flight, and the groups' sums meet in LDS. (One group that
+// walks all 32 runs of a single token: 14 us of latency where the attention itself takes 82.)
 template <typename E>
-__global__ __launch_bounds__(256) void attention_join_kernel(const FwdParams p, FastDiv div_pieces, FastDiv div_rows, uint32_t pieces, uint32_t total) {
+__global__ __launch_bounds__(256) void attention_join_kernel(const FwdParams p, FastDiv div_rows, uint32_t groups_log2, uint32_t rows) {
+  __shared__ float sums[256][10];
   const AttnShape& a = p.a;
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  const uint32_t br = div_by(i, div_pieces), d = (i - br * pieces) * 8;
-  const uint32_t bh = div_by(br, div_rows), row = br - bh * a.R;
-  const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv, t = div_by(row, a.div_g), g = row - t * a.G;
+  const uint32_t groups = 1u << groups_log2, lane = threadIdx.x & 15, unit = threadIdx.x >> 4, group = unit & (groups - 1);
+  const uint32_t br = blockIdx.x * (16 >> groups_log2) + (unit >> groups_log2), d = lane * 8;
+  const bool real = br < rows && d < (uint32_t)a.D;
+  const uint32_t bh = div_by(min(br, rows - 1), div_rows), row = min(br, rows - 1) - bh * a.R;
   const float* lse = p.part_lse + (int64_t)bh * p.splits * a.R + row;
-  float top = -INFINITY;
-  for (uint32_t s = 0; s < p.splits; ++s) top = fmaxf(top, lse[(int64_t)s * a.R]);
-  const float at = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, acc[8] = {};
-  for (uint32_t s = 0; s < p.splits; ++s) {
-    const float w = __builtin_amdgcn_exp2f(lse[(int64_t)s * a.R] - at);
-    const f32x4* src = reinterpret_cast<const f32x4*>(p.part + (((int64_t)bh * p.splits + s) * a.R + row) * a.D + d);
-    const f32x4 x = src[0], y = src[1];
-    sum += w;
+  const float* part = p.part + ((int64_t)bh * p.splits * a.R + row) * a.D + (real ? d : 0);
+  const int64_t step = (int64_t)a.R * a.D;
+  float m = -INFINITY, sum = 0.0f, acc[8] = {};
+  for (uint32_t s0 = group; s0 < p.splits; s0 += 4 * groups) {
+    float l[4];
+    f32x4 x[4], y[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      acc[e] += w * x[e];
-      acc[4 + e] += w * y[e];
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t s = min(s0 + k * groups, p.splits - 1);
+      l[k] = lse[(int64_t)s * a.R];
+      x[k] = *reinterpret_cast<const f32x4*>(part + s * step);
+      y[k] = *reinterpret_cast<const f32x4*>(part + s * step + 4);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (s0 + k * groups >= p.splits || l[k] == -INFINITY) continue;  // a run without a visible key
+      const float top = fmaxf(m, l[k]), keep = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(l[k] - top);
+      m = top;
+      sum = sum * keep + w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[e] = acc[e] * keep + w * x[k][e];
+        acc[4 + e] = acc[4 + e] * keep + w * y[k][e];
+      }
     }
   }
+  if (groups > 1) {
+    float* mine = sums[threadIdx.x];
+    mine[0] = m;
+    mine[1] = sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mine[2 + e] = acc[e];
+    __syncthreads();
+    if (group) return;
+    for (uint32_t g = 1; g < groups; ++g) {
+      const float* other = sums[threadIdx.x + 16 * g];
+      const float top = fmaxf(m, other[0]);
+      if (other[1] == 0.0f) continue;
+      const float keep = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(other[0] - top);
+      m = top;
+      sum = sum * keep + w * other[1];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = acc[e] * keep + w * other[2 + e];
+    }
+  }
+  if (!real) return;
+  const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv, t = div_by(row, a.div_g), g = row - t * a.G;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (p.lse && d == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = sum == 0.0f ? -INFINITY : (at + __log2f(sum)) * LN2;
+  if (p.lse && d == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = sum == 0.0f ? -INFINITY : (m + __log2f(sum)) * LN2;
   E* dst = static_cast<E*>(p.out) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D + d;
   *reinterpret_cast<u32x4*>(dst) = u32x4{pack2<E>(acc[0] * inv, acc[1] * inv), pack2<E>(acc[2] * inv, acc[3] * inv),
                                          pack2<E>(acc[4] * inv, acc[5] * inv), pack2<E>(acc[6] * inv, acc[7] * inv)};
@@ -228,7 +264,8 @@ Cut cut(int B, int Tq, int Tk, int Hq, int Hkv) {
 
 template <typename E, int DB>
 void launch(const FwdParams& p, int waves, hipStream_t s) {
-  constexpr size_t lds = 4 * Tile<DB == 3 ? 128 : DB * 32>::BYTES;
+  constexpr int DP = DB == 3 ? 128 : DB * 32;
+  constexpr size_t lds = 4 * Tile<DP>::BYTES;
   if (waves == 1) attention_kernel<E, DB, 1><<<dim3(p.blocks), dim3(64), lds, s>>>(p);
   else if (waves == 2) attention_kernel<E, DB, 2><<<dim3(p.blocks), dim3(128), lds, s>>>(p);
   else attention_kernel<E, DB, 4><<<dim3(p.blocks), dim3(256), lds, s>>>(p);
@@ -242,8 +279,11 @@ void launch_e(const FwdParams& p, int waves, hipStream_t s) {
   else if (db == 3) launch<E, 3>(p, waves, s);
   else launch<E, 4>(p, waves, s);
   if (p.splits > 1) {
-    const uint32_t pieces = p.a.D / 8, total = (uint32_t)(p.blocks / p.row_tiles / p.splits) * p.a.R * pieces;
-    attention_join_kernel<E><<<dim3((total + 255) / 256), dim3(256), 0, s>>>(p, fast_div(pieces), fast_div(p.a.R), pieces, total);
+    const uint32_t rows = p.blocks / p.row_tiles / p.splits * p.a.R;
+    uint32_t log2 = 0;
+    while (log2 < 4 && (4u << log2) < p.splits) ++log2;  // four runs a group
+    const uint32_t per = 16 >> log2;
+    attention_join_kernel<E><<<dim3((rows + per - 1) / per), dim3(256), 0, s>>>(p, fast_div(p.a.R), log2, rows);
   }
 }
 
@@ -301,7 +341,7 @@ extern "C" int sa_cross_attention(const void* q, const void* k, const void* v, i
   SA_REQUIRE(((uintptr_t)out & 15) == 0, "sa_cross_attention: addresses are multiples of 16");
   const Cut c = cut(B, Tq, Tk, Hq, Hkv);
   const uint64_t blocks = (uint64_t)c.row_tiles * c.splits * B * Hkv;
-  SA_REQUIRE(blocks < (1ull << 31) && (uint64_t)B * Hq * Tq * D / 8 < (1ull << 31), "sa_cross_attention: too many rows");
+  SA_REQUIRE(blocks < (1ull << 31) && (uint64_t)B * Hq * Tq < (1ull << 31) - 1024, "sa_cross_attention: too many rows");
   if (c.splits > 1 && workspace_bytes < sa_cross_attention_workspace(B, Tq, Tk, Hq, Hkv, D))
     return fail(SA_ERR_WORKSPACE, "sa_cross_attention: workspace of %zu bytes is too small", workspace_bytes);
   p.out = out;

@@ -1,15 +1,22 @@
 // Gradients of cross attention. With w = softmax (from the stored logarithms of its denominators, not kept), dw = do v^T,
 // ds = w (dw - rowsum(do * out)):
 //     dv = w^T do        dk = scale ds^T q        dq = scale ds k
-// Two kernels, both without atomics, so that sums have one order: one whose waves own keys and walk the rows (dk, dv: four products),
-// one whose waves own rows and walk the keys (dq: three). A combined kernel would save two of the seven products and need
-// atomics or a float32 dq read and written once per run of keys. Shared heads are rows like any others (attention.h): dk and dv sum
-// over them by themselves. Few rows or few keys: runs of the walked side go to several workgroups, and a last kernel adds them in order.
+// Two sides, both without atomics, so that sums have one order: one whose waves own keys and walk the rows (dk, dv: four products), one
+// whose waves own rows and walk the keys (dq: three). One that does both would save two of the seven products and need
+// atomics or a float32 dq read and written once per tile of keys. Shared heads are rows like any others (attention.h): dk and dv sum
+// over them by themselves. Where one side owns little, runs of what it walks go to several workgroups, and a last
+// kernel adds their float32 sums in order.
 #include "attention.h"
 
 namespace {
 
 using namespace sa;
+
+struct Side {
+  uint32_t blocks, tiles, splits;  // workgroups; of them along the owned side, along the walked side
+  int run;                         // rows (keys) of a run: a multiple of TILE
+  FastDiv div_tiles, div_splits;
+};
 
 struct BwdParams {
   AttnShape a;
@@ -19,9 +26,9 @@ struct BwdParams {
   float *lse2, *delta;      // [B * Hkv][R]: log2 of the denominator less LIFT; rowsum(do * out)
   void *dq, *dk, *dv;       // contiguous
   float *part_dq, *part_dk, *part_dv;  // [splits] of the whole gradient each, or NULL
-  uint32_t blocks, tiles, splits;      // tiles: workgroups along the owned side
-  int run;                  // rows (keys) of a run: a multiple of TILE
-  FastDiv div_tiles, div_splits, div_heads, div_hq;
+  Side kv, rows;            // who owns keys and walks rows (dk, dv); who owns rows and walks keys (dq)
+  uint32_t heads;           // B * Hkv
+  FastDiv div_heads, div_hq;
 };
 
 // w is rounded to 16 bits for w^T do, ds for the other two. bf16 has the range of float32. fp16 has not: w moves up by 2^14 (held down to
@@ -125,16 +132,16 @@ __device__ __forceinline__ void store_column(E* dst, float* part, const f32x16* 
 
 // dk, dv: a wave owns 32 keys (k and v in registers) and walks rows in tiles of 64
 template <typename E, int DB, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void attention_dkv_kernel(const BwdParams p) {
+__device__ __forceinline__ void keys_side(const BwdParams& p, uint32_t block, char* lds) {
   constexpr int DP = DB == 3 ? 128 : DB * 32, KS = DB * 2;
   using T = Tile<DP>;
   constexpr int STAGE = 2 * T::BYTES + 2 * TILE * 4;  // q, dout, lse2, delta
-  extern __shared__ __align__(1024) char lds[];
   const AttnShape& a = p.a;
+  const Side& side = p.kv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
-  const uint32_t id = xcd_run(blockIdx.x, p.blocks);
-  const uint32_t bhs = div_by(id, p.div_tiles), tile = id - bhs * p.tiles;
-  const uint32_t bh = div_by(bhs, p.div_splits), split = bhs - bh * p.splits;
+  const uint32_t id = xcd_run(block, side.blocks);
+  const uint32_t bhs = div_by(id, side.div_tiles), tile = id - bhs * side.tiles;
+  const uint32_t bh = div_by(bhs, side.div_splits), split = bhs - bh * side.splits;
   const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv;
 
   int length = a.Tk;
@@ -154,7 +161,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_dkv_kernel(const BwdPara
       vf[ks] = in ? *reinterpret_cast<const s16x8*>(vs_ + d) : s16x8{};
     }
   }
-  const uint32_t first = split * (uint32_t)p.run, end = min(first + (uint32_t)p.run, a.R);
+  const uint32_t first = split * (uint32_t)side.run, end = min(first + (uint32_t)side.run, a.R);
   const int tiles = key0 < length && first < end ? (int)((end - first + TILE - 1) / TILE) : 0;  // no visible key in this tile: nothing to walk
   const E* qbase = static_cast<const E*>(a.q) + (int64_t)b * a.qb + (int64_t)(hk * a.G) * a.qh;
   const E* obase = static_cast<const E*>(p.dout) + (int64_t)b * p.ob + (int64_t)(hk * a.G) * p.oh;
@@ -223,22 +230,22 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_dkv_kernel(const BwdPara
     for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
   }
   const int64_t at = (((int64_t)b * a.Tk + key) * a.Hkv + hk) * a.D;
-  const int64_t whole = (int64_t)(p.blocks / (p.tiles * p.splits)) * a.Tk * a.D;
+  const int64_t whole = (int64_t)p.heads * a.Tk * a.D;
   store_column<E>(static_cast<E*>(p.dk) + at, p.part_dk ? p.part_dk + split * whole + at : nullptr, dk, DB, a.D, h, a.scale * Lift<E>::BACK * range.back());
   store_column<E>(static_cast<E*>(p.dv) + at, p.part_dv ? p.part_dv + split * whole + at : nullptr, dv, DB, a.D, h, Lift<E>::BACK);
 }
 
 // dq: a wave owns 32 rows (q and dout in registers) and walks keys in tiles of 64
 template <typename E, int DB, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void attention_dq_kernel(const BwdParams p) {
+__device__ __forceinline__ void rows_side(const BwdParams& p, uint32_t block, char* lds) {
   constexpr int DP = DB == 3 ? 128 : DB * 32, KS = DB * 2;
   using T = Tile<DP>;
-  extern __shared__ __align__(1024) char lds[];
   const AttnShape& a = p.a;
+  const Side& side = p.rows;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
-  const uint32_t id = xcd_run(blockIdx.x, p.blocks);
-  const uint32_t bhs = div_by(id, p.div_tiles), tile = id - bhs * p.tiles;
-  const uint32_t bh = div_by(bhs, p.div_splits), split = bhs - bh * p.splits;
+  const uint32_t id = xcd_run(block, side.blocks);
+  const uint32_t bhs = div_by(id, side.div_tiles), tile = id - bhs * side.tiles;
+  const uint32_t bh = div_by(bhs, side.div_splits), split = bhs - bh * side.splits;
   const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv;
 
   const uint32_t row = tile * (NW * 32) + wave * 32 + n;
@@ -258,7 +265,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_dq_kernel(const BwdParam
   const float lse2 = p.lse2[(int64_t)bh * a.R + rr], delta = p.delta[(int64_t)bh * a.R + rr];
   int length = a.Tk;
   if (a.lengths) length = min(max(a.lengths[b], 0), a.Tk);
-  const int first = (int)split * p.run, end = min(first + p.run, length);
+  const int first = (int)split * side.run, end = min(first + side.run, length);
   const int tiles = end > first ? (end - first + TILE - 1) / TILE : 0;
   const E* kbase = static_cast<const E*>(a.k) + (int64_t)b * a.kb + (int64_t)hk * a.kh;
   const E* vbase = static_cast<const E*>(a.v) + (int64_t)b * a.vb + (int64_t)hk * a.vh;
@@ -310,7 +317,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_dq_kernel(const BwdParam
       for (int ks = 0; ks < KS; ++ks) s = Mfma<E>::run(read_a(kt, oa[ks] + blk * 32 * T::ROW), qf[ks], s);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) dp = Mfma<E>::run(read_a(vt, oa[ks] + blk * 32 * T::ROW), df[ks], dp);
-      if (now != ~0ull) hide(s, (uint32_t)(now >> (32 * blk)), h, -INFINITY);
+      if (now != ~0ull) hide(s, (uint32_t)(now >> (32 * blk)), h);
 #pragma unroll
       for (int e = 0; e < 16; ++e) dp[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.c, -lse2)) * (dp[e] - delta);
       range.follow(dp, dq, DB);
@@ -324,125 +331,120 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_dq_kernel(const BwdParam
   }
   if (!real) return;
   const int64_t at = (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D;
-  const int64_t whole = (int64_t)(p.blocks / (p.tiles * p.splits)) * a.R * a.D;
+  const int64_t whole = (int64_t)p.heads * a.R * a.D;
   store_column<E>(static_cast<E*>(p.dq) + at, p.part_dq ? p.part_dq + split * whole + at : nullptr, dq, DB, a.D, h, a.scale * Lift<E>::BACK * range.back());
 }
 
-// adds the runs' gradients, in their order; a thread has 8 values
+// Both sides in one launch: neither needs the other, and one's last workgroups fill up with the other's. Rows come first, their
+// walks are the longer ones where keys are many.
+template <typename E, int DB, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void attention_bwd_kernel(const BwdParams p) {
+  extern __shared__ __align__(1024) char lds[];
+  if (blockIdx.x < p.rows.blocks) rows_side<E, DB, NW>(p, blockIdx.x, lds);
+  else keys_side<E, DB, NW>(p, blockIdx.x - p.rows.blocks, lds);
+}
+
+// Adds the runs' gradients, in their order, of up to three tensors; a thread has 8 values of one.
+struct AddParams {
+  const float* part[3];
+  void* dst[3];
+  int64_t n[3];
+  int splits[3];
+  uint32_t first[3];  // first workgroup of each
+};
 template <typename E>
-__global__ __launch_bounds__(256) void attention_add_kernel(const float* part, E* dst, int64_t n, int splits) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+__global__ __launch_bounds__(256) void attention_add_kernel(const AddParams p) {
+  const int k = blockIdx.x >= p.first[2] ? 2 : blockIdx.x >= p.first[1] ? 1 : 0;
+  const int64_t i = ((int64_t)(blockIdx.x - p.first[k]) * 256 + threadIdx.x) * 8, n = p.n[k];
   if (i >= n) return;
   f32x4 x = {}, y = {};
-  for (int s = 0; s < splits; ++s) {
-    const f32x4* src = reinterpret_cast<const f32x4*>(part + s * n + i);
+#pragma unroll 4
+  for (int s = 0; s < p.splits[k]; ++s) {
+    const f32x4* src = reinterpret_cast<const f32x4*>(p.part[k] + s * n + i);
     x += src[0];
     y += src[1];
   }
-  *reinterpret_cast<u32x4*>(dst + i) = u32x4{pack2<E>(x[0], x[1]), pack2<E>(x[2], x[3]), pack2<E>(y[0], y[1]), pack2<E>(y[2], y[3])};
+  *reinterpret_cast<u32x4*>(static_cast<E*>(p.dst[k]) + i) = u32x4{pack2<E>(x[0], x[1]), pack2<E>(x[2], x[3]), pack2<E>(y[0], y[1]), pack2<E>(y[2], y[3])};
 }
 
-// How one of the two kernels is cut: `own` rows (keys) among waves of 32, `walk` keys (rows) among runs.
-struct Cut {
-  int waves;
-  uint32_t tiles, splits;
-  int run;
-};
-Cut cut(uint64_t heads, uint64_t own, uint64_t walk) {
-  Cut c;
-  c.waves = own <= 32 ? 1 : own <= 64 ? 2 : 4;
-  c.tiles = (uint32_t)((own + c.waves * 32 - 1) / (c.waves * 32));
-  const uint64_t blocks = c.tiles * heads, want = 2048 / c.waves, walked = (walk + TILE - 1) / TILE;
+// How a side is cut: what it owns among waves of 32, what it walks among runs.
+Side cut(int waves, uint64_t heads, uint64_t own, uint64_t walk) {
+  Side c;
+  c.tiles = (uint32_t)((own + waves * 32 - 1) / (waves * 32));
+  const uint64_t blocks = c.tiles * heads, want = 2048 / waves, walked = (walk + TILE - 1) / TILE;
   uint64_t splits = blocks ? want / blocks : 1;
   splits = std::max<uint64_t>(1, std::min(splits, walked / 4));
   const uint64_t per = std::max<uint64_t>(1, (walked + splits - 1) / splits);
   c.run = (int)(per * TILE);
   c.splits = (uint32_t)std::max<uint64_t>(1, (walked + per - 1) / per);
+  c.blocks = (uint32_t)std::min<uint64_t>(blocks * c.splits, 0xFFFFFFFFu);
+  c.div_tiles = fast_div(std::max(1u, c.tiles));
+  c.div_splits = fast_div(c.splits);
   return c;
 }
 
 struct Layout {
-  Cut kv, q;
+  int waves;
+  Side kv, rows;
   size_t stats, dq, dkv;  // floats of each part of the workspace
   size_t total() const { return 2 * stats + dq + 2 * dkv; }
 };
 Layout layout(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
   Layout l;
-  const uint64_t R = (uint64_t)Tq * (Hq / Hkv);
-  l.kv = cut((uint64_t)B * Hkv, Tk, R);
-  l.q = cut((uint64_t)B * Hkv, R, Tk);
+  const uint64_t R = (uint64_t)Tq * (Hq / Hkv), heads = (uint64_t)B * Hkv, most = std::max<uint64_t>(R, Tk);
+  l.waves = most <= 32 ? 1 : most <= 64 ? 2 : 4;
+  l.kv = cut(l.waves, heads, Tk, R);
+  l.rows = cut(l.waves, heads, R, Tk);
   l.stats = ((size_t)B * Hq * Tq + 3) / 4 * 4;
-  l.dq = l.q.splits > 1 ? (size_t)l.q.splits * B * Hq * Tq * D : 0;
+  l.dq = l.rows.splits > 1 ? (size_t)l.rows.splits * B * Hq * Tq * D : 0;
   l.dkv = l.kv.splits > 1 ? (size_t)l.kv.splits * B * Hkv * Tk * D : 0;
   return l;
 }
 
-void set(BwdParams& p, const Cut& c, uint64_t heads) {
-  p.blocks = (uint32_t)(c.tiles * c.splits * heads);
-  p.tiles = c.tiles;
-  p.splits = c.splits;
-  p.run = c.run;
-  p.div_tiles = fast_div(c.tiles);
-  p.div_splits = fast_div(c.splits);
-}
-
 template <typename E, int DB>
-void launch_kv(const BwdParams& p, int waves, hipStream_t s) {
-  constexpr size_t lds = 2 * (2 * Tile<DB == 3 ? 128 : DB * 32>::BYTES + 2 * TILE * 4);
+void launch_sides(const BwdParams& p, int waves, hipStream_t s) {
+  constexpr size_t lds = 2 * (2 * Tile<DB == 3 ? 128 : DB * 32>::BYTES + 2 * TILE * 4);  // the keys' side, which has the rows' numbers beside its tiles
   auto go = [&](auto kernel) {
     if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    kernel<<<dim3(p.blocks), dim3(waves * 64), lds, s>>>(p);
+    kernel<<<dim3(p.rows.blocks + p.kv.blocks), dim3(waves * 64), lds, s>>>(p);
   };
-  if (waves == 1) go(attention_dkv_kernel<E, DB, 1>);
-  else if (waves == 2) go(attention_dkv_kernel<E, DB, 2>);
-  else go(attention_dkv_kernel<E, DB, 4>);
-}
-
-template <typename E, int DB>
-void launch_q(const BwdParams& p, int waves, hipStream_t s) {
-  constexpr size_t lds = 4 * Tile<DB == 3 ? 128 : DB * 32>::BYTES;
-  if (waves == 1) attention_dq_kernel<E, DB, 1><<<dim3(p.blocks), dim3(64), lds, s>>>(p);
-  else if (waves == 2) attention_dq_kernel<E, DB, 2><<<dim3(p.blocks), dim3(128), lds, s>>>(p);
-  else attention_dq_kernel<E, DB, 4><<<dim3(p.blocks), dim3(256), lds, s>>>(p);
+  if (waves == 1) go(attention_bwd_kernel<E, DB, 1>);
+  else if (waves == 2) go(attention_bwd_kernel<E, DB, 2>);
+  else go(attention_bwd_kernel<E, DB, 4>);
 }
 
 template <typename E>
-int launch(BwdParams& p, const Layout& l, int B, hipStream_t s) {
+int launch(const BwdParams& p, int waves, hipStream_t s) {
   const AttnShape& a = p.a;
-  const uint64_t heads = (uint64_t)B * a.Hkv;
   const int db = (a.D + 31) / 32;
   if (a.R) {
-    const uint32_t rows = (uint32_t)B * a.Hq * a.Tq;
+    const uint32_t rows = p.heads * a.R;
     attention_stats_kernel<E><<<dim3((rows + 15) / 16), dim3(256), 0, s>>>(p, rows);
     SA_LAUNCH_CHECK();
   }
-  if (a.Tk) {
-    set(p, l.kv, heads);
-    if (db == 1) launch_kv<E, 1>(p, l.kv.waves, s);
-    else if (db == 2) launch_kv<E, 2>(p, l.kv.waves, s);
-    else if (db == 3) launch_kv<E, 3>(p, l.kv.waves, s);
-    else launch_kv<E, 4>(p, l.kv.waves, s);
+  if (p.rows.blocks + p.kv.blocks == 0) return SA_OK;
+  if (db == 1) launch_sides<E, 1>(p, waves, s);
+  else if (db == 2) launch_sides<E, 2>(p, waves, s);
+  else if (db == 3) launch_sides<E, 3>(p, waves, s);
+  else launch_sides<E, 4>(p, waves, s);
+  SA_LAUNCH_CHECK();
+  AddParams add = {};
+  uint32_t blocks = 0;
+  auto sum = [&](int k, const float* part, void* dst, uint64_t tokens, uint32_t splits) {
+    add.first[k] = blocks;
+    if (!part) return;
+    add.part[k] = part;
+    add.dst[k] = dst;
+    add.n[k] = (int64_t)(p.heads * tokens * a.D);
+    add.splits[k] = (int)splits;
+    blocks += (uint32_t)((add.n[k] / 8 + 255) / 256);
+  };
+  sum(0, p.part_dk, p.dk, a.Tk, p.kv.splits);
+  sum(1, p.part_dv, p.dv, a.Tk, p.kv.splits);
+  sum(2, p.part_dq, p.dq, a.R, p.rows.splits);
+  if (blocks) {
+    attention_add_kernel<E><<<dim3(blocks), dim3(256), 0, s>>>(add);
     SA_LAUNCH_CHECK();
-    if (p.part_dk) {
-      const int64_t n = (int64_t)heads * a.Tk * a.D;
-      const dim3 grid((uint32_t)((n / 8 + 255) / 256));
-      attention_add_kernel<E><<<grid, dim3(256), 0, s>>>(p.part_dk, static_cast<E*>(p.dk), n, (int)l.kv.splits);
-      attention_add_kernel<E><<<grid, dim3(256), 0, s>>>(p.part_dv, static_cast<E*>(p.dv), n, (int)l.kv.splits);
-      SA_LAUNCH_CHECK();
-    }
-  }
-  if (a.R) {
-    set(p, l.q, heads);
-    if (db == 1) launch_q<E, 1>(p, l.q.waves, s);
-    else if (db == 2) launch_q<E, 2>(p, l.q.waves, s);
-    else if (db == 3) launch_q<E, 3>(p, l.q.waves, s);
-    else launch_q<E, 4>(p, l.q.waves, s);
-    SA_LAUNCH_CHECK();
-    if (p.part_dq) {
-      const int64_t n = (int64_t)heads * a.R * a.D;
-      attention_add_kernel<E><<<dim3((uint32_t)((n / 8 + 255) / 256)), dim3(256), 0, s>>>(p.part_dq, static_cast<E*>(p.dq), n, (int)l.q.splits);
-      SA_LAUNCH_CHECK();
-    }
   }
   return SA_OK;
 }
@@ -469,9 +471,7 @@ extern "C" int sa_cross_attention_backward(const void* q, const void* k, const v
   SA_REQUIRE(TILE * strides[1] + G * strides[2] < far && TILE * dout_strides[1] + G * dout_strides[2] < far,
              "%s: 64 tokens and the heads on one key head span less than 2^30 elements of q and of dout", who);
   const Layout l = layout(B, Tq, Tk, Hq, Hkv, D);
-  const uint64_t heads = (uint64_t)B * Hkv, most = 1ull << 31;
-  SA_REQUIRE((uint64_t)l.kv.tiles * l.kv.splits * heads < most && (uint64_t)l.q.tiles * l.q.splits * heads < most && (uint64_t)B * Hq * Tq < most - 1024,
-             "%s: too many rows", who);
+  SA_REQUIRE((uint64_t)l.kv.blocks + l.rows.blocks < (1ull << 31) && (uint64_t)B * Hq * Tq < (1ull << 31) - 1024 && (uint64_t)B * Hkv < (1ull << 31), "%s: too many rows", who);
   if (workspace_bytes < l.total() * sizeof(float)) return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", who, workspace_bytes);
   p.out = out;
   p.dout = dout;
@@ -488,7 +488,10 @@ extern "C" int sa_cross_attention_backward(const void* q, const void* k, const v
   p.part_dq = l.dq ? w + 2 * l.stats : nullptr;
   p.part_dk = l.dkv ? w + 2 * l.stats + l.dq : nullptr;
   p.part_dv = l.dkv ? w + 2 * l.stats + l.dq + l.dkv : nullptr;
+  p.kv = l.kv;
+  p.rows = l.rows;
+  p.heads = (uint32_t)B * Hkv;
   p.div_heads = fast_div(Hkv);
   p.div_hq = fast_div(Hq);
-  return dtype == SA_F16 ? launch<_Float16>(p, l, B, (hipStream_t)stream) : launch<__bf16>(p, l, B, (hipStream_t)stream);
+  return dtype == SA_F16 ? launch<_Float16>(p, l.waves, (hipStream_t)stream) : launch<__bf16>(p, l.waves, (hipStream_t)stream);
 }
