@@ -165,10 +165,21 @@ __device__ __forceinline__ void hide(f32x16& s, uint32_t seen, int h) {
   }
 }
 
-// workgroups that read the same keys are neighbours in `id`: give each of the eight XCDs (workgroups go round them) a run of ids
-__device__ __forceinline__ uint32_t xcd_run(uint32_t block, uint32_t n) {
-  const uint32_t x = block & 7, q = n >> 3, r = n & 7;
-  return x * q + min(x, r) + (block >> 3);
+// Which head and which of its `per` pieces of work a workgroup has. Workgroups go round the eight XCDs, each with its own L2: all pieces
+// of a head, which read the same keys (rows), go to one XCD, and heads go round the XCDs, so that images with few keys or none, whose
+// heads are neighbours, leave no XCD idle. What is left of the heads after whole rounds is cut into eight runs of pieces.
+struct Piece {
+  uint32_t head, at;
+};
+__device__ __forceinline__ Piece piece_of(uint32_t block, uint32_t heads, uint32_t per, const FastDiv& div_per) {
+  const uint32_t whole = (heads & ~7u) * per, x = block & 7;
+  if (block < whole) {
+    const uint32_t slot = block >> 3, round = div_by(slot, div_per);
+    return {round * 8 + x, slot - round * per};
+  }
+  const uint32_t n = (heads & 7) * per, q = n >> 3, r = n & 7;
+  const uint32_t id = x * q + min(x, r) + ((block - whole) >> 3), head = div_by(id, div_per);
+  return {(heads & ~7u) + head, id - head * per};
 }
 
 // what forward and backward know of a call

@@ -13,8 +13,8 @@ struct FwdParams {
   float* lse;             // [B, Hq, Tq] natural logarithm of the softmax's denominator, or NULL
   float* part;            // splits > 1: [B * Hkv][splits][R][D] of each run of keys, normalised
   float* part_lse;        // and their base-2 logarithms [B * Hkv][splits][R]
-  uint32_t blocks, row_tiles, splits;
-  FastDiv div_tiles, div_splits, div_heads;
+  uint32_t blocks, heads, row_tiles, splits;  // heads: B * Hkv; blocks: heads * row_tiles * splits
+  FastDiv div_tiles, div_pieces, div_heads;
   int split_keys;         // keys of a run: a multiple of TILE
 };
 
@@ -37,9 +37,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
   extern __shared__ __align__(1024) char lds[];  // [2 stages][k tile, v tile]
   const AttnShape& a = p.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
-  const uint32_t id = xcd_run(blockIdx.x, p.blocks);
-  const uint32_t bhs = div_by(id, p.div_tiles), tile = id - bhs * p.row_tiles;
-  const uint32_t bh = div_by(bhs, p.div_splits), split = bhs - bh * p.splits;
+  const Piece piece = piece_of(blockIdx.x, p.heads, p.row_tiles * p.splits, p.div_pieces);
+  const uint32_t bh = piece.head, split = div_by(piece.at, p.div_tiles), tile = piece.at - split * p.row_tiles;
   const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv;
 
   const uint32_t row = tile * (NW * 32) + wave * 32 + n;
@@ -279,7 +278,7 @@ void launch_e(const FwdParams& p, int waves, hipStream_t s) {
   else if (db == 3) launch<E, 3>(p, waves, s);
   else launch<E, 4>(p, waves, s);
   if (p.splits > 1) {
-    const uint32_t rows = p.blocks / p.row_tiles / p.splits * p.a.R;
+    const uint32_t rows = p.heads * p.a.R;
     uint32_t log2 = 0;
     while (log2 < 4 && (4u << log2) < p.splits) ++log2;  // four runs a group
     const uint32_t per = 16 >> log2;
@@ -353,7 +352,8 @@ extern "C" int sa_cross_attention(const void* q, const void* k, const void* v, i
   p.splits = c.splits;
   p.split_keys = c.split_keys;
   p.div_tiles = fast_div(c.row_tiles);
-  p.div_splits = fast_div(c.splits);
+  p.heads = (uint32_t)B * Hkv;
+  p.div_pieces = fast_div(c.row_tiles * c.splits);
   p.div_heads = fast_div(Hkv);
   if (dtype == SA_F16) launch_e<_Float16>(p, c.waves, (hipStream_t)stream);
   else launch_e<__bf16>(p, c.waves, (hipStream_t)stream);

@@ -15,7 +15,7 @@ using namespace sa;
 struct Side {
   uint32_t blocks, tiles, splits;  // workgroups; of them along the owned side, along the walked side
   int run;                         // rows (keys) of a run: a multiple of TILE
-  FastDiv div_tiles, div_splits;
+  FastDiv div_tiles, div_pieces;
 };
 
 struct BwdParams {
@@ -139,9 +139,8 @@ __device__ __forceinline__ void keys_side(const BwdParams& p, uint32_t block, ch
   const AttnShape& a = p.a;
   const Side& side = p.kv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
-  const uint32_t id = xcd_run(block, side.blocks);
-  const uint32_t bhs = div_by(id, side.div_tiles), tile = id - bhs * side.tiles;
-  const uint32_t bh = div_by(bhs, side.div_splits), split = bhs - bh * side.splits;
+  const Piece piece = piece_of(block, p.heads, side.tiles * side.splits, side.div_pieces);
+  const uint32_t bh = piece.head, split = div_by(piece.at, side.div_tiles), tile = piece.at - split * side.tiles;
   const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv;
 
   int length = a.Tk;
@@ -243,9 +242,8 @@ __device__ __forceinline__ void rows_side(const BwdParams& p, uint32_t block, ch
   const AttnShape& a = p.a;
   const Side& side = p.rows;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
-  const uint32_t id = xcd_run(block, side.blocks);
-  const uint32_t bhs = div_by(id, side.div_tiles), tile = id - bhs * side.tiles;
-  const uint32_t bh = div_by(bhs, side.div_splits), split = bhs - bh * side.splits;
+  const Piece piece = piece_of(block, p.heads, side.tiles * side.splits, side.div_pieces);
+  const uint32_t bh = piece.head, split = div_by(piece.at, side.div_tiles), tile = piece.at - split * side.tiles;
   const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv;
 
   const uint32_t row = tile * (NW * 32) + wave * 32 + n;
@@ -379,7 +377,7 @@ Side cut(int waves, uint64_t heads, uint64_t own, uint64_t walk) {
   c.splits = (uint32_t)std::max<uint64_t>(1, (walked + per - 1) / per);
   c.blocks = (uint32_t)std::min<uint64_t>(blocks * c.splits, 0xFFFFFFFFu);
   c.div_tiles = fast_div(std::max(1u, c.tiles));
-  c.div_splits = fast_div(c.splits);
+  c.div_pieces = fast_div(std::max(1u, c.tiles * c.splits));
   return c;
 }
 
