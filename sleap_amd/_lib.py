@@ -201,6 +201,28 @@ def lib(dtype: str = None):
     return h
 
 
+def token_host():
+    """The C++ host side of the token operators (csrc/token_host.cpp), built beside the libraries; raises if it can not be loaded."""
+    import importlib.machinery
+    import importlib.util
+
+    import torch  # noqa: F401  (its libraries are what the module links against)
+
+    from . import build as _build
+
+    path = _build.HOST
+    if not os.path.exists(path):
+        try:
+            _build.build_host(verbose=False)
+        except Exception as e:  # noqa: BLE001
+            raise ImportError(f"{os.path.basename(path)} not found at {path} and could not be built ({e}); run `python -m sleap_amd.build` "
+                              "(needs g++ and torch's headers). There is no fallback.") from e
+    spec = importlib.util.spec_from_file_location(_build.HOST_MODULE, path, loader=importlib.machinery.ExtensionFileLoader(_build.HOST_MODULE, path))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
 def check(code, what=""):
     if code != SA_OK:
         msg = lib().sa_last_error()

@@ -13,6 +13,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libsleap_amd.so")
+HOST_MODULE = "_token_host"
+HOST = os.path.join(LIBDIR, HOST_MODULE + ".so")
 ARCH = "gfx950"
 
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]  # the host pass says that it does not know it: harmless
@@ -106,10 +108,38 @@ def _build_variant(dtype, force, verbose):
 def build(force=False, verbose=True, dtypes=("bf16", "fp16")):
     """Compile every storage-type variant (fp16 = the default the Python layer loads, bf16); returns the path of the bf16
     library file (`libsleap_amd.so`, the historical name)."""
+    from concurrent.futures import ThreadPoolExecutor
+
     os.makedirs(LIBDIR, exist_ok=True)
-    for d in dtypes:
-        _build_variant(d, force, verbose)
+    with ThreadPoolExecutor(max_workers=1) as ex:  # host code, beside the device compilations
+        host = ex.submit(build_host, force, verbose)
+        for d in dtypes:
+            _build_variant(d, force, verbose)
+        host.result()
     return LIB
+
+
+def build_host(force=False, verbose=True):
+    """The host side of the token operators (csrc/token_host.cpp): a Python module on torch's C++ interface, host code only."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    src = os.path.join(CSRC, "token_host.cpp")
+    newest = max(os.path.getmtime(f) for f in (src, os.path.join(HERE, "..", "include", "sleap_amd.h")))
+    if not force and os.path.exists(HOST) and os.path.getmtime(HOST) >= newest:
+        return HOST
+    os.makedirs(LIBDIR, exist_ok=True)
+    include = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", src, "-o", HOST, "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-DTORCH_EXTENSION_NAME={HOST_MODULE}", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[a for p in include for a in ("-isystem", p)], "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-ltorch_cpu",
+           "-ltorch_python", "-lc10_hip"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return HOST
 
 
 if __name__ == "__main__":

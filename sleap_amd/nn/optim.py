@@ -25,7 +25,7 @@ class AdamW(torch.optim.Optimizer):
         if len({id(p) for p in params}) != len(params):
             raise ValueError("AdamW: the same parameter twice in a group")
         for p in params:
-            if not isinstance(p, torch.Tensor) or not p.is_cuda or p.dtype not in ops._TOKEN_TYPES or not p.is_contiguous():
+            if not isinstance(p, torch.Tensor) or not p.is_cuda or p.dtype not in (torch.float32, torch.float16, torch.bfloat16) or not p.is_contiguous():
                 raise ValueError("AdamW: parameters are contiguous float32, float16 or bfloat16 CUDA tensors (there is no CPU fallback)")
         super().add_param_group({**group, "params": params})
 

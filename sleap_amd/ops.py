@@ -5,7 +5,6 @@ torch stream. Shapes and meanings follow include/sleap_amd.h.
 """
 import collections
 import ctypes as C
-import math
 
 import numpy as np
 import torch
@@ -402,81 +401,21 @@ def optical_flow_pyr_lk(prev: "FlowPyramid", nxt: "FlowPyramid", points, max_cou
 
 # --------------------------------------------------------------------------------------------------
 # token operators (csrc/rotary.hip, attention.hip, attention_bwd.hip, adamw.hip): keypoint queries and feature-map tokens. Unlike the
-# layer wrappers above they take any torch layout, check their arguments, run on the device of their tensors and have gradients.
+# layer wrappers above they take any torch layout, check their arguments, run on the device of their tensors and have gradients; their
+# host side is C++ (csrc/token_host.cpp), which calls the same C ABI.
 # --------------------------------------------------------------------------------------------------
-_TOKEN_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # SA_F32, SA_F16, SA_BF16
-_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}     # SA_POS_*
-_I3, _I9 = C.c_int64 * 3, C.c_int64 * 9
+_token_host = None
 
 
-def _launch(name, index, *args):
-    """One C call on the tensors' own device `index` and its current stream. (The raw accessors: what torch.cuda.current_stream and
-    current_device wrap, without building their objects -- 2 of the 15 us that a small call costs its host.)"""
-    fn = getattr(_lib.lib(), name)
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        check(rc, name)
-
-
-def _cuda_tensors(who, names, tensors):
-    index = None
-    for t, name in zip(tensors, names):
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise ValueError(f"{who}: {name} must be a CUDA tensor (there is no CPU fallback)")
-        if index is None:
-            index = t.get_device()
-        elif t.get_device() != index:
-            raise ValueError(f"{who}: {name} is on {t.device}, not on cuda:{index}")
-    return index
-
-
-def _token_layout(t, elements, limit=None, group=0):
-    """A (B, T, heads, D) tensor as the kernels take it -> (tensor, [batch, token, head] strides in elements, 0 where there is nothing to
-    step over): `t` itself if its last dimension is contiguous, every other stride and the address are whole multiples of `elements`
-    values and (limit, group: see the callers) 64 tokens and `group` heads span less than `limit`; else a contiguous copy."""
-    for _ in range(2):
-        (nb, nt, nh, nd), (b, n, h, one) = t.shape, t.stride()
-        b, n, h = b if nb > 1 else 0, n if nt > 1 else 0, h if nh > 1 else 0
-        if (one == 1 or nd == 1) and not (b % elements or n % elements or h % elements or t.data_ptr() % (elements * t.element_size())) and (
-                limit is None or 64 * n + group * h < limit) or nb * nt * nh * nd == 0:
-            break
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t, (b, n, h)
-
-
-def _rotary_call(x, positions, sections, theta, ladder, interleaved, inverse):
-    x, strides = _token_layout(x, 2 if interleaved else 1)
-    B, T, H, D = x.shape
-    y = torch.empty((B, T, H, D), dtype=x.dtype, device=x.device)
-    if B and T:
-        places = positions.stride() if positions.dim() == 3 and positions.shape[0] > 1 else (0, *positions.stride()[-2:])
-        n = len(sections)
-        _launch("sa_rotary_axes", x.get_device(), x.data_ptr(), _TOKEN_TYPES[x.dtype], B, T, H, D, _I3(*strides), positions.data_ptr(),
-                _POSITION_TYPES[positions.dtype], _I3(*places), n, (C.c_int * n)(*sections), theta, ladder == "shared", interleaved, inverse,
-                y.data_ptr())
-    return y
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, positions, sections, theta, ladder, interleaved, inverse):
-        ctx.save_for_backward(positions)
-        ctx.how = (sections, theta, ladder, interleaved, inverse)
-        return _rotary_call(x, positions, *ctx.how)
-
-    @staticmethod
-    def backward(ctx, dy):
-        (positions,) = ctx.saved_tensors
-        sections, theta, ladder, interleaved, inverse = ctx.how
-        how = (sections, theta, ladder, interleaved, not inverse)  # linear in x: its gradient is the turn the other way ...
-        dx = _Rotary.apply(dy, positions, *how) if dy.requires_grad and torch.is_grad_enabled() else _rotary_call(dy, positions, *how)
-        return dx, None, None, None, None, None, None  # ... which has a gradient again
+def _token():
+    global _token_host
+    if _token_host is None:
+        host, h = _lib.token_host(), _lib.lib()
+        names = ("sa_last_error", "sa_rotary_axes", "sa_cross_attention_workspace", "sa_cross_attention", "sa_cross_attention_backward_workspace",
+                 "sa_cross_attention_backward", "sa_adamw_step")
+        host.bind({n: C.cast(getattr(h, n), C.c_void_p).value for n in names}, _lib.SleapAmdError)
+        _token_host = host
+    return _token_host
 
 
 def rotary_axes(x, positions, sections, theta=10000.0, ladder="axis", interleaved=False, inverse=False):
@@ -490,120 +429,7 @@ def rotary_axes(x, positions, sections, theta=10000.0, ladder="axis", interleave
     interleaved pairs are (2j, 2j + 1) instead of (j, j + P)
     inverse     turn the other way
     Differentiable in x."""
-    _cuda_tensors("rotary_axes", ("x", "positions"), (x, positions))
-    if x.dim() != 4 or x.shape[3] % 2 or x.shape[3] < 2 or x.shape[3] > 4096 or not 1 <= x.shape[2] <= 4096:
-        raise ValueError(f"rotary_axes: x must be (B, T, heads, even size): got {tuple(x.shape)}")
-    if x.dtype not in _TOKEN_TYPES:
-        raise TypeError(f"rotary_axes: x must be float32, float16 or bfloat16: got {x.dtype}")
-    if positions.dtype not in _POSITION_TYPES:
-        raise TypeError(f"rotary_axes: positions must be int32, int64 or float32: got {positions.dtype}")
-    sections = tuple(int(n) for n in sections)
-    B, T, _, D = x.shape
-    if not 1 <= len(sections) <= 8 or min(sections) < 0 or not 1 <= sum(sections) <= min(D // 2, 128):
-        raise ValueError(f"rotary_axes: sections {sections} do not fit a head of {D} (at most 8 axes and 128 pairs of two values)")
-    if tuple(positions.shape) not in ((T, len(sections)), (B, T, len(sections)), (1, T, len(sections))):
-        raise ValueError(f"rotary_axes: positions {tuple(positions.shape)} for {B} x {T} tokens and {len(sections)} axes")
-    if ladder not in ("axis", "shared"):
-        raise ValueError(f"rotary_axes: ladder {ladder!r}: 'axis' or 'shared'")
-    if not 0 < theta < 1e30:
-        raise ValueError(f"rotary_axes: theta {theta}")
-    if positions.requires_grad:
-        raise ValueError("rotary_axes: there is no gradient for positions")
-    how = (sections, float(theta), ladder, bool(interleaved), bool(inverse))
-    if x.requires_grad and torch.is_grad_enabled():
-        return _Rotary.apply(x, positions, *how)
-    return _rotary_call(x, positions, *how)
-
-
-# What the attention kernels address from one 64-bit base with 32 bits: 64 tokens of keys or values, and in the backward pass 64 tokens
-# and the heads on one key head of q and dout, in elements. Wider layouts are copied.
-_KEY_SPAN, _ROW_SPAN = 64 << 23, 1 << 30
-
-
-def _attention_args(q, k, v, sq, sk, sv, lengths, mask, scale):
-    B, Tq, H, D = q.shape
-    if mask is None:
-        m, sm = None, None
-    else:
-        m, sm = mask.data_ptr(), _I3(mask.stride(0) if mask.shape[0] > 1 else 0, mask.stride(1), 0)
-    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), _TOKEN_TYPES[q.dtype], B, Tq, k.shape[1], H, k.shape[2], D, _I9(*sq, *sk, *sv),
-            None if lengths is None else lengths.data_ptr(), m, sm, scale)
-
-
-def _workspace(name, q, k):
-    """Scratch of this call alone: the allocator orders its next use, and a captured graph has its own."""
-    B, Tq, H, D = q.shape
-    n = getattr(_lib.lib(), name)(B, Tq, k.shape[1], H, k.shape[2], D)
-    return torch.empty((n,), dtype=torch.uint8, device=q.device) if n else None, n
-
-
-def _attention_forward(q, k, v, lengths, mask, scale, want_lse):
-    (q, sq), (k, sk), (v, sv) = _token_layout(q, 8), _token_layout(k, 8, _KEY_SPAN), _token_layout(v, 8, _KEY_SPAN)
-    B, Tq, H, D = q.shape
-    out = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
-    if B and Tq:
-        ws, n = _workspace("sa_cross_attention_workspace", q, k)
-        _launch("sa_cross_attention", q.get_device(), *_attention_args(q, k, v, sq, sk, sv, lengths, mask, scale), out.data_ptr(),
-                lse.data_ptr() if want_lse else None, ws.data_ptr() if n else None, n)
-    return out, lse
-
-
-def _attention_backward(dout, q, k, v, out, lse, lengths, mask, scale):
-    group = q.shape[2] // k.shape[2]
-    (q, sq), (k, sk), (v, sv) = _token_layout(q, 8, _ROW_SPAN, group), _token_layout(k, 8, _KEY_SPAN), _token_layout(v, 8, _KEY_SPAN)
-    dout, so = _token_layout(dout, 8, _ROW_SPAN, group)
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    if dq.numel() or dk.numel():
-        ws, n = _workspace("sa_cross_attention_backward_workspace", q, k)
-        _launch("sa_cross_attention_backward", q.get_device(), *_attention_args(q, k, v, sq, sk, sv, lengths, mask, scale), out.data_ptr(),
-                lse.data_ptr(), dout.data_ptr(), _I3(*so), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr() if n else None, n)
-    return dq, dk, dv
-
-
-class _CrossAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, lengths, mask, scale):
-        out, lse = _attention_forward(q, k, v, lengths, mask, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths, mask)
-        ctx.scale = scale
-        ctx.mark_non_differentiable(lse)
-        ctx.set_materialize_grads(False)
-        return out, lse
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, _):
-        if dout is None:
-            return None, None, None, None, None, None
-        return (*_attention_backward(dout, *ctx.saved_tensors, ctx.scale), None, None, None)
-
-
-def _attention_checks(who, q, k, v, key_lengths, key_mask, scale):
-    """-> (key_lengths as contiguous int32, scale as a number) of a call that the kernels can take"""
-    _cuda_tensors(who, ("q", "k", "v", "key_lengths", "key_mask"), (q, k, v, key_lengths, key_mask))
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise ValueError(f"{who}: q (B, Tq, heads, D), k and v (B, Tk, key heads, D): got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"{who}: q, k and v must all be float16 or all bfloat16: got {q.dtype}, {k.dtype}, {v.dtype}")
-    B, _, H, D = q.shape
-    Tk, K = k.shape[1:3]
-    if D % 8 or not 8 <= D <= 128:
-        raise ValueError(f"{who}: head size {D}: a multiple of 8, at most 128")
-    if H < 1 or K < 1 or H % K:
-        raise ValueError(f"{who}: {H} query heads do not share {K} key heads evenly")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 1e-30 <= scale <= 1e30:
-        raise ValueError(f"{who}: scale {scale} must be positive and finite")
-    if key_lengths is not None:
-        if key_lengths.dtype not in (torch.int32, torch.int64) or key_lengths.shape != (B,):
-            raise ValueError(f"{who}: key_lengths must be ({B},) int32 or int64: got {tuple(key_lengths.shape)} {key_lengths.dtype}")
-        if key_lengths.dtype == torch.int64:
-            key_lengths = key_lengths.clamp(0, Tk).to(torch.int32)
-        key_lengths = key_lengths.contiguous()
-    if key_mask is not None and (key_mask.dtype != torch.bool or key_mask.shape not in ((B, Tk), (1, Tk))):
-        raise ValueError(f"{who}: key_mask must be ({B}, {Tk}) bool, True where a key is visible: got {tuple(key_mask.shape)} {key_mask.dtype}")
-    return key_lengths, scale
+    return _token().rotary_axes(x, positions, sections, theta, ladder, interleaved, inverse)
 
 
 def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, return_lse=False):
@@ -617,12 +443,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, return
     return_lse   also the natural logarithm of the softmax's denominators, (B, H, Tq) float32, without a gradient
     A query that sees no key gives zeros (lse: -inf) and passes no gradient. Softmax and sums are float32, weights are rounded to q's
     type before the product with v; results do not depend on the order in which workgroups run. Differentiable in q, k and v, once."""
-    key_lengths, scale = _attention_checks("cross_attention", q, k, v, key_lengths, key_mask, scale)
-    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        out, lse = _CrossAttention.apply(q, k, v, key_lengths, key_mask, scale)
-    else:
-        out, lse = _attention_forward(q, k, v, key_lengths, key_mask, scale, return_lse)
-    return (out, lse) if return_lse else out
+    return _token().cross_attention(q, k, v, key_lengths, key_mask, scale, return_lse)
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_exp_avg_sqs=None):
@@ -636,60 +457,4 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
     exp_avgs, exp_avg_sqs, max_exp_avg_sqs (amsgrad, or None)   float32 tensors of the same sizes
     step            t >= 1, or a one-element int64 CUDA tensor that already holds it; lr likewise a number or a one-element float32 CUDA
                     tensor. A captured step takes its count as a tensor only, and a learning rate given as a number stays that of the capture."""
-    lists = [params, grads, exp_avgs, exp_avg_sqs] + ([max_exp_avg_sqs] if max_exp_avg_sqs is not None else [])
-    lists = [list(x) for x in lists]
-    n = len(lists[0])
-    if any(len(x) != n for x in lists):
-        raise ValueError(f"adamw_step: lists of {[len(x) for x in lists]} tensors")
-    if n == 0:
-        return
-    dev_step, dev_lr = isinstance(step, torch.Tensor), isinstance(lr, torch.Tensor)
-    if dev_step and (step.dtype != torch.int64 or step.numel() != 1) or dev_lr and (lr.dtype != torch.float32 or lr.numel() != 1):
-        raise ValueError("adamw_step: a step tensor is one int64, a learning rate tensor one float32")
-    if not dev_step and int(step) < 1:
-        raise ValueError(f"adamw_step: step {step}: the first is 1")
-    b1, b2 = (float(b) for b in betas)
-    if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0 and weight_decay >= 0 and (dev_lr or lr >= 0)):
-        raise ValueError(f"adamw_step: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
-    # Hundreds of tensors in five lists: each property is read by one map() over its C accessor (the checks of 448 tensors take the host as
-    # long as the step of their 66 M values takes the GPU).
-    Tensor, kinds = torch.Tensor, ("params", "grads", "exp_avgs", "exp_avg_sqs", "max_exp_avg_sqs")
-    try:
-        sizes = list(map(Tensor.numel, lists[0]))
-        where = list(map(Tensor.get_device, lists[0]))
-        types = [t.dtype for t in lists[0]]
-        for x, kind in zip(lists, kinds):
-            if x is not lists[0] and list(map(Tensor.numel, x)) != sizes:
-                raise ValueError(f"adamw_step: {kind} differ in size from params")
-            if not all(map(Tensor.is_contiguous, x)):
-                raise ValueError(f"adamw_step: {kind} must be contiguous")
-            if min(where) < 0 or x is not lists[0] and list(map(Tensor.get_device, x)) != where:
-                raise ValueError("adamw_step: CUDA tensors, a parameter, its gradient and its states on one GPU (there is no CPU fallback)")
-    except TypeError as e:
-        raise ValueError(f"adamw_step: lists of CUDA tensors (there is no CPU fallback): {e}") from e
-    if [t.dtype for t in lists[1]] != types or not all(t in _TOKEN_TYPES for t in set(types)):
-        raise TypeError("adamw_step: params and grads must be pairs of one type: float32, float16 or bfloat16")
-    if {t.dtype for x in lists[2:] for t in x} != {torch.float32}:
-        raise TypeError("adamw_step: the states must be float32")
-    if dev_step and step.get_device() not in where or dev_lr and lr.get_device() not in where or (dev_step or dev_lr) and len(set(where)) > 1:
-        raise ValueError("adamw_step: step and learning rate tensors must be on the GPU of the parameters")
-    if not dev_step and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("adamw_step: a captured step needs its count as a tensor (every replay would repeat this one)")
-    table = np.zeros((n, 6), np.int64)  # sa_adamw_tensor
-    for j, x in enumerate(lists):
-        table[:, j] = list(map(Tensor.data_ptr, x))
-    table[:, 5] = sizes
-    held = [p for p, k in zip(table[:, 0].tolist(), sizes) if k]
-    if len(set(held)) != len(held):
-        raise ValueError("adamw_step: the same parameter twice")
-    groups = {}
-    if len(set(types)) == 1 and len(set(where)) == 1:
-        groups[types[0], where[0]] = table
-    else:
-        for i, key in enumerate(zip(types, where)):
-            groups.setdefault(key, []).append(i)
-        groups = {key: np.ascontiguousarray(table[rows]) for key, rows in groups.items()}
-    for (dtype, index), t in groups.items():
-        _launch("sa_adamw_step", index, t.ctypes.data, len(t), _TOKEN_TYPES[dtype], int(len(lists) == 5),
-                0.0 if dev_lr else float(lr), lr.data_ptr() if dev_lr else None, b1, b2, float(eps), float(weight_decay),
-                1 if dev_step else int(step), step.data_ptr() if dev_step else None)
+    _token().adamw_step(params, grads, exp_avgs, exp_avg_sqs, max_exp_avg_sqs, step, lr, betas, eps, weight_decay)
