@@ -86,6 +86,32 @@ __device__ __forceinline__ float sum_halves(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Column n of a transposed result (C registers: rows d) as a row of D values, n 32-row blocks of `acc` times `by`: 16-bit to dst, or float32
+// to `part`. A lane has four values of each eight and its half-wave's partner the other four: one exchange of two dwords gives each
+// lane eight neighbours, so that it stores 16 bytes.
+template <typename E, int N>
+__device__ __forceinline__ void store_row(E* dst, float* part, const f32x16 (&acc)[N], int D, int h, float by) {
+#pragma unroll
+  for (int db = 0; db < N; ++db)
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const f32x16& x = acc[db];
+      if (part) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = 4 * (j + e), d = db * 32 + (j + e) * 8 + h * 4;
+          if (d < D) *reinterpret_cast<f32x4*>(part + d) = f32x4{x[i] * by, x[i + 1] * by, x[i + 2] * by, x[i + 3] * by};
+        }
+        continue;
+      }
+      const int i = 4 * j;
+      const auto lo = __builtin_amdgcn_permlane32_swap(pack2<E>(x[i] * by, x[i + 1] * by), pack2<E>(x[i + 4] * by, x[i + 5] * by), false, false);
+      const auto hi = __builtin_amdgcn_permlane32_swap(pack2<E>(x[i + 2] * by, x[i + 3] * by), pack2<E>(x[i + 6] * by, x[i + 7] * by), false, false);
+      const int d = db * 32 + (j + h) * 8;
+      if (d < D) *reinterpret_cast<u32x4*>(dst + d) = u32x4{lo[0], hi[0], lo[1], hi[1]};
+    }
+}
+
 template <int DP>
 __device__ __host__ constexpr int swizzle(int row) {
   constexpr int PER_LINE = 128 / DP, PAIRS = DP / 16;  // rows of 256 bytes, 32-byte pairs of a row

@@ -146,29 +146,16 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
 
   l = sum_halves(l);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if (!real) return;
+  E* dst = static_cast<E*>(p.out) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D;
+  float* part = nullptr;
   if (p.splits > 1) {
     const int64_t at = ((int64_t)bh * p.splits + split) * a.R + row;
-    if (h == 0) p.part_lse[at] = l == 0.0f ? -INFINITY : shift + __log2f(l);
-    float* dst = p.part + at * a.D;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int d = db * 32 + j * 8 + h * 4;
-        if (d < a.D) *reinterpret_cast<f32x4*>(dst + d) = f32x4{o[db][4 * j] * inv, o[db][4 * j + 1] * inv, o[db][4 * j + 2] * inv, o[db][4 * j + 3] * inv};
-      }
-    return;
+    if (real && h == 0) p.part_lse[at] = l == 0.0f ? -INFINITY : shift + __log2f(l);
+    part = p.part + at * a.D;
+  } else if (p.lse && real && h == 0) {
+    p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = l == 0.0f ? -INFINITY : (shift + __log2f(l)) * LN2;
   }
-  if (p.lse && h == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = l == 0.0f ? -INFINITY : (shift + __log2f(l)) * LN2;
-  E* dst = static_cast<E*>(p.out) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D;
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = db * 32 + j * 8 + h * 4;
-      if (d < a.D) *reinterpret_cast<u32x2*>(dst + d) = u32x2{pack2<E>(o[db][4 * j] * inv, o[db][4 * j + 1] * inv), pack2<E>(o[db][4 * j + 2] * inv, o[db][4 * j + 3] * inv)};
-    }
+  store_row<E>(dst, part, o, real ? a.D : 0, h, inv);
 }
 
 // Joins the runs of keys: out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max). A row has 16 lanes of 8 values and `groups` of

@@ -117,19 +117,6 @@ __device__ __forceinline__ void copy_rows(char* lds, const Pieces<DP, NW>& at, c
   }
 }
 
-template <typename E>
-__device__ __forceinline__ void store_column(E* dst, float* part, const f32x16* acc, int n, int D, int h, float by) {
-  for (int db = 0; db < n; ++db)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = db * 32 + j * 8 + h * 4;
-      if (d >= D) continue;
-      const f32x4 v = {acc[db][4 * j] * by, acc[db][4 * j + 1] * by, acc[db][4 * j + 2] * by, acc[db][4 * j + 3] * by};
-      if (part) *reinterpret_cast<f32x4*>(part + d) = v;
-      else *reinterpret_cast<u32x2*>(dst + d) = u32x2{pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3])};
-    }
-}
-
 // dk, dv: a wave owns 32 keys (k and v in registers) and walks rows in tiles of 64
 template <typename E, int DB, int NW>
 __device__ __forceinline__ void keys_side(const BwdParams& p, uint32_t block, char* lds) {
@@ -223,15 +210,15 @@ __device__ __forceinline__ void keys_side(const BwdParams& p, uint32_t block, ch
       }
     }
   }
-  if (key >= a.Tk) return;
   if (!seen) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
   }
   const int64_t at = (((int64_t)b * a.Tk + key) * a.Hkv + hk) * a.D;
+  const int D = key < a.Tk ? a.D : 0;  // (both lanes of a key take part in its exchanges)
   const int64_t whole = (int64_t)p.heads * a.Tk * a.D;
-  store_column<E>(static_cast<E*>(p.dk) + at, p.part_dk ? p.part_dk + split * whole + at : nullptr, dk, DB, a.D, h, a.scale * Lift<E>::BACK * range.back());
-  store_column<E>(static_cast<E*>(p.dv) + at, p.part_dv ? p.part_dv + split * whole + at : nullptr, dv, DB, a.D, h, Lift<E>::BACK);
+  store_row<E>(static_cast<E*>(p.dk) + at, p.part_dk ? p.part_dk + split * whole + at : nullptr, dk, D, h, a.scale * Lift<E>::BACK * range.back());
+  store_row<E>(static_cast<E*>(p.dv) + at, p.part_dv ? p.part_dv + split * whole + at : nullptr, dv, D, h, Lift<E>::BACK);
 }
 
 // dq: a wave owns 32 rows (q and dout in registers) and walks keys in tiles of 64
@@ -327,10 +314,9 @@ __device__ __forceinline__ void rows_side(const BwdParams& p, uint32_t block, ch
       }
     }
   }
-  if (!real) return;
   const int64_t at = (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D;
   const int64_t whole = (int64_t)p.heads * a.R * a.D;
-  store_column<E>(static_cast<E*>(p.dq) + at, p.part_dq ? p.part_dq + split * whole + at : nullptr, dq, DB, a.D, h, a.scale * Lift<E>::BACK * range.back());
+  store_row<E>(static_cast<E*>(p.dq) + at, p.part_dq ? p.part_dq + split * whole + at : nullptr, dq, real ? a.D : 0, h, a.scale * Lift<E>::BACK * range.back());
 }
 
 // Both sides in one launch: neither needs the other, and one's last workgroups fill up with the other's. Rows come first, their
