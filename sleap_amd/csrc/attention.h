@@ -86,32 +86,6 @@ __device__ __forceinline__ float sum_halves(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Column n of a transposed result (C registers: rows d) as a row of D values, n 32-row blocks of `acc` times `by`: 16-bit to dst, or float32
-// to `part`. A lane has four values of each eight and its half-wave's partner the other four: one exchange of two dwords gives each
-// lane eight neighbours, so that it stores 16 bytes.
-template <typename E, int N>
-__device__ __forceinline__ void store_row(E* dst, float* part, const f32x16 (&acc)[N], int D, int h, float by) {
-#pragma unroll
-  for (int db = 0; db < N; ++db)
-#pragma unroll
-    for (int j = 0; j < 4; j += 2) {
-      const f32x16& x = acc[db];
-      if (part) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 4 * (j + e), d = db * 32 + (j + e) * 8 + h * 4;
-          if (d < D) *reinterpret_cast<f32x4*>(part + d) = f32x4{x[i] * by, x[i + 1] * by, x[i + 2] * by, x[i + 3] * by};
-        }
-        continue;
-      }
-      const int i = 4 * j;
-      const auto lo = __builtin_amdgcn_permlane32_swap(pack2<E>(x[i] * by, x[i + 1] * by), pack2<E>(x[i + 4] * by, x[i + 5] * by), false, false);
-      const auto hi = __builtin_amdgcn_permlane32_swap(pack2<E>(x[i + 2] * by, x[i + 3] * by), pack2<E>(x[i + 6] * by, x[i + 7] * by), false, false);
-      const int d = db * 32 + (j + h) * 8;
-      if (d < D) *reinterpret_cast<u32x4*>(dst + d) = u32x4{lo[0], hi[0], lo[1], hi[1]};
-    }
-}
-
 template <int DP>
 __device__ __host__ constexpr int swizzle(int row) {
   constexpr int PER_LINE = 128 / DP, PAIRS = DP / 16;  // rows of 256 bytes, 32-byte pairs of a row
@@ -130,6 +104,45 @@ struct Tile {
     return row * ROW + ((c ^ swizzle<DP>(row)) << 4) + (lane & 1) * 8;
   }
 };
+
+// A wave's transposed result (C registers: 32 columns, N blocks of 32 rows d) times `by` as 32 rows of D values.
+// float32, to rows of a workspace: 16 bytes a lane and store.
+template <int N>
+__device__ __forceinline__ void store_part(float* row, const f32x16 (&acc)[N], int D, int h, float by) {
+#pragma unroll
+  for (int db = 0; db < N; ++db)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = db * 32 + j * 8 + h * 4;
+      if (d < D) *reinterpret_cast<f32x4*>(row + d) = f32x4{acc[db][4 * j] * by, acc[db][4 * j + 1] * by, acc[db][4 * j + 2] * by, acc[db][4 * j + 3] * by};
+    }
+}
+// 16-bit, by way of LDS (32 * ROW bytes of the wave's own): a lane has four values of each eight and its partner in the other half-wave the
+// other four, one exchange of two dwords makes 16 bytes of them, and rows are read back whole, so that stores fill lines.
+// `row_of(i)`: where row i begins, or NULL. (8-byte stores straight from the registers: 84 us for the gradients of 8 x 8 x 192 x 4096 x
+// 64, 16-byte ones 70.)
+template <typename E, int DP, int N, typename F>
+__device__ __forceinline__ void store_rows(char* lds, const f32x16 (&acc)[N], int lane, int D, float by, F row_of) {
+  using T = Tile<DP>;
+  const int n = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int db = 0; db < N; ++db)
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const f32x16& x = acc[db];
+      const int i = 4 * j;
+      const auto lo = __builtin_amdgcn_permlane32_swap(pack2<E>(x[i] * by, x[i + 1] * by), pack2<E>(x[i + 4] * by, x[i + 5] * by), false, false);
+      const auto hi = __builtin_amdgcn_permlane32_swap(pack2<E>(x[i + 2] * by, x[i + 3] * by), pack2<E>(x[i + 6] * by, x[i + 7] * by), false, false);
+      *reinterpret_cast<u32x4*>(lds + n * T::ROW + (((db * 4 + j + h) ^ swizzle<DP>(n)) << 4)) = u32x4{lo[0], hi[0], lo[1], hi[1]};
+    }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // of this wave alone
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    const int at = k * 64 + lane, row = at / (DP / 8), c = at & (DP / 8 - 1);
+    E* dst = row_of(row);
+    if (dst && c * 8 < D) *reinterpret_cast<u32x4*>(dst + c * 8) = *reinterpret_cast<const u32x4*>(lds + row * T::ROW + ((c ^ swizzle<DP>(row)) << 4));
+  }
+}
 
 __device__ __forceinline__ s16x8 read_a(const char* lds, int off) { return *reinterpret_cast<const s16x8*>(lds + off); }
 __device__ __forceinline__ s16x8 read_t(const char* lds, int off, int step) {

@@ -146,16 +146,19 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
 
   l = sum_halves(l);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  E* dst = static_cast<E*>(p.out) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D;
-  float* part = nullptr;
   if (p.splits > 1) {
+    if (!real) return;
     const int64_t at = ((int64_t)bh * p.splits + split) * a.R + row;
-    if (real && h == 0) p.part_lse[at] = l == 0.0f ? -INFINITY : shift + __log2f(l);
-    part = p.part + at * a.D;
-  } else if (p.lse && real && h == 0) {
-    p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = l == 0.0f ? -INFINITY : (shift + __log2f(l)) * LN2;
+    if (h == 0) p.part_lse[at] = l == 0.0f ? -INFINITY : shift + __log2f(l);
+    store_part(p.part + at * a.D, o, a.D, h, inv);
+    return;
   }
-  store_row<E>(dst, part, o, real ? a.D : 0, h, inv);
+  if (p.lse && real && h == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = l == 0.0f ? -INFINITY : (shift + __log2f(l)) * LN2;
+  tile_barrier();  // the last tile has been read
+  store_rows<E, DP>(lds + wave * 32 * T::ROW, o, lane, a.D, inv, [&](int i) -> E* {
+    const uint32_t r = row - n + i, t = div_by(r, a.div_g), g = r - t * a.G;
+    return r < a.R ? static_cast<E*>(p.out) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D : nullptr;
+  });
 }
 
 // Joins the runs of keys: out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max). A row has 16 lanes of 8 values and `groups` of

@@ -214,11 +214,22 @@ __device__ __forceinline__ void keys_side(const BwdParams& p, uint32_t block, ch
 #pragma unroll
     for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
   }
-  const int64_t at = (((int64_t)b * a.Tk + key) * a.Hkv + hk) * a.D;
-  const int D = key < a.Tk ? a.D : 0;  // (both lanes of a key take part in its exchanges)
-  const int64_t whole = (int64_t)p.heads * a.Tk * a.D;
-  store_row<E>(static_cast<E*>(p.dk) + at, p.part_dk ? p.part_dk + split * whole + at : nullptr, dk, D, h, a.scale * Lift<E>::BACK * range.back());
-  store_row<E>(static_cast<E*>(p.dv) + at, p.part_dv ? p.part_dv + split * whole + at : nullptr, dv, D, h, Lift<E>::BACK);
+  const float by_k = a.scale * Lift<E>::BACK * range.back(), by_v = Lift<E>::BACK;
+  auto place = [&](int64_t k) { return (((int64_t)b * a.Tk + k) * a.Hkv + hk) * a.D; };
+  if (p.part_dk) {
+    if (key >= a.Tk) return;
+    const int64_t at = split * ((int64_t)p.heads * a.Tk * a.D) + place(key);
+    store_part(p.part_dk + at, dk, a.D, h, by_k);
+    store_part(p.part_dv + at, dv, a.D, h, by_v);
+    return;
+  }
+  tile_barrier();  // the last tile has been read
+  auto row_of = [&](void* base) {
+    return [=](int i) -> E* { return key - n + i < a.Tk ? static_cast<E*>(base) + place(key - n + i) : nullptr; };
+  };
+  char* own = lds + wave * 32 * T::ROW;
+  store_rows<E, DP>(own, dk, lane, a.D, by_k, row_of(p.dk));
+  store_rows<E, DP>(own, dv, lane, a.D, by_v, row_of(p.dv));
 }
 
 // dq: a wave owns 32 rows (q and dout in registers) and walks keys in tiles of 64
@@ -314,9 +325,16 @@ __device__ __forceinline__ void rows_side(const BwdParams& p, uint32_t block, ch
       }
     }
   }
-  const int64_t at = (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D;
-  const int64_t whole = (int64_t)p.heads * a.R * a.D;
-  store_row<E>(static_cast<E*>(p.dq) + at, p.part_dq ? p.part_dq + split * whole + at : nullptr, dq, real ? a.D : 0, h, a.scale * Lift<E>::BACK * range.back());
+  const float by = a.scale * Lift<E>::BACK * range.back();
+  if (p.part_dq) {
+    if (real) store_part(p.part_dq + split * ((int64_t)p.heads * a.R * a.D) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D, dq, a.D, h, by);
+    return;
+  }
+  tile_barrier();  // the last tile has been read
+  store_rows<E, DP>(lds + wave * 32 * T::ROW, dq, lane, a.D, by, [&](int i) -> E* {
+    const uint32_t r = row - n + i, t = div_by(r, a.div_g), g = r - t * a.G;
+    return r < a.R ? static_cast<E*>(p.dq) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D : nullptr;
+  });
 }
 
 // Both sides in one launch: neither needs the other, and one's last workgroups fill up with the other's. Rows come first, their
