@@ -63,43 +63,37 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
   const T* xb = static_cast<const T*>(p.x) + (int64_t)b * p.xb;
   T* yb = static_cast<T*>(p.y) + (int64_t)b * p.T * p.H * p.D;
   const uint32_t items = (uint32_t)nt * p.H * p.G;
-  for (uint32_t i = threadIdx.x; i < items; i += 256) {
+  for (uint32_t i = threadIdx.x; i < items; i += 256) {  // (two or four pieces a lane and turn: the same time)
     const uint32_t row = div_by(i, p.div_g), g = i - row * p.G;
     const uint32_t t = div_by(row, p.div_h), h = row - t * p.H;
-    const T* src = xb + (int64_t)(t0 + t) * p.xt + (int64_t)h * p.xh;
-    T* dst = yb + ((int64_t)(t0 + t) * p.H + h) * p.D;
-    if (g >= (uint32_t)p.rot) {  // values behind the pairs pass
-      const int e = (INTERLEAVED ? 0 : p.P) + (int)g * V;
-      *reinterpret_cast<Pc*>(dst + e) = *reinterpret_cast<const Pc*>(src + e);
-      continue;
-    }
-    const float2* w = cs + t * p.P;
-    if constexpr (INTERLEAVED) {
-      const int e = (int)g * V;
-      const Pc a = *reinterpret_cast<const Pc*>(src + e);
-      Pc o;
+    const bool turned = g < (uint32_t)p.rot;  // values behind the pairs pass
+    const int e = (INTERLEAVED || turned ? 0 : p.P) + (int)g * V;
+    const T* src = xb + (int64_t)(t0 + t) * p.xt + (int64_t)h * p.xh + e;
+    T* dst = yb + ((int64_t)(t0 + t) * p.H + h) * p.D + e;
+    Pc a = *reinterpret_cast<const Pc*>(src);
+    if (turned) {
+      const float2* w = cs + t * p.P + (INTERLEAVED ? g * (V / 2) : g * V);
+      if constexpr (INTERLEAVED) {
 #pragma unroll
-      for (int k = 0; k < V; k += 2) {
-        const float2 q = w[(e + k) >> 1];
-        const float u = to_f32(a.e[k]), v = to_f32(a.e[k + 1]);
-        o.e[k] = from_f32<T>(u * q.x - v * q.y);
-        o.e[k + 1] = from_f32<T>(v * q.x + u * q.y);
-      }
-      *reinterpret_cast<Pc*>(dst + e) = o;
-    } else {
-      const int e = (int)g * V;
-      const Pc a = *reinterpret_cast<const Pc*>(src + e), c = *reinterpret_cast<const Pc*>(src + p.P + e);
-      Pc o0, o1;
+        for (int k = 0; k < V; k += 2) {
+          const float2 q = w[k >> 1];
+          const float x = to_f32(a.e[k]), y = to_f32(a.e[k + 1]);
+          a.e[k] = from_f32<T>(x * q.x - y * q.y);
+          a.e[k + 1] = from_f32<T>(y * q.x + x * q.y);
+        }
+      } else {
+        Pc c = *reinterpret_cast<const Pc*>(src + p.P);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float2 q = w[e + k];
-        const float u = to_f32(a.e[k]), v = to_f32(c.e[k]);
-        o0.e[k] = from_f32<T>(u * q.x - v * q.y);
-        o1.e[k] = from_f32<T>(v * q.x + u * q.y);
+        for (int k = 0; k < V; ++k) {
+          const float2 q = w[k];
+          const float x = to_f32(a.e[k]), y = to_f32(c.e[k]);
+          a.e[k] = from_f32<T>(x * q.x - y * q.y);
+          c.e[k] = from_f32<T>(y * q.x + x * q.y);
+        }
+        *reinterpret_cast<Pc*>(dst + p.P) = c;
       }
-      *reinterpret_cast<Pc*>(dst + e) = o0;
-      *reinterpret_cast<Pc*>(dst + p.P + e) = o1;
     }
+    *reinterpret_cast<Pc*>(dst) = a;
   }
 }
 
