@@ -742,20 +742,22 @@ int sa_rotary_axes(const void* x, int dtype, int B, int T, int H, int D, const i
  *                into a result, NaN and infinities included
  *   out          [B,Tq,Hq,D] contiguous; zeros where no key is visible
  *   lse          [B,Hq,Tq] natural logarithm of the softmax's denominator (-inf where no key is visible), or NULL
+ *   out_low      like out: out + out_low is the result with about twice the bits of its type (for the gradients of few keys; half as many
+ *                products again), or NULL
  *   workspace    sa_cross_attention_workspace bytes (0: none): runs of keys that several workgroups work on */
 size_t sa_cross_attention_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D);
 int sa_cross_attention(const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D,
                        const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, const int64_t* mask_strides,
-                       float scale, void* out, float* lse, void* workspace, size_t workspace_bytes, sa_stream_t stream);
+                       float scale, void* out, float* lse, void* out_low, void* workspace, size_t workspace_bytes, sa_stream_t stream);
 
-/* Gradients of sa_cross_attention from its out and lse and from dout [B,Tq,Hq,D] (dout_strides: HOST, batch, token, head) ->
+/* Gradients of sa_cross_attention from its out, out_low (or NULL) and lse and from dout [B,Tq,Hq,D] (dout_strides: HOST, batch, token, head) ->
  * dq [B,Tq,Hq,D], dk and dv [B,Tk,Hkv,D], contiguous; shared heads are summed; hidden keys and rows that see none get zeros. No
  * atomics: the same call gives the same bits. workspace: sa_cross_attention_backward_workspace bytes. */
 size_t sa_cross_attention_backward_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D);
 int sa_cross_attention_backward(const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D,
                                 const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, const int64_t* mask_strides,
-                                float scale, const void* out, const float* lse, const void* dout, const int64_t* dout_strides, void* dq,
-                                void* dk, void* dv, void* workspace, size_t workspace_bytes, sa_stream_t stream);
+                                float scale, const void* out, const void* out_low, const float* lse, const void* dout,
+                                const int64_t* dout_strides, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, sa_stream_t stream);
 
 /* One AdamW step over n tensors of one type, in place (decoupled decay; 32-bit states and arithmetic; a 16-bit parameter is rounded once):
  *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  [vmax = max(vmax, v)];  p = p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v | vmax)/sqrt(1-b2^t) + eps)

@@ -128,9 +128,9 @@ SIGNATURES = {
     "sa_yuv420_to_bgr": (_i, [_p, _p, _p, _i, _i, _i, _i, _p, _i]),
     "sa_rotary_axes": (_i, [_p, _i, _i, _i, _i, _i, _p, _p, _i, _p, _i, _p, C.c_double, _i, _i, _i, _p, _p]),
     "sa_cross_attention_workspace": (_sz, [_i, _i, _i, _i, _i, _i]),
-    "sa_cross_attention": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _f, _p, _p, _p, _sz, _p]),
+    "sa_cross_attention": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _f, _p, _p, _p, _p, _sz, _p]),
     "sa_cross_attention_backward_workspace": (_sz, [_i, _i, _i, _i, _i, _i]),
-    "sa_cross_attention_backward": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _f, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "sa_cross_attention_backward": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
     "sa_adamw_step": (_i, [_p, _i, _i, _i, C.c_double, _p, C.c_double, C.c_double, C.c_double, C.c_double, C.c_int64, _p, _p]),
 }
 

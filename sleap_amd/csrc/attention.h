@@ -69,12 +69,22 @@ __device__ __forceinline__ s16x8 pack8(const f32x16& c, int s) {
   return __builtin_bit_cast(s16x8, v);
 }
 
-// the other half-wave's value of the same column
-__device__ __forceinline__ float other_half(float v) {
-  const uint32_t u = __float_as_uint(v);
-  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // lanes < 32: {own, upper}; lanes >= 32: {lower, own}
-  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+// what rounding to 16 bits takes from a value
+template <typename E>
+__device__ __forceinline__ float rest_of(float v) {
+  return v - static_cast<float>(static_cast<E>(v));
 }
+// and from registers 8s .. 8s + 7 of a C, given what they were rounded to
+template <typename E>
+__device__ __forceinline__ s16x8 pack8_rest(const f32x16& c, int s, s16x8 rounded) {
+  const typename Mfma<E>::v8 r = __builtin_bit_cast(typename Mfma<E>::v8, rounded);
+  f32x16 x;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = c[8 * s + e] - static_cast<float>(r[e]);
+  return pack8<E>(x, 0);
+}
+
+// the two half-waves' values of the same column
 __device__ __forceinline__ float max_halves(float v) {
   const uint32_t u = __float_as_uint(v);
   const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);

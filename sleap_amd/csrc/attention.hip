@@ -11,6 +11,7 @@ struct FwdParams {
   AttnShape a;
   void* out;              // [B, Tq, Hq, D] contiguous
   float* lse;             // [B, Hq, Tq] natural logarithm of the softmax's denominator, or NULL
+  void* low;              // like out, what its rounding left, rounded: out + low has twice the bits; or NULL
   float* part;            // splits > 1: [B * Hkv][splits][R][D] of each run of keys, normalised
   float* part_lse;        // and their base-2 logarithms [B * Hkv][splits][R]
   uint32_t blocks, heads, row_tiles, splits;  // heads: B * Hkv; blocks: heads * row_tiles * splits
@@ -30,7 +31,10 @@ struct Range<_Float16> {
 };
 constexpr float GROW = 8.0f;
 
-template <typename E, int DB, int NW>
+// LOW: weights are multiplied in two terms, rounded and what that left, and `low` is written. For gradients over few keys: rowsum(do * out)
+// has to cancel against w^T (do v^T) there, and the roundings of w and out alone made dq and dk over 3 keys 2.2 times as inexact as
+// their own rounding (600 keys: 1.5 times; from 4096 on it no longer shows).
+template <typename E, int DB, int NW, bool LOW>
 __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p) {
   constexpr int DP = DB == 3 ? 128 : DB * 32, KS = DB * 2;
   using T = Tile<DP>;
@@ -138,9 +142,16 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
     l += l0 + l1;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      const s16x8 w = pack8<E>(kk < 2 ? s0 : s1, kk & 1);
+      const f32x16& s = kk < 2 ? s0 : s1;
+      const s16x8 w = pack8<E>(s, kk & 1);
+      s16x8 rest;
+      if constexpr (LOW) rest = pack8_rest<E>(s, kk & 1, w);
 #pragma unroll
-      for (int db = 0; db < DB; ++db) o[db] = Mfma<E>::run(read_t(vt, ot[db] + kk * 16 * T::ROW, 8 * T::ROW), w, o[db]);
+      for (int db = 0; db < DB; ++db) {
+        const s16x8 v = read_t(vt, ot[db] + kk * 16 * T::ROW, 8 * T::ROW);
+        o[db] = Mfma<E>::run(v, w, o[db]);
+        if constexpr (LOW) o[db] = Mfma<E>::run(v, rest, o[db]);
+      }
     }
   }
 
@@ -155,10 +166,20 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
   }
   if (p.lse && real && h == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = l == 0.0f ? -INFINITY : (shift + __log2f(l)) * LN2;
   tile_barrier();  // the last tile has been read
-  store_rows<E, DP>(lds + wave * 32 * T::ROW, o, lane, a.D, inv, [&](int i) -> E* {
-    const uint32_t r = row - n + i, t = div_by(r, a.div_g), g = r - t * a.G;
-    return r < a.R ? static_cast<E*>(p.out) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D : nullptr;
-  });
+  auto row_of = [&](void* base) {
+    return [=](int i) -> E* {
+      const uint32_t r = row - n + i, t = div_by(r, a.div_g), g = r - t * a.G;
+      return r < a.R ? static_cast<E*>(base) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D : nullptr;
+    };
+  };
+  store_rows<E, DP>(lds + wave * 32 * T::ROW, o, lane, a.D, inv, row_of(p.out));
+  if constexpr (LOW) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] = rest_of<E>(o[db][e] * inv);
+    store_rows<E, DP>(lds + wave * 32 * T::ROW, o, lane, a.D, 1.0f, row_of(p.low));
+  }
 }
 
 // Joins the runs of keys: out = sum_s 2^(lse_s - max) part_s / sum_s 2^(lse_s - max). A row has 16 lanes of 8 values and `groups` of
@@ -222,9 +243,14 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const FwdParams p, 
   const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv, t = div_by(row, a.div_g), g = row - t * a.G;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   if (p.lse && d == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = sum == 0.0f ? -INFINITY : (m + __log2f(sum)) * LN2;
-  E* dst = static_cast<E*>(p.out) + (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D + d;
-  *reinterpret_cast<u32x4*>(dst) = u32x4{pack2<E>(acc[0] * inv, acc[1] * inv), pack2<E>(acc[2] * inv, acc[3] * inv),
-                                         pack2<E>(acc[4] * inv, acc[5] * inv), pack2<E>(acc[6] * inv, acc[7] * inv)};
+  const int64_t at = (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D + d;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] *= inv;
+  *reinterpret_cast<u32x4*>(static_cast<E*>(p.out) + at) = u32x4{pack2<E>(acc[0], acc[1]), pack2<E>(acc[2], acc[3]), pack2<E>(acc[4], acc[5]), pack2<E>(acc[6], acc[7])};
+  if (!p.low) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = rest_of<E>(acc[e]);
+  *reinterpret_cast<u32x4*>(static_cast<E*>(p.low) + at) = u32x4{pack2<E>(acc[0], acc[1]), pack2<E>(acc[2], acc[3]), pack2<E>(acc[4], acc[5]), pack2<E>(acc[6], acc[7])};
 }
 
 // How a call is cut: waves of a workgroup (32 rows each) and runs of keys.
@@ -251,13 +277,18 @@ Cut cut(int B, int Tq, int Tk, int Hq, int Hkv) {
   return c;
 }
 
+template <typename E, int DB, bool LOW>
+void launch_low(const FwdParams& p, int waves, hipStream_t s) {
+  constexpr size_t lds = 4 * Tile<DB == 3 ? 128 : DB * 32>::BYTES;
+  if (waves == 1) attention_kernel<E, DB, 1, LOW><<<dim3(p.blocks), dim3(64), lds, s>>>(p);
+  else if (waves == 2) attention_kernel<E, DB, 2, LOW><<<dim3(p.blocks), dim3(128), lds, s>>>(p);
+  else attention_kernel<E, DB, 4, LOW><<<dim3(p.blocks), dim3(256), lds, s>>>(p);
+}
+
 template <typename E, int DB>
 void launch(const FwdParams& p, int waves, hipStream_t s) {
-  constexpr int DP = DB == 3 ? 128 : DB * 32;
-  constexpr size_t lds = 4 * Tile<DP>::BYTES;
-  if (waves == 1) attention_kernel<E, DB, 1><<<dim3(p.blocks), dim3(64), lds, s>>>(p);
-  else if (waves == 2) attention_kernel<E, DB, 2><<<dim3(p.blocks), dim3(128), lds, s>>>(p);
-  else attention_kernel<E, DB, 4><<<dim3(p.blocks), dim3(256), lds, s>>>(p);
+  if (p.low) launch_low<E, DB, true>(p, waves, s);
+  else launch_low<E, DB, false>(p, waves, s);
 }
 
 template <typename E>
@@ -323,11 +354,11 @@ extern "C" size_t sa_cross_attention_workspace(int B, int Tq, int Tk, int Hq, in
 
 extern "C" int sa_cross_attention(const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D,
                                   const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, const int64_t* mask_strides,
-                                  float scale, void* out, float* lse, void* workspace, size_t workspace_bytes, sa_stream_t stream) {
+                                  float scale, void* out, float* lse, void* out_low, void* workspace, size_t workspace_bytes, sa_stream_t stream) {
   FwdParams p;
   if (int rc = attention_shape("sa_cross_attention", &p.a, q, k, v, dtype, B, Tq, Tk, Hq, Hkv, D, strides, key_lengths, key_mask, mask_strides, scale)) return rc;
   if (B == 0 || Tq == 0) return SA_OK;
-  SA_REQUIRE(((uintptr_t)out & 15) == 0, "sa_cross_attention: addresses are multiples of 16");
+  SA_REQUIRE((((uintptr_t)out | (uintptr_t)out_low | (uintptr_t)workspace) & 15) == 0, "sa_cross_attention: addresses are multiples of 16");
   const Cut c = cut(B, Tq, Tk, Hq, Hkv);
   const uint64_t blocks = (uint64_t)c.row_tiles * c.splits * B * Hkv;
   SA_REQUIRE(blocks < (1ull << 31) && (uint64_t)B * Hq * Tq < (1ull << 31) - 1024, "sa_cross_attention: too many rows");
@@ -335,6 +366,7 @@ extern "C" int sa_cross_attention(const void* q, const void* k, const void* v, i
     return fail(SA_ERR_WORKSPACE, "sa_cross_attention: workspace of %zu bytes is too small", workspace_bytes);
   p.out = out;
   p.lse = lse;
+  p.low = out_low;
   p.part = static_cast<float*>(workspace);
   p.part_lse = p.part + (size_t)B * Hq * Tq * c.splits * D;
   p.blocks = (uint32_t)blocks;

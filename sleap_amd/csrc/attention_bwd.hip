@@ -20,7 +20,7 @@ struct Side {
 
 struct BwdParams {
   AttnShape a;
-  const void *out, *dout;
+  const void *out, *low, *dout;  // low: what the rounding of out left, or NULL
   int64_t ob, ot, oh;       // strides of dout
   const float* lse;         // [B, Hq, Tq]
   float *lse2, *delta;      // [B * Hkv][R]: log2 of the denominator less LIFT; rowsum(do * out)
@@ -86,6 +86,11 @@ __global__ __launch_bounds__(256) void attention_stats_kernel(const BwdParams p,
     y.v = *reinterpret_cast<const s16x8*>(static_cast<const E*>(p.dout) + (int64_t)b * p.ob + (int64_t)t * p.ot + (int64_t)hh * p.oh + d);
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum += to_f32(x.e[e]) * to_f32(y.e[e]);
+    if (p.low) {
+      x.v = *reinterpret_cast<const s16x8*>(static_cast<const E*>(p.low) + (int64_t)ic * a.D + d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += to_f32(x.e[e]) * to_f32(y.e[e]);
+    }
   }
 #pragma unroll
   for (int w = 8; w; w >>= 1) sum += __shfl_xor(sum, w);
@@ -460,14 +465,14 @@ extern "C" size_t sa_cross_attention_backward_workspace(int B, int Tq, int Tk, i
 
 extern "C" int sa_cross_attention_backward(const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq, int Hkv,
                                            int D, const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask,
-                                           const int64_t* mask_strides, float scale, const void* out, const float* lse, const void* dout,
+                                           const int64_t* mask_strides, float scale, const void* out, const void* out_low, const float* lse, const void* dout,
                                            const int64_t* dout_strides, void* dq, void* dk, void* dv, void* workspace,
                                            size_t workspace_bytes, sa_stream_t stream) {
   const char* who = "sa_cross_attention_backward";
   BwdParams p;
   if (int rc = attention_shape(who, &p.a, q, k, v, dtype, B, Tq, Tk, Hq, Hkv, D, strides, key_lengths, key_mask, mask_strides, scale)) return rc;
   if (B == 0) return SA_OK;
-  SA_REQUIRE((((uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) & 15) == 0, "%s: addresses are multiples of 16", who);
+  SA_REQUIRE((((uintptr_t)out | (uintptr_t)out_low | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) & 15) == 0, "%s: addresses are multiples of 16", who);
   for (int i = 0; i < 3; ++i) SA_REQUIRE(dout_strides[i] >= 0 && dout_strides[i] % 8 == 0, "%s: strides are multiples of 8 elements", who);
   const int64_t G = Hq / Hkv, far = 1ll << 30;
   SA_REQUIRE(TILE * strides[1] + G * strides[2] < far && TILE * dout_strides[1] + G * dout_strides[2] < far,
@@ -476,6 +481,7 @@ extern "C" int sa_cross_attention_backward(const void* q, const void* k, const v
   SA_REQUIRE((uint64_t)l.kv.blocks + l.rows.blocks < (1ull << 31) && (uint64_t)B * Hq * Tq < (1ull << 31) - 1024 && (uint64_t)B * Hkv < (1ull << 31), "%s: too many rows", who);
   if (workspace_bytes < l.total() * sizeof(float)) return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", who, workspace_bytes);
   p.out = out;
+  p.low = out_low;
   p.dout = dout;
   p.ob = dout_strides[0];
   p.ot = dout_strides[1];

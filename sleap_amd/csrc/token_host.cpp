@@ -190,26 +190,34 @@ Tensor workspace(size_t bytes, const Tensor& like) {  // of one call: the alloca
   return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
-std::pair<Tensor, Tensor> attend(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Keys& keys, bool want_lse) {
+// Up to this many keys a forward pass that is to be differentiated keeps its output in two terms (attention.hip: LOW).
+constexpr int64_t FEW_KEYS = 2048;
+
+struct Attended {
+  Tensor out, lse, low;
+};
+Attended attend(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Keys& keys, bool want_lse, bool want_low) {
   const Laid q = laid_out(q_, 8), k = laid_out(k_, 8, KEY_SPAN), v = laid_out(v_, 8, KEY_SPAN);
   const int B = (int)q.t.size(0), Tq = (int)q.t.size(1), H = (int)q.t.size(2), D = (int)q.t.size(3), Tk = (int)k.t.size(1), K = (int)k.t.size(2);
-  Tensor out = at::empty({B, Tq, H, D}, q.t.options()), lse;
+  Tensor out = at::empty({B, Tq, H, D}, q.t.options()), lse, low;
+  if (want_low) low = at::empty_like(out);
   if (want_lse) lse = at::empty({B, H, Tq}, q.t.options().dtype(at::kFloat));
-  if (B == 0 || Tq == 0) return {out, lse};
+  if (B == 0 || Tq == 0) return {out, lse, low};
   const size_t bytes = entry.attention_workspace(B, Tq, Tk, H, K, D);
   const Tensor ws = workspace(bytes, q.t);
   const int64_t strides[9] = {q.s[0], q.s[1], q.s[2], k.s[0], k.s[1], k.s[2], v.s[0], v.s[1], v.s[2]};
   const auto ms = keys.strides();
   const c10::OptionalDeviceGuard guard(q.t.device());
   check(entry.attention(q.t.data_ptr(), k.t.data_ptr(), v.t.data_ptr(), type_of(q.t), B, Tq, Tk, H, K, D, strides, keys.n(), keys.m(), ms.data(),
-                      keys.scale, out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
+                      keys.scale, out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr,
+                      want_low ? low.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
                       stream_of(q.t.device())),
         "sa_cross_attention");
-  return {out, lse};
+  return {out, lse, low};
 }
 
 std::array<Tensor, 3> attend_backward(const Tensor& dout_, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& out, const Tensor& lse,
-                                      const Keys& keys) {
+                                      const Tensor& low, const Keys& keys) {
   const int64_t group = q_.size(2) / k_.size(2);
   const Laid q = laid_out(q_, 8, ROW_SPAN, group), k = laid_out(k_, 8, KEY_SPAN), v = laid_out(v_, 8, KEY_SPAN), dout = laid_out(dout_, 8, ROW_SPAN, group);
   const int B = (int)q.t.size(0), Tq = (int)q.t.size(1), H = (int)q.t.size(2), D = (int)q.t.size(3), Tk = (int)k.t.size(1), K = (int)k.t.size(2);
@@ -221,7 +229,7 @@ std::array<Tensor, 3> attend_backward(const Tensor& dout_, const Tensor& q_, con
   const auto ms = keys.strides();
   const c10::OptionalDeviceGuard guard(q.t.device());
   check(entry.attention_backward(q.t.data_ptr(), k.t.data_ptr(), v.t.data_ptr(), type_of(q.t), B, Tq, Tk, H, K, D, strides, keys.n(), keys.m(),
-                               ms.data(), keys.scale, out.data_ptr(), lse.data_ptr<float>(), dout.t.data_ptr(), dout.s.data(), dq.data_ptr(),
+                               ms.data(), keys.scale, out.data_ptr(), low.defined() ? low.data_ptr() : nullptr, lse.data_ptr<float>(), dout.t.data_ptr(), dout.s.data(), dq.data_ptr(),
                                dk.data_ptr(), dv.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q.t.device())),
         "sa_cross_attention_backward");
   return {dq, dk, dv};
@@ -229,8 +237,8 @@ std::array<Tensor, 3> attend_backward(const Tensor& dout_, const Tensor& q_, con
 
 struct CrossAttention : torch::autograd::Function<CrossAttention> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Keys& keys, bool want_lse) {
-    auto [out, lse] = attend(q, k, v, keys, true);
-    ctx->save_for_backward({q, k, v, out, lse, keys.lengths, keys.mask});
+    const auto [out, lse, low] = attend(q, k, v, keys, true, k.size(1) <= FEW_KEYS);
+    ctx->save_for_backward({q, k, v, out, lse, low, keys.lengths, keys.mask});
     ctx->saved_data["scale"] = (double)keys.scale;
     ctx->set_materialize_grads(false);
     if (!want_lse) return {out};
@@ -240,8 +248,8 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
-    const Keys keys = {saved[5], saved[6], (float)ctx->saved_data["scale"].toDouble()};
-    const auto [dq, dk, dv] = attend_backward(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], keys);
+    const Keys keys = {saved[6], saved[7], (float)ctx->saved_data["scale"].toDouble()};
+    const auto [dq, dk, dv] = attend_backward(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], keys);
     variable_list got = {dq, dk, dv};
     if (at::GradMode::is_enabled()) {  // create_graph: a second gradient has to fail, not to miss what these depend on
       for (auto& t : got) t = t.detach().set_requires_grad(true);
@@ -280,7 +288,7 @@ py::object cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
     const auto got = CrossAttention::apply(q, k, v, keys, return_lse);
     return return_lse ? py::object(py::make_tuple(got[0], got[1])) : py::cast(got[0]);
   }
-  const auto [out, lse] = attend(q, k, v, keys, return_lse);
+  const auto [out, lse, low] = attend(q, k, v, keys, return_lse, false);
   return return_lse ? py::object(py::make_tuple(out, lse)) : py::cast(out);
 }
 

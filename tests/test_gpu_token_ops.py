@@ -127,7 +127,7 @@ def check(q, k, v, dout, lengths=None, mask=None, scale=None):
     far = {"out": oracle.worst(out, want["out"]), "lse": oracle.worst(lse, want["lse"])}
     leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
     again = ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask, scale=scale)
-    assert torch.equal(again, out)
+    far["out, differentiated"] = oracle.worst(again.detach(), want["out"])  # (over few keys with two-term weights: other bits)
     grads = torch.autograd.grad(again, leaves, dout)
     for name, x in zip(("dq", "dk", "dv"), grads):
         assert x.dtype == q.dtype

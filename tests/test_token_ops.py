@@ -47,8 +47,8 @@ def test_attention_entry_points_refuse():
     def call(dtype=1, B=1, Tq=4, Tk=8, H=2, K=2, D=32, strides=(64, 64, 32) * 3, scale=1.0, q=256, k=256, out=256, ws=0, backward=False, so=(64, 64, 32)):
         args = (q, k, 256, dtype, B, Tq, Tk, H, K, D, i64(*strides), None, None, None, scale)
         if backward:
-            return h.sa_cross_attention_backward(*args, out, 256, 256, i64(*so), 256, 256, 256, 256, ws, None)
-        return h.sa_cross_attention(*args, out, None, 256, ws, None)
+            return h.sa_cross_attention_backward(*args, out, None, 256, 256, i64(*so), 256, 256, 256, 256, ws, None)
+        return h.sa_cross_attention(*args, out, None, None, 256, ws, None)
 
     for backward in (False, True):
         def no(text, **kw):
