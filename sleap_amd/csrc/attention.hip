@@ -320,6 +320,9 @@ int attention_shape(const char* who, AttnShape* a, const void* q, const void* k,
   SA_REQUIRE(Tk <= (1 << 30) && (uint64_t)Tq * (Hq / Hkv) < (1ull << 31) - 1024 && (uint64_t)B * Hq < (1ull << 31), "%s: too many rows", who);
   for (int i = 0; i < 9; ++i) SA_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, "%s: strides are multiples of 8 elements", who);
   for (int i = 3; i < 9; i += 3) SA_REQUIRE(strides[i + 1] < (1ll << 23), "%s: token strides of keys and values are below 2^23 elements", who);
+  SA_REQUIRE(!mask || mask_strides, "%s: a mask needs its strides", who);
+  const uint64_t rows = (uint64_t)B * Tq, keys = (uint64_t)B * Tk;
+  SA_REQUIRE((q || !rows) && ((k && v) || !keys), "%s: null address", who);
   SA_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0, "%s: addresses are multiples of 16", who);
   a->q = q;
   a->k = k;
@@ -358,11 +361,12 @@ extern "C" int sa_cross_attention(const void* q, const void* k, const void* v, i
   FwdParams p;
   if (int rc = attention_shape("sa_cross_attention", &p.a, q, k, v, dtype, B, Tq, Tk, Hq, Hkv, D, strides, key_lengths, key_mask, mask_strides, scale)) return rc;
   if (B == 0 || Tq == 0) return SA_OK;
+  SA_REQUIRE(out, "sa_cross_attention: null address");
   SA_REQUIRE((((uintptr_t)out | (uintptr_t)out_low | (uintptr_t)workspace) & 15) == 0, "sa_cross_attention: addresses are multiples of 16");
   const Cut c = cut(B, Tq, Tk, Hq, Hkv);
   const uint64_t blocks = (uint64_t)c.row_tiles * c.splits * B * Hkv;
   SA_REQUIRE(blocks < (1ull << 31) && (uint64_t)B * Hq * Tq < (1ull << 31) - 1024, "sa_cross_attention: too many rows");
-  if (c.splits > 1 && workspace_bytes < sa_cross_attention_workspace(B, Tq, Tk, Hq, Hkv, D))
+  if (c.splits > 1 && (!workspace || workspace_bytes < sa_cross_attention_workspace(B, Tq, Tk, Hq, Hkv, D)))
     return fail(SA_ERR_WORKSPACE, "sa_cross_attention: workspace of %zu bytes is too small", workspace_bytes);
   p.out = out;
   p.lse = lse;

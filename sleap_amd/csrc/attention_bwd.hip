@@ -471,7 +471,8 @@ extern "C" int sa_cross_attention_backward(const void* q, const void* k, const v
   const char* who = "sa_cross_attention_backward";
   BwdParams p;
   if (int rc = attention_shape(who, &p.a, q, k, v, dtype, B, Tq, Tk, Hq, Hkv, D, strides, key_lengths, key_mask, mask_strides, scale)) return rc;
-  if (B == 0) return SA_OK;
+  if (B == 0 || (Tq == 0 && Tk == 0)) return SA_OK;
+  SA_REQUIRE((Tq == 0 || (out && lse && dout && dq)) && (Tk == 0 || (dk && dv)), "%s: null address", who);
   SA_REQUIRE((((uintptr_t)out | (uintptr_t)out_low | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) & 15) == 0, "%s: addresses are multiples of 16", who);
   for (int i = 0; i < 3; ++i) SA_REQUIRE(dout_strides[i] >= 0 && dout_strides[i] % 8 == 0, "%s: strides are multiples of 8 elements", who);
   const int64_t G = Hq / Hkv, far = 1ll << 30;
@@ -479,7 +480,7 @@ extern "C" int sa_cross_attention_backward(const void* q, const void* k, const v
              "%s: 64 tokens and the heads on one key head span less than 2^30 elements of q and of dout", who);
   const Layout l = layout(B, Tq, Tk, Hq, Hkv, D);
   SA_REQUIRE((uint64_t)l.kv.blocks + l.rows.blocks < (1ull << 31) && (uint64_t)B * Hq * Tq < (1ull << 31) - 1024 && (uint64_t)B * Hkv < (1ull << 31), "%s: too many rows", who);
-  if (workspace_bytes < l.total() * sizeof(float)) return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", who, workspace_bytes);
+  if (l.total() && (!workspace || workspace_bytes < l.total() * sizeof(float))) return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", who, workspace_bytes);
   p.out = out;
   p.low = out_low;
   p.dout = dout;

@@ -131,6 +131,7 @@ extern "C" int sa_rotary_axes(const void* x, int dtype, int B, int T, int H, int
   }
   SA_REQUIRE(P >= 1 && P <= MAX_PAIRS && 2 * P <= D, "sa_rotary_axes: %d pairs in heads of %d (1 to %d, two values each)", P, D, MAX_PAIRS);
   if (B == 0 || T == 0) return SA_OK;
+  SA_REQUIRE(x && positions && y, "sa_rotary_axes: null address");
   RotaryParams p;
   p.x = x;
   p.y = y;

@@ -81,6 +81,21 @@ void on_one_gpu(const char* who, std::initializer_list<std::pair<const char*, co
   }
 }
 
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+
+// A graph that was built outside of a capture and still lives holds the leaf's gradient node, and with it the stream that it was built on:
+// a captured backward pass would pull that stream into the capture, where torch's engine ends the process. Refused before it starts.
+void not_held_elsewhere(const char* who, std::initializer_list<const Tensor*> tensors) {
+  if (!capturing()) return;
+  for (const Tensor* t : tensors) {
+    if (!t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto held = node ? node->stream() : std::nullopt;
+    if (held && held->id() != c10::hip::getCurrentHIPStream(t->get_device()).id())
+      throw std::runtime_error(text(who, ": captured while a graph from outside of the capture holds the same leaf: delete that graph first (or capture a detached leaf)"));
+  }
+}
+
 // A (B, T, heads, D) tensor as the kernels take it: `t` itself if its last dimension is contiguous, every other stride and the address are
 // whole multiples of `elements` values and 64 tokens and `group` heads span less than `limit` (if any); else a contiguous copy.
 // Strides are 0 where there is nothing to step over.
@@ -89,6 +104,7 @@ struct Laid {
   std::array<int64_t, 3> s;
 };
 Laid laid_out(Tensor t, int64_t elements, int64_t limit = 0, int64_t group = 0) {
+  t = t.resolve_neg();
   for (int turn = 0;; ++turn) {
     std::array<int64_t, 3> s;
     for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
@@ -168,7 +184,9 @@ Tensor rotary_axes(const Tensor& x, const Tensor& positions, const std::vector<i
   if (!(theta > 0 && theta < 1e30)) bad_value(who, ": theta ", theta);
   if (positions.requires_grad()) bad_value(who, ": there is no gradient for positions");
   const Turn how = {{sections.begin(), sections.end()}, theta, ladder == "shared", interleaved, inverse};
-  return x.requires_grad() && at::GradMode::is_enabled() ? Rotary::apply(x, positions, how) : turn(x, positions, how);
+  if (!x.requires_grad() || !at::GradMode::is_enabled()) return turn(x, positions, how);
+  not_held_elsewhere(who, {&x});
+  return Rotary::apply(x, positions, how);
 }
 
 // ---------------------------------------------------------------------------------------------- cross attention
@@ -285,6 +303,7 @@ py::object cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
   if (keys.mask.defined() && (keys.mask.scalar_type() != at::kBool || keys.mask.dim() != 2 || (keys.mask.size(0) != B && keys.mask.size(0) != 1) || keys.mask.size(1) != Tk))
     bad_value(who, ": key_mask must be (", B, ", ", Tk, ") bool, True where a key is visible: got ", keys.mask.sizes(), " ", keys.mask.scalar_type());
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+    not_held_elsewhere(who, {&q, &k, &v});
     const auto got = CrossAttention::apply(q, k, v, keys, return_lse);
     return return_lse ? py::object(py::make_tuple(got[0], got[1])) : py::cast(got[0]);
   }
@@ -327,8 +346,8 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
   if (n == 0) return;
 
   std::map<std::pair<int, int>, std::vector<sa_adamw_tensor>> groups;  // by type and device
-  std::vector<void*> held;
-  held.reserve(n);
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;  // where each thing that the step writes begins and ends
+  written.reserve(n * (lists - 1));
   for (Py_ssize_t i = 0; i < n; ++i) {
     const Tensor* x[5] = {};
     for (int j = 0; j < lists; ++j) {
@@ -346,15 +365,20 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
     if (x[0]->numel() == 0) continue;
     groups[{type, x[0]->get_device()}].push_back({x[0]->data_ptr(), x[1]->data_ptr(), x[2]->data_ptr<float>(), x[3]->data_ptr<float>(),
                                                   ams ? x[4]->data_ptr<float>() : nullptr, x[0]->numel()});
-    held.push_back(x[0]->data_ptr());
+    for (int j = 0; j < lists; ++j)
+      if (j != 1) {
+        const auto at = reinterpret_cast<uintptr_t>(x[j]->data_ptr());
+        written.push_back({at, at + x[j]->nbytes()});
+      }
   }
-  std::sort(held.begin(), held.end());
-  if (std::adjacent_find(held.begin(), held.end()) != held.end()) bad_value(who, ": the same parameter twice");
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i].first < written[i - 1].second) bad_value(who, ": the same parameter or state twice, or two that overlap");
   for (const auto& [key, tensors] : groups)
     for (const py::object* o : {&step, &lr})
       if (THPVariable_Check(o->ptr()) && THPVariable_Unpack(o->ptr()).get_device() != key.second)
         bad_value(who, ": step and learning rate tensors must be on the GPU of the parameters");
-  if (!groups.empty() && !dev_step && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+  if (!groups.empty() && !dev_step && capturing())
     throw std::runtime_error("adamw_step: a captured step needs its count as a tensor (every replay would repeat this one)");
   for (const auto& [key, tensors] : groups) {
     const c10::Device device(c10::kCUDA, (c10::DeviceIndex)key.second);
@@ -363,6 +387,11 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
                          eps, weight_decay, t, dev_step ? THPVariable_Unpack(step.ptr()).data_ptr<int64_t>() : nullptr, stream_of(device)),
           "sa_adamw_step");
   }
+  for (int j = 0; j < lists; ++j)  // a graph that saved one of them has to notice
+    for (Py_ssize_t i = 0; j != 1 && i < n; ++i) {
+      const Tensor& x = THPVariable_Unpack(items[j][i]);
+      if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+    }
 }
 
 template <typename F>

@@ -79,6 +79,37 @@ def test_rotary_gradient_is_the_inverse_turn():
     assert oracle.worst(again, oracle.rotary(d, p, (5, 6, 4))) <= 1
 
 
+def test_rotary_refusals():
+    from sleap_amd import ops
+
+    x, p = normal(rng(6), 2, 5, 2, 16, dtype=torch.float32), torch.zeros((5, 2), device=DEV)
+    for bad, kind, text in ((dict(x=x[0]), ValueError, "x must be"), (dict(x=x[..., :15]), ValueError, "even"), (dict(x=x.double()), TypeError, "float32"),
+                            (dict(positions=p.double()), TypeError, "positions"), (dict(positions=p[:4]), ValueError, "positions"),
+                            (dict(positions=p[:, :1]), ValueError, "positions"), (dict(positions=p.expand(3, 5, 2)), ValueError, "positions"),
+                            (dict(positions=p.clone().requires_grad_(True)), ValueError, "gradient"), (dict(sections=(4, 5)), ValueError, "sections"),
+                            (dict(sections=(0, 0)), ValueError, "sections"), (dict(sections=()), ValueError, "sections"), (dict(sections=(-1, 2)), ValueError, "sections"),
+                            (dict(sections=(1,) * 9), ValueError, "sections"), (dict(ladder="none"), ValueError, "ladder"), (dict(theta=0.0), ValueError, "theta"),
+                            (dict(theta=math.nan), ValueError, "theta"), (dict(positions=p.cpu()), ValueError, "CUDA")):
+        with pytest.raises(kind, match=text):
+            ops.rotary_axes(**{**dict(x=x, positions=p, sections=(4, 4)), **bad})
+
+
+def test_attention_refusals():
+    from sleap_amd import ops
+
+    q, k, v, _, _, _ = make(rng(7), 2, 5, 9, 4, 2, 16, torch.float16)
+    lengths, mask = torch.ones(2, dtype=torch.int32, device=DEV), torch.ones((2, 9), dtype=torch.bool, device=DEV)
+    for bad, kind, text in ((dict(q=q[0]), ValueError, "q \\(B"), (dict(k=k[:1]), ValueError, "q \\(B"), (dict(v=v[:, :8]), ValueError, "q \\(B"),
+                            (dict(q=q.float()), TypeError, "float16"), (dict(q=q.bfloat16()), TypeError, "float16"),
+                            (dict(q=q[..., :12], k=k[..., :12], v=v[..., :12]), ValueError, "head size"), (dict(q=q[:, :, :3]), ValueError, "share"),
+                            (dict(k=k[:, :, :0], v=v[:, :, :0]), ValueError, "share"), (dict(scale=0.0), ValueError, "scale"), (dict(scale=-1.0), ValueError, "scale"),
+                            (dict(scale=math.inf), ValueError, "scale"), (dict(key_lengths=lengths[:1]), ValueError, "key_lengths"),
+                            (dict(key_lengths=lengths.float()), ValueError, "key_lengths"), (dict(key_mask=mask[:, :8]), ValueError, "key_mask"),
+                            (dict(key_mask=mask.float()), ValueError, "key_mask"), (dict(key_mask=mask.cpu()), ValueError, "CUDA")):
+        with pytest.raises(kind, match=text):
+            ops.cross_attention(**{**dict(q=q, k=k, v=v), **bad})
+
+
 @pytest.mark.parametrize("B,T", [(0, 5), (3, 0)])
 def test_rotary_of_nothing(B, T):
     from sleap_amd import ops
@@ -311,11 +342,10 @@ def test_captured_calls_follow_their_inputs():
     """Forward and backward in a graph each, replayed on new inputs with eager work between; each graph has its own scratch."""
     from sleap_amd import ops
 
-    shape = (2, 24, 1300, 4, 2, 64)
     graphs = []
-    for seed in (18, 19):
+    for seed, shape in ((18, (2, 24, 1300, 4, 2, 64)), (19, (1, 150, 2600, 2, 2, 128))):
         q, k, v, dout, _, _ = make(rng(seed), *shape, torch.bfloat16)
-        p = torch.randint(0, 1000, (24, 2), generator=rng(seed), device=DEV)
+        p = torch.randint(0, 1000, (shape[1], 2), generator=rng(seed), device=DEV)
 
         def step(q=q, k=k, v=v, dout=dout, p=p):
             leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
@@ -341,6 +371,87 @@ def test_captured_calls_follow_their_inputs():
         for _, held, step, _ in graphs:
             for a, b in zip(held, step()):
                 assert torch.equal(a, b)
+
+
+def test_second_gradients_are_refused():
+    from sleap_amd import ops
+
+    q, k, v, dout, _, _ = make(rng(30), 1, 4, 6, 1, 1, 16, torch.float16)
+    q.requires_grad_(True)
+    (dq,) = torch.autograd.grad(ops.cross_attention(q, k, v), q, dout, create_graph=True)
+    with pytest.raises(RuntimeError, match="first gradients only"):
+        dq.sum().backward()
+
+
+def test_a_changed_input_is_noticed():
+    from sleap_amd import ops
+
+    q, k, v, dout, lengths, _ = make(rng(31), 2, 4, 6, 1, 1, 16, torch.float16, "lengths")
+    for t in (k, lengths):
+        leaf = q.clone().requires_grad_(True)
+        out = ops.cross_attention(leaf, k, v, key_lengths=lengths)
+        t.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            out.backward(dout)
+
+
+def test_a_capture_beside_a_living_graph_of_its_leaves_is_refused():
+    from sleap_amd import ops
+
+    q, k, v, dout, _, _ = make(rng(32), 1, 4, 6, 1, 1, 16, torch.float16)
+    q.requires_grad_(True)
+    x = normal(rng(33), 1, 4, 1, 16, dtype=torch.float32).requires_grad_(True)
+    p = torch.zeros((4, 1), device=DEV)
+    eager = [ops.cross_attention(q, k, v), ops.rotary_axes(x, p, (4,))]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.zeros(1, device=DEV)
+        with pytest.raises(RuntimeError, match="holds the same leaf"):
+            ops.cross_attention(q, k, v)
+        with pytest.raises(RuntimeError, match="holds the same leaf"):
+            ops.rotary_axes(x, p, (4,))
+        held = ops.cross_attention(q.detach(), k, v)  # without a gradient: nothing to refuse
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, ops.cross_attention(q.detach(), k, v))
+    eager[0].backward(dout)  # the eager graphs are whole
+    eager[1].sum().backward()
+    assert q.grad is not None and x.grad is not None
+
+
+def test_two_calls_at_once_on_two_streams():
+    """Calls with scratch, from two threads on streams of their own, do not meet."""
+    import threading
+
+    from sleap_amd import ops
+
+    sets = [make(rng(34 + i), 2, 9, 3000 + 500 * i, 4, 2, 64, torch.bfloat16) for i in range(2)]
+    want = []
+    for q, k, v, dout, _, _ in sets:
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = ops.cross_attention(*leaves)
+        want.append([out.detach(), *torch.autograd.grad(out, leaves, dout)])
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        q, k, v, dout, _, _ = sets[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+                out = ops.cross_attention(*leaves)
+                got = [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 # --------------------------------------------------------------------------------------------------
@@ -388,6 +499,37 @@ def test_adamw_of_mixed_types_and_of_its_corners():
     for a, b in zip(p, before):
         assert oracle.worst(a, (b * 0.75, b.abs() * 1.01 * oracle.UNIT[a.dtype] + oracle.TINY[a.dtype])) <= 1
     ops.adamw_step([], [], [], [], step=1, lr=1.0)
+
+
+def test_adamw_refuses_what_it_would_write_twice():
+    from sleap_amd import ops
+
+    p, gr, m, v, _ = tensors(rng(26), [40, 40], torch.float32, False)
+    for lists in (([p[0], p[0]], gr, m, v), ([p[0][:30], p[0][20:]], [gr[0][:30], gr[0][20:]], [m[0][:30], m[1][:20]], [v[0][:30], v[1][:20]]),
+                  (p, gr, [m[0], m[0]], v), (p, gr, m, [m[0], v[1]]), (p, gr, [p[1], m[1]], v)):
+        with pytest.raises(ValueError, match="twice"):
+            ops.adamw_step(*lists, step=1, lr=1e-3)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.adamw_step([p[0][::2]], [gr[0][::2]], [m[0][::2]], [v[0][::2]], step=1, lr=1e-3)
+    with pytest.raises(ValueError, match="size"):
+        ops.adamw_step(p, [gr[0], gr[1][:7]], m, v, step=1, lr=1e-3)
+    with pytest.raises(TypeError, match="one type"):
+        ops.adamw_step(p, [t.half() for t in gr], m, v, step=1, lr=1e-3)
+    with pytest.raises(TypeError, match="float32"):
+        ops.adamw_step(p, gr, [t.half() for t in m], v, step=1, lr=1e-3)
+    with pytest.raises(ValueError, match="step"):
+        ops.adamw_step(p, gr, m, v, step=0, lr=1e-3)
+
+
+def test_an_adamw_step_is_noticed_by_graphs():
+    from sleap_amd import ops
+
+    w = normal(rng(27), 8, dtype=torch.float32).requires_grad_(True)
+    loss = (w * w).sum()
+    states = [torch.zeros(8, device=DEV) for _ in range(2)]
+    ops.adamw_step([w], [torch.ones(8, device=DEV)], states[:1], states[1:], step=1, lr=1e-3)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
 
 
 def test_a_captured_adamw_step_counts_on():

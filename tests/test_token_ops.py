@@ -37,6 +37,7 @@ def test_rotary_entry_point_refuses():
     refused(call(theta=0.0), "theta")
     refused(call(theta=math.inf), "theta")
     refused(call(interleaved=1, x=260), "interleaved")
+    refused(call(x=None), "null address")
     refused(call(interleaved=1, T=2, xs=(8, 9, 8)), "interleaved")
     assert call(B=0) == 0 and call(T=0) == 0
 
@@ -44,11 +45,11 @@ def test_rotary_entry_point_refuses():
 def test_attention_entry_points_refuse():
     h = _lib.lib()
 
-    def call(dtype=1, B=1, Tq=4, Tk=8, H=2, K=2, D=32, strides=(64, 64, 32) * 3, scale=1.0, q=256, k=256, out=256, ws=0, backward=False, so=(64, 64, 32)):
-        args = (q, k, 256, dtype, B, Tq, Tk, H, K, D, i64(*strides), None, None, None, scale)
+    def call(dtype=1, B=1, Tq=4, Tk=8, H=2, K=2, D=32, strides=(64, 64, 32) * 3, scale=1.0, q=256, k=256, out=256, ws=0, backward=False, so=(64, 64, 32), mask=None, wsp=256):
+        args = (q, k, 256, dtype, B, Tq, Tk, H, K, D, i64(*strides), None, mask, None, scale)
         if backward:
-            return h.sa_cross_attention_backward(*args, out, None, 256, 256, i64(*so), 256, 256, 256, 256, ws, None)
-        return h.sa_cross_attention(*args, out, None, None, 256, ws, None)
+            return h.sa_cross_attention_backward(*args, out, None, 256, 256, i64(*so), 256, 256, 256, wsp, ws, None)
+        return h.sa_cross_attention(*args, out, None, None, wsp, ws, None)
 
     for backward in (False, True):
         def no(text, **kw):
@@ -71,8 +72,14 @@ def test_attention_entry_points_refuse():
         no("token strides", strides=(64, 64, 32, 64, 1 << 23, 32, 64, 64, 32))
         no("addresses", q=264)
         no("addresses", out=264)
+        no("null address", q=None)
+        no("null address", k=None)
+        no("null address", out=None)
+        no("strides", mask=256)
     assert call(B=0) == 0 and call(Tq=0) == 0
     refused(call(Tq=1, Tk=100000), "workspace")
+    refused(call(Tq=1, Tk=100000, ws=1 << 40, wsp=None), "workspace")
+    refused(call(backward=True, ws=1 << 40, wsp=None), "workspace")
     refused(call(backward=True), "workspace")
     refused(call(backward=True, so=(64, 60, 32)), "strides")
     refused(call(backward=True, so=(64, 1 << 24, 32), ws=1 << 40), "span")
