@@ -374,17 +374,16 @@ __global__ __launch_bounds__(256) void attention_add_kernel(const AddParams p) {
   *reinterpret_cast<u32x4*>(static_cast<E*>(p.dst[k]) + i) = u32x4{pack2<E>(x[0], x[1]), pack2<E>(x[2], x[3]), pack2<E>(y[0], y[1]), pack2<E>(y[2], y[3])};
 }
 
-// How a side is cut: what it owns among waves of 32, what it walks among runs.
-Side cut(int waves, uint64_t heads, uint64_t own, uint64_t walk) {
+// How a side is cut: what it owns among waves of 32, what it walks among `splits` runs.
+Side cut(int waves, uint64_t heads, uint64_t own, uint64_t walk, double splits_) {
   Side c;
   c.tiles = (uint32_t)((own + waves * 32 - 1) / (waves * 32));
-  const uint64_t blocks = c.tiles * heads, want = 2048 / waves, walked = (walk + TILE - 1) / TILE;
-  uint64_t splits = blocks ? want / blocks : 1;
-  splits = std::max<uint64_t>(1, std::min(splits, walked / 4));
+  const uint64_t walked = (walk + TILE - 1) / TILE, most = std::max<uint64_t>(1, walked / 4);  // a run of at least four tiles
+  const uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(most, (uint64_t)(splits_ + 0.5)));
   const uint64_t per = std::max<uint64_t>(1, (walked + splits - 1) / splits);
   c.run = (int)(per * TILE);
   c.splits = (uint32_t)std::max<uint64_t>(1, (walked + per - 1) / per);
-  c.blocks = (uint32_t)std::min<uint64_t>(blocks * c.splits, 0xFFFFFFFFu);
+  c.blocks = (uint32_t)std::min<uint64_t>(c.tiles * heads * c.splits, 0xFFFFFFFFu);
   c.div_tiles = fast_div(std::max(1u, c.tiles));
   c.div_pieces = fast_div(std::max(1u, c.tiles * c.splits));
   return c;
@@ -400,8 +399,15 @@ Layout layout(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
   Layout l;
   const uint64_t R = (uint64_t)Tq * (Hq / Hkv), heads = (uint64_t)B * Hkv, most = std::max<uint64_t>(R, Tk);
   l.waves = most <= 32 ? 1 : most <= 64 ? 2 : 4;
-  l.kv = cut(l.waves, heads, Tk, R);
-  l.rows = cut(l.waves, heads, R, Tk);
+  // Work of a workgroup of each side in products of a tile, and what falls to one of the eight-waves-a-CU places. Fewer workgroups than
+  // places: runs of that length. More: of half of it, so that the last ones are short (8 x 4096 x 8192 x 128: 424 us, runs of the
+  // whole length 464; 3 x 2 x 1668 x 1531 x 40: 20 us, runs of half of it 24).
+  auto tiles = [](uint64_t n, uint64_t of) { return (n + of - 1) / of; };
+  const double places = 2048.0 / l.waves, nk = (double)(heads * tiles(Tk, l.waves * 32)), nr = (double)(heads * tiles(R, l.waves * 32));
+  const double wk = 4.0 * tiles(R, TILE), wr = 3.0 * tiles(Tk, TILE);
+  const double each = (nk * wk + nr * wr) / places * (nk + nr <= places ? 1.0 : 0.5);
+  l.kv = cut(l.waves, heads, Tk, R, each > 0 ? wk / each : 1);
+  l.rows = cut(l.waves, heads, R, Tk, each > 0 ? wr / each : 1);
   l.stats = ((size_t)B * Hq * Tq + 3) / 4 * 4;
   l.dq = l.rows.splits > 1 ? (size_t)l.rows.splits * B * Hq * Tq * D : 0;
   l.dkv = l.kv.splits > 1 ? (size_t)l.kv.splits * B * Hkv * Tk * D : 0;
