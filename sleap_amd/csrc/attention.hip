@@ -259,7 +259,7 @@ struct Cut {
   uint32_t row_tiles, splits;
   int split_keys;
 };
-Cut cut(int B, int Tq, int Tk, int Hq, int Hkv) {
+Cut cut(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
   const uint64_t R = (uint64_t)Tq * (Hq / Hkv);
   Cut c;
   c.waves = R <= 32 ? 1 : R <= 64 ? 2 : 4;
@@ -271,6 +271,20 @@ Cut cut(int B, int Tq, int Tk, int Hq, int Hkv) {
   const uint64_t most = key_tiles / 4;   // a run of at least four tiles
   if (splits > most) splits = most;
   if (splits < 1) splits = 1;
+  if (c.waves == 4 && blocks > want) {
+    // More workgroups than places: the last round may be nearly empty. Runs even it out and cost a float32 result written and read
+    // for each; in microseconds, a tile at two workgroups a CU 0.45 + 0.005 D, 4 bytes a value twice at 4 TB/s, 6 for the launch that joins.
+    // (17 heads x 4096 x 8192 x 128, 544 workgroups: 402 us whole, 337 in the runs chosen here; 1024 of them, 16 heads x 4096 x 16384 x 128, stay whole.)
+    double best = 0;
+    for (uint64_t s = 1; s <= 8 && (s == 1 || s <= most); ++s) {
+      const double rounds = (double)((blocks * s + want - 1) / want), run = (double)((key_tiles + s - 1) / s);
+      const double cost = rounds * run * (0.45 + 0.005 * D) + (s > 1 ? 6 + (double)s * R * B * Hkv * D * 8 / 4e6 : 0);
+      if (s == 1 || cost < best) {
+        best = cost;
+        splits = s;
+      }
+    }
+  }
   const uint32_t per = key_tiles ? (uint32_t)((key_tiles + splits - 1) / splits) : 1;
   c.split_keys = (int)per * TILE;
   c.splits = key_tiles ? (key_tiles + per - 1) / per : 1;
@@ -351,7 +365,7 @@ int attention_shape(const char* who, AttnShape* a, const void* q, const void* k,
 
 extern "C" size_t sa_cross_attention_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
   if (B < 1 || Tq < 1 || Tk < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1) return 0;
-  const Cut c = cut(B, Tq, Tk, Hq, Hkv);
+  const Cut c = cut(B, Tq, Tk, Hq, Hkv, D);
   return c.splits > 1 ? (size_t)B * Hq * Tq * c.splits * (D + 1) * sizeof(float) : 0;
 }
 
@@ -363,7 +377,7 @@ extern "C" int sa_cross_attention(const void* q, const void* k, const void* v, i
   if (B == 0 || Tq == 0) return SA_OK;
   SA_REQUIRE(out, "sa_cross_attention: null address");
   SA_REQUIRE((((uintptr_t)out | (uintptr_t)out_low | (uintptr_t)workspace) & 15) == 0, "sa_cross_attention: addresses are multiples of 16");
-  const Cut c = cut(B, Tq, Tk, Hq, Hkv);
+  const Cut c = cut(B, Tq, Tk, Hq, Hkv, D);
   const uint64_t blocks = (uint64_t)c.row_tiles * c.splits * B * Hkv;
   SA_REQUIRE(blocks < (1ull << 31) && (uint64_t)B * Hq * Tq < (1ull << 31) - 1024, "sa_cross_attention: too many rows");
   if (c.splits > 1 && (!workspace || workspace_bytes < sa_cross_attention_workspace(B, Tq, Tk, Hq, Hkv, D)))
