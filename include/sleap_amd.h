@@ -761,7 +761,7 @@ int sa_cross_attention_backward(const void* q, const void* k, const void* v, int
 
 /* One AdamW step over n tensors of one type, in place (decoupled decay; 32-bit states and arithmetic; a 16-bit parameter is rounded once):
  *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  [vmax = max(vmax, v)];  p = p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v | vmax)/sqrt(1-b2^t) + eps)
- *   tensors    HOST array; its addresses travel in the launches' arguments (64 tensors a launch): nothing is kept after the call
+ *   tensors    HOST array; its addresses (48 bits) travel in the launches' arguments (128 tensors a launch, 108 with amsgrad): nothing is kept after the call
  *   step       t >= 1, or step_dev: DEVICE counter that already holds t (a captured step); lr_dev: DEVICE learning rate or NULL */
 typedef struct {
   void* param;             /* dtype, n contiguous values */

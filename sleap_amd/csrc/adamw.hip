@@ -4,8 +4,8 @@
 // in 32 bits per value whatever the parameter's type; a 16-bit parameter is rounded once, to nearest.
 //
 // Memory bound: 28 bytes a value with float32 parameters (36 with the running maximum). A launch carries the addresses of up to
-// SLOTS tensors in its arguments -- no table in device memory to fill, nothing kept between calls, and a captured launch holds its
-// own copy -- and as many workgroups as the tensors have pieces of CHUNK values; a workgroup finds its tensor with one ballot.
+// 128 tensors in its arguments -- no table in device memory to fill, nothing kept between calls, and a captured launch holds its
+// own copy -- and as many workgroups as the tensors have pieces of CHUNK values; a workgroup finds its tensor with two ballots.
 #include "sa_common.h"
 #include "token_types.h"
 
@@ -13,26 +13,34 @@ namespace {
 
 using namespace sa;
 
-constexpr int SLOTS = 64;      // 64 x 48 bytes + the piece table: within the 4 KB of kernel arguments
-constexpr int CHUNK = 4096;    // values of a workgroup: 256 threads x 4 pieces of 4
+constexpr int CHUNK = 4096;  // values of a workgroup: 256 threads x 4 pieces of 4
 
+// What a workgroup has of its tensor
 struct Slot {
   void* p;
   const void* g;
   float *m, *v, *w;
-  int64_t n;
+  int n;
 };
 
+// As many tensors as the 4 KB of kernel arguments hold (448 tensors of four addresses: 4 launches; as plain structures of 48 bytes 7): 48-bit
+// addresses in two parts, and of the size only what the workgroups' numbers do not say already.
+template <bool AMS>
 struct AdamwParams {
-  Slot slot[SLOTS];
-  uint32_t first[SLOTS];      // first workgroup of each tensor
+  static constexpr int ADDRESSES = AMS ? 5 : 4, SLOTS = AMS ? 108 : 128;
+  uint32_t low[ADDRESSES][SLOTS];
+  uint16_t high[ADDRESSES][SLOTS];
+  uint16_t tail[SLOTS];     // values of a tensor's last workgroup
+  uint32_t first[SLOTS];    // first workgroup of each tensor
+  uint32_t blocks;
   int n;
   float lr, decay, b1, b2, eps;
-  float c1, c2;               // 1 - b1^t, sqrt(1 - b2^t) of a step counted on the host
-  const float* lr_dev;        // a learning rate in device memory (or NULL)
-  const int64_t* step_dev;    // a step counter in device memory (or NULL)
+  float c1, c2;             // 1 - b1^t, sqrt(1 - b2^t) of a step counted on the host
+  const float* lr_dev;      // a learning rate in device memory (or NULL)
+  const int64_t* step_dev;  // a step counter in device memory (or NULL)
   double b1d, b2d;
 };
+static_assert(sizeof(AdamwParams<false>) <= 4096 && sizeof(AdamwParams<true>) <= 4096, "kernel arguments");
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
@@ -53,19 +61,18 @@ __device__ __forceinline__ void one(float& p, float g, float& m, float& v, float
 }
 
 template <typename T, bool AMS, int V>
-__device__ __forceinline__ void chunk(const Slot& s, int64_t at, const Rates& r) {
+__device__ __forceinline__ void chunk(const Slot& s, const Rates& r) {
   T* p = static_cast<T*>(s.p);
   const T* g = static_cast<const T*>(s.g);
-  const int64_t end = min(at + CHUNK, s.n);
   constexpr int K = CHUNK / (256 * V);
-  if (V > 1 && end - at == CHUNK) {  // a whole piece: every load is issued before the first use
+  if (V > 1 && s.n == CHUNK) {  // a whole piece: every load is issued before the first use
     using VT = Vec<T, V>;
     using VF = Vec<float, V>;
     VT pp[K], gg[K];
     VF mm[K], vv[K], ww[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int64_t i = at + (k * 256 + threadIdx.x) * V;
+      const int i = (k * 256 + threadIdx.x) * V;
       pp[k] = *reinterpret_cast<const VT*>(p + i);
       gg[k] = *reinterpret_cast<const VT*>(g + i);
       mm[k] = *reinterpret_cast<const VF*>(s.m + i);
@@ -74,7 +81,7 @@ __device__ __forceinline__ void chunk(const Slot& s, int64_t at, const Rates& r)
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int64_t i = at + (k * 256 + threadIdx.x) * V;
+      const int i = (k * 256 + threadIdx.x) * V;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float x = to_f32(pp[k].e[e]);
@@ -88,7 +95,7 @@ __device__ __forceinline__ void chunk(const Slot& s, int64_t at, const Rates& r)
     }
     return;
   }
-  for (int64_t i = at + threadIdx.x; i < end; i += 256) {
+  for (int i = threadIdx.x; i < s.n; i += 256) {
     float x = to_f32(p[i]), m = s.m[i], v = s.v[i], w = AMS ? s.w[i] : 0.0f;
     one<AMS>(x, to_f32(g[i]), m, v, w, r);
     p[i] = from_f32<T>(x);
@@ -99,11 +106,15 @@ __device__ __forceinline__ void chunk(const Slot& s, int64_t at, const Rates& r)
 }
 
 template <typename T, bool AMS>
-__global__ __launch_bounds__(256) void adamw_kernel(const AdamwParams a) {
-  // the last tensor that begins at or before this workgroup: one read and a ballot (SLOTS == lanes of a wave)
-  const uint32_t lane = threadIdx.x & 63;
-  const uint64_t begun = __ballot((int)lane < a.n && a.first[lane] <= blockIdx.x);
-  const int lo = __builtin_amdgcn_readfirstlane(63 - __clzll(begun));
+__global__ __launch_bounds__(256) void adamw_kernel(const AdamwParams<AMS> a) {
+  // the last tensor that begins at or before this workgroup: two reads and ballots for up to 128
+  const int lane = threadIdx.x & 63;
+  const uint64_t one_ = __ballot(lane < a.n && a.first[lane] <= blockIdx.x);
+  const uint64_t two = __ballot(lane + 64 < a.n && a.first[min(lane + 64, a.SLOTS - 1)] <= blockIdx.x);
+  const int slot = __builtin_amdgcn_readfirstlane(two ? 127 - __clzll(two) : 63 - __clzll(one_));
+  const uint32_t begin = a.first[slot], end = slot + 1 < a.n ? a.first[slot + 1] : a.blocks;
+  const int64_t at = (int64_t)(blockIdx.x - begin) * CHUNK;
+  auto address = [&](int k) { return (uint64_t)a.high[k][slot] << 32 | a.low[k][slot]; };
   float c1 = a.c1, c2 = a.c2;
   if (a.step_dev) {
     const double t = (double)*a.step_dev;
@@ -112,18 +123,46 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwParams a) {
   }
   const float lr = a.lr_dev ? *a.lr_dev : a.lr;
   const Rates r = {a.b1, (float)(1.0 - a.b1d), a.b2, (float)(1.0 - a.b2d), a.eps, 1.0f - lr * a.decay, lr / c1, 1.0f / c2};
-  const Slot s = a.slot[lo];
+  Slot s;
+  s.p = reinterpret_cast<T*>(address(0)) + at;
+  s.g = reinterpret_cast<const T*>(address(1)) + at;
+  s.m = reinterpret_cast<float*>(address(2)) + at;
+  s.v = reinterpret_cast<float*>(address(3)) + at;
+  s.w = AMS ? reinterpret_cast<float*>(address(AMS ? 4 : 0)) + at : nullptr;
+  s.n = blockIdx.x + 1 == end ? a.tail[slot] : CHUNK;
   const uint64_t any = (uint64_t)s.m | (uint64_t)s.v | (AMS ? (uint64_t)s.w : 0);
   const bool wide = any % 16 == 0 && ((uint64_t)s.p | (uint64_t)s.g) % (4 * sizeof(T)) == 0;
-  const int64_t at = (int64_t)(blockIdx.x - a.first[lo]) * CHUNK;
-  if (wide) chunk<T, AMS, 4>(s, at, r);
-  else chunk<T, AMS, 1>(s, at, r);
+  if (wide) chunk<T, AMS, 4>(s, r);
+  else chunk<T, AMS, 1>(s, r);
 }
 
-template <typename T>
-void launch(const AdamwParams& a, bool ams, uint32_t blocks, hipStream_t s) {
-  if (ams) adamw_kernel<T, true><<<dim3(blocks), dim3(256), 0, s>>>(a);
-  else adamw_kernel<T, false><<<dim3(blocks), dim3(256), 0, s>>>(a);
+template <bool AMS>
+int step_all(AdamwParams<AMS>& a, const sa_adamw_tensor* tensors, int n, int dtype, hipStream_t s) {
+  for (int at = 0; at < n;) {
+    a.n = 0;
+    a.blocks = 0;
+    for (; at < n && a.n < a.SLOTS; ++at) {
+      const sa_adamw_tensor& t = tensors[at];
+      if (t.n == 0) continue;
+      const void* address[5] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.max_exp_avg_sq};
+      for (int k = 0; k < a.ADDRESSES; ++k) {
+        a.low[k][a.n] = (uint32_t)(uintptr_t)address[k];
+        a.high[k][a.n] = (uint16_t)((uintptr_t)address[k] >> 32);
+      }
+      const uint32_t pieces = (uint32_t)((t.n + CHUNK - 1) / CHUNK);
+      if (a.n && (uint64_t)a.blocks + pieces >= (1ull << 31)) break;  // a launch's workgroups
+      a.tail[a.n] = (uint16_t)(t.n - (int64_t)(pieces - 1) * CHUNK);
+      a.first[a.n++] = a.blocks;
+      a.blocks += pieces;
+    }
+    if (a.n == 0) break;
+    const dim3 grid(a.blocks), block(256);
+    if (dtype == SA_F32) adamw_kernel<float, AMS><<<grid, block, 0, s>>>(a);
+    else if (dtype == SA_F16) adamw_kernel<_Float16, AMS><<<grid, block, 0, s>>>(a);
+    else adamw_kernel<__bf16, AMS><<<grid, block, 0, s>>>(a);
+    SA_LAUNCH_CHECK();
+  }
+  return SA_OK;
 }
 
 }  // namespace
@@ -139,36 +178,28 @@ extern "C" int sa_adamw_step(const sa_adamw_tensor* tensors, int n, int dtype, i
     const sa_adamw_tensor& t = tensors[i];
     SA_REQUIRE(t.n >= 0 && (t.n == 0 || (t.param && t.grad && t.exp_avg && t.exp_avg_sq && (!amsgrad || t.max_exp_avg_sq))),
                "sa_adamw_step: tensor %d has a negative size or a null address", i);
+    SA_REQUIRE((((uintptr_t)t.param | (uintptr_t)t.grad | (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq | (uintptr_t)(amsgrad ? t.max_exp_avg_sq : nullptr)) >> 48) == 0,
+               "sa_adamw_step: tensor %d: addresses have 48 bits", i);
     SA_REQUIRE((t.n + CHUNK - 1) / CHUNK < (1ll << 24), "sa_adamw_step: tensor %d has more than 2^36 values", i);
   }
-  AdamwParams a;
-  a.lr = (float)lr;
-  a.decay = (float)weight_decay;
-  a.b1 = (float)beta1;
-  a.b2 = (float)beta2;
-  a.eps = (float)eps;
-  a.b1d = beta1;
-  a.b2d = beta2;
-  a.c1 = (float)(1.0 - pow(beta1, (double)step));
-  a.c2 = (float)sqrt(1.0 - pow(beta2, (double)step));
-  a.lr_dev = lr_dev;
-  a.step_dev = step_dev;
-  for (int at = 0; at < n;) {
-    a.n = 0;
-    uint32_t blocks = 0;
-    for (; at < n && a.n < SLOTS; ++at) {
-      const sa_adamw_tensor& t = tensors[at];
-      if (t.n == 0) continue;
-      a.slot[a.n] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.max_exp_avg_sq, t.n};
-      a.first[a.n++] = blocks;
-      blocks += (uint32_t)((t.n + CHUNK - 1) / CHUNK);
-    }
-    if (a.n == 0) break;
-    const hipStream_t s = (hipStream_t)stream;
-    if (dtype == SA_F32) launch<float>(a, amsgrad, blocks, s);
-    else if (dtype == SA_F16) launch<_Float16>(a, amsgrad, blocks, s);
-    else launch<__bf16>(a, amsgrad, blocks, s);
-    SA_LAUNCH_CHECK();
+  auto go = [&](auto& a) {
+    a.lr = (float)lr;
+    a.decay = (float)weight_decay;
+    a.b1 = (float)beta1;
+    a.b2 = (float)beta2;
+    a.eps = (float)eps;
+    a.b1d = beta1;
+    a.b2d = beta2;
+    a.c1 = (float)(1.0 - pow(beta1, (double)step));
+    a.c2 = (float)sqrt(1.0 - pow(beta2, (double)step));
+    a.lr_dev = lr_dev;
+    a.step_dev = step_dev;
+    return step_all(a, tensors, n, dtype, (hipStream_t)stream);
+  };
+  if (amsgrad) {
+    AdamwParams<true> a;
+    return go(a);
   }
-  return SA_OK;
+  AdamwParams<false> a;
+  return go(a);
 }

@@ -346,14 +346,18 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
   if (n == 0) return;
 
   std::map<std::pair<int, int>, std::vector<sa_adamw_tensor>> groups;  // by type and device
-  std::vector<std::pair<uintptr_t, uintptr_t>> written;  // where each thing that the step writes begins and ends
-  written.reserve(n * (lists - 1));
+  std::pair<int, int> last_key = {-1, -1};
+  std::vector<sa_adamw_tensor>* last = nullptr;
+  using Range = std::pair<uintptr_t, uintptr_t>;  // where something that the step writes begins and ends
+  std::vector<Range> written[5];
+  for (int j = 0; j < lists; ++j)
+    if (j != 1) written[j].reserve(n);
   for (Py_ssize_t i = 0; i < n; ++i) {
     const Tensor* x[5] = {};
     for (int j = 0; j < lists; ++j) {
       if (!THPVariable_Check(items[j][i])) bad_value(who, ": lists of CUDA tensors: ", names[j], "[", i, "] is none");
       x[j] = &THPVariable_Unpack(items[j][i]);
-      if (!x[j]->is_cuda() || x[j]->device() != x[0]->device())
+      if (!x[j]->is_cuda() || x[j]->get_device() != x[0]->get_device())
         bad_value(who, ": CUDA tensors, a parameter, its gradient and its states on one GPU (there is no CPU fallback): ", names[j], "[", i, "] is on ", x[j]->device());
       if (x[j]->layout() != at::kStrided || !x[j]->is_contiguous()) bad_value(who, ": ", names[j], "[", i, "] must be contiguous");
       if (x[j]->numel() != x[0]->numel()) bad_value(who, ": ", names[j], "[", i, "] differs in size from its parameter");
@@ -363,17 +367,31 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
     if (type < 0 || x[1]->scalar_type() != x[0]->scalar_type())
       bad_type(who, ": params and grads must be pairs of one type: float32, float16 or bfloat16");
     if (x[0]->numel() == 0) continue;
-    groups[{type, x[0]->get_device()}].push_back({x[0]->data_ptr(), x[1]->data_ptr(), x[2]->data_ptr<float>(), x[3]->data_ptr<float>(),
-                                                  ams ? x[4]->data_ptr<float>() : nullptr, x[0]->numel()});
-    for (int j = 0; j < lists; ++j)
-      if (j != 1) {
-        const auto at = reinterpret_cast<uintptr_t>(x[j]->data_ptr());
-        written.push_back({at, at + x[j]->nbytes()});
-      }
+    const std::pair<int, int> key = {type, (int)x[0]->get_device()};
+    if (key != last_key) {
+      last_key = key;
+      last = &groups[key];
+      if (last->empty()) last->reserve(n);
+    }
+    const int64_t count = x[0]->numel();
+    void* at[5] = {};
+    for (int j = 0; j < lists; ++j) {
+      at[j] = x[j]->data_ptr();
+      if (j != 1) written[j].push_back({reinterpret_cast<uintptr_t>(at[j]), reinterpret_cast<uintptr_t>(at[j]) + count * (j ? 4 : x[0]->element_size())});
+    }
+    last->push_back({at[0], at[1], static_cast<float*>(at[2]), static_cast<float*>(at[3]), static_cast<float*>(at[4]), count});
   }
-  std::sort(written.begin(), written.end());
-  for (size_t i = 1; i < written.size(); ++i)
-    if (written[i].first < written[i - 1].second) bad_value(who, ": the same parameter or state twice, or two that overlap");
+  // Lists are mostly in the order of their addresses: sorted one by one where they are not, and merged, the whole check is linear.
+  std::vector<Range> all;
+  all.reserve(n * (lists - 1));
+  for (auto& w : written) {
+    if (!std::is_sorted(w.begin(), w.end())) std::sort(w.begin(), w.end());
+    const auto middle = (ptrdiff_t)all.size();
+    all.insert(all.end(), w.begin(), w.end());
+    if (middle && !w.empty() && all[middle] < all[middle - 1]) std::inplace_merge(all.begin(), all.begin() + middle, all.end());
+  }
+  for (size_t i = 1; i < all.size(); ++i)
+    if (all[i].first < all[i - 1].second) bad_value(who, ": the same parameter or state twice, or two that overlap");
   for (const auto& [key, tensors] : groups)
     for (const py::object* o : {&step, &lr})
       if (THPVariable_Check(o->ptr()) && THPVariable_Unpack(o->ptr()).get_device() != key.second)

@@ -448,7 +448,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, return
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_exp_avg_sqs=None):
-    """One AdamW step over many tensors, in place, in as few launches as there are 64 tensors of one type and device:
+    """One AdamW step over many tensors, in place, a launch for up to 128 of one type and device:
 
         m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  [vmax = max(vmax, v)]
         p = p (1 - lr wd) - lr / (1-b1^t) m / (sqrt(v or vmax) / sqrt(1-b2^t) + eps)
