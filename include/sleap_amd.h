@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define SA_ABI_VERSION 8  /* 8 (round 6): + sa_h264_decode_slice. 7 (round 6): + sa_find_local_peaks_rough; sa_conv3x3_pair_bf16 accepts 32 -> 64 -> 64. 6 (round 5): + sa_conv3x3_set_persistent. 5 (round 4): + sa_conv3x3_ex_heads_bf16. 4 (round 4): + sa_tensor_absmax, sa_imgconv_pack_tiled, sa_pack_pointwise_weights,
+#define SA_ABI_VERSION 8  /* + sa_rotary_axes, sa_cross_attention*, sa_adamw_step: additions alone, what was there is as it was. 8 (round 6): + sa_h264_decode_slice. 7 (round 6): + sa_find_local_peaks_rough; sa_conv3x3_pair_bf16 accepts 32 -> 64 -> 64. 6 (round 5): + sa_conv3x3_set_persistent. 5 (round 4): + sa_conv3x3_ex_heads_bf16. 4 (round 4): + sa_tensor_absmax, sa_imgconv_pack_tiled, sa_pack_pointwise_weights,
                             sa_pointwise_packed_elems, sa_conv3x3_bneck_bf16; SA_LAYOUT_PLANES16 accepted in the `relu` argument of
                             sa_conv1x1_bf16 / sa_convk_bf16 / sa_convt_s2_bf16 */
 

@@ -11,11 +11,9 @@
 // {4h .. 4h + 3, 8 + 4h .. 8 + 4h + 3}, h = l >> 5. The A operand in that order is two transposed reads from LDS
 // (ds_read_b64_tr_b16: 16 lanes read four rows of 16 values and lane i gets column i), so no value of a softmax passes through LDS.
 //
-// Tiles in LDS are rows of DP 16-bit values (DP = 32, 64 or 128). Pieces of 16 bytes are exchanged within a row, piece c to
-// c ^ swizzle(row), in steps of 32 bytes, so that eight rows read at one piece (A operand) and four rows read at 32 neighbouring
-// bytes (transposed) fall into different banks. Tiles come by buffer_load ... lds: the swizzle is applied to the source offset,
-// and a lane whose key is hidden or whose piece lies behind D gets an offset out of range, which writes zeros: what hidden
-// keys hold (NaN, infinities) never enters a product.
+// Tiles in LDS are rows of DP 16-bit values (DP = 32, 64 or 128), the 16-byte pieces of a row exchanged against bank conflicts (swizzle
+// below). They come by buffer_load ... lds: the exchange is applied to the source offset, and a lane whose key is hidden or whose
+// piece lies behind D gets an offset out of range, which writes zeros: what hidden keys hold (NaN, infinities) never enters a product.
 #pragma once
 #include "sa_common.h"
 #include "token_types.h"
