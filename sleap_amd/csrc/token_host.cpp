@@ -16,6 +16,7 @@
 #include <cmath>
 #include <map>
 #include <sstream>
+#include <unordered_set>
 
 #include "../../include/sleap_amd.h"
 
@@ -81,18 +82,30 @@ void on_one_gpu(const char* who, std::initializer_list<std::pair<const char*, co
   }
 }
 
-bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+bool capturing(const at::Device& d) {
+  const c10::OptionalDeviceGuard guard(d);
+  return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
 
-// A graph that was built outside of a capture and still lives holds the leaf's gradient node, and with it the stream that it was built on:
-// a captured backward pass would pull that stream into the capture, where torch's engine ends the process. Refused before it starts.
+// A graph that was built outside of a capture and still lives holds the gradient nodes of its leaves, and with them the stream that it was
+// built on: a captured backward pass that reaches one of its nodes would pull that stream into the capture, where torch's engine ends the
+// process. Refused before it starts; everything that the inputs hang on is looked at, while capturing only.
 void not_held_elsewhere(const char* who, std::initializer_list<const Tensor*> tensors) {
-  if (!capturing()) return;
-  for (const Tensor* t : tensors) {
-    if (!t->requires_grad() || !t->is_leaf()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-    const auto held = node ? node->stream() : std::nullopt;
-    if (held && held->id() != c10::hip::getCurrentHIPStream(t->get_device()).id())
+  if (!capturing((*tensors.begin())->device())) return;
+  std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+  std::unordered_set<const torch::autograd::Node*> met;
+  auto meet = [&](const std::shared_ptr<torch::autograd::Node>& node) {
+    if (node && met.insert(node.get()).second) todo.push_back(node);
+  };
+  for (const Tensor* t : tensors)
+    if (t->requires_grad()) meet(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+  while (!todo.empty()) {
+    const auto node = std::move(todo.back());
+    todo.pop_back();
+    const auto held = node->stream();
+    if (held && held->id() != c10::hip::getCurrentHIPStream(held->device_index()).id())
       throw std::runtime_error(text(who, ": captured while a graph from outside of the capture holds the same leaf: delete that graph first (or capture a detached leaf)"));
+    for (const auto& edge : node->next_edges()) meet(edge.function);
   }
 }
 
@@ -396,10 +409,12 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
     for (const py::object* o : {&step, &lr})
       if (THPVariable_Check(o->ptr()) && THPVariable_Unpack(o->ptr()).get_device() != key.second)
         bad_value(who, ": step and learning rate tensors must be on the GPU of the parameters");
-  if (!groups.empty() && !dev_step && capturing())
-    throw std::runtime_error("adamw_step: a captured step needs its count as a tensor (every replay would repeat this one)");
+  auto device_of = [](const std::pair<int, int>& key) { return c10::Device(c10::kCUDA, (c10::DeviceIndex)key.second); };
+  for (const auto& [key, tensors] : groups)
+    if (!dev_step && capturing(device_of(key)))
+      throw std::runtime_error("adamw_step: a captured step needs its count as a tensor (every replay would repeat this one)");
   for (const auto& [key, tensors] : groups) {
-    const c10::Device device(c10::kCUDA, (c10::DeviceIndex)key.second);
+    const c10::Device device = device_of(key);
     const c10::OptionalDeviceGuard guard(device);
     check(entry.adamw_step(tensors.data(), (int)tensors.size(), key.first, ams, rate, dev_lr ? THPVariable_Unpack(lr.ptr()).data_ptr<float>() : nullptr, b1, b2,
                          eps, weight_decay, t, dev_step ? THPVariable_Unpack(step.ptr()).data_ptr<int64_t>() : nullptr, stream_of(device)),

@@ -420,6 +420,29 @@ def test_a_capture_beside_a_living_graph_of_its_leaves_is_refused():
     assert q.grad is not None and x.grad is not None
 
 
+def test_a_capture_on_top_of_a_living_graph_is_refused():
+    """As above where the held leaf, or a node from outside of the capture, is not an input itself but what an input hangs on."""
+    from sleap_amd import ops
+
+    q, k, v, dout, _, _ = make(rng(34), 1, 4, 6, 1, 1, 16, torch.float16)
+    q.requires_grad_(True)
+    twice = q * 2
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.zeros(1, device=DEV)
+        for call in (lambda: ops.cross_attention(twice, k, v), lambda: ops.cross_attention(q * 3, k, v), lambda: ops.cross_attention(k, (q * 3)[:, :1].expand(1, 6, 1, 16), v),
+                     lambda: ops.rotary_axes(twice, torch.zeros((4, 1), device=DEV), (4,))):
+            with pytest.raises(RuntimeError, match="holds the same leaf"):
+                call()
+    twice.backward(dout)  # the eager graph is whole
+    assert torch.equal(q.grad, dout * 2)
+    del twice
+    leaf = q.detach().requires_grad_(True)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        ops.cross_attention(leaf * 3, k, v)  # built in the capture altogether
+
+
 def test_two_calls_at_once_on_two_streams():
     """Calls with scratch, from two threads on streams of their own, do not meet."""
     import threading
