@@ -363,8 +363,8 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
   std::vector<sa_adamw_tensor>* last = nullptr;
   using Range = std::pair<uintptr_t, uintptr_t>;  // where something that the step writes begins and ends
   std::vector<Range> written[5];
-  for (int j = 0; j < lists; ++j)
-    if (j != 1) written[j].reserve(n);
+  std::vector<Range> read;  // the gradients; one may be its own parameter, whose values are read ahead of being written
+  for (int j = 0; j < lists; ++j) (j == 1 ? read : written[j]).reserve(n);
   for (Py_ssize_t i = 0; i < n; ++i) {
     const Tensor* x[5] = {};
     for (int j = 0; j < lists; ++j) {
@@ -390,7 +390,10 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
     void* at[5] = {};
     for (int j = 0; j < lists; ++j) {
       at[j] = x[j]->data_ptr();
-      if (j != 1) written[j].push_back({reinterpret_cast<uintptr_t>(at[j]), reinterpret_cast<uintptr_t>(at[j]) + count * (j ? 4 : x[0]->element_size())});
+      const auto begin = reinterpret_cast<uintptr_t>(at[j]);
+      const Range range = {begin, begin + count * (j >= 2 ? 4 : x[0]->element_size())};
+      if (j != 1) written[j].push_back(range);
+      else if (at[1] != at[0]) read.push_back(range);
     }
     last->push_back({at[0], at[1], static_cast<float*>(at[2]), static_cast<float*>(at[3]), static_cast<float*>(at[4]), count});
   }
@@ -405,6 +408,12 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
   }
   for (size_t i = 1; i < all.size(); ++i)
     if (all[i].first < all[i - 1].second) bad_value(who, ": the same parameter or state twice, or two that overlap");
+  if (!std::is_sorted(read.begin(), read.end())) std::sort(read.begin(), read.end());
+  size_t next = 0;
+  for (const Range& r : read) {
+    while (next < all.size() && all[next].second <= r.first) ++next;
+    if (next < all.size() && all[next].first < r.second) bad_value(who, ": a gradient overlaps with something that the step writes");
+  }
   for (const auto& [key, tensors] : groups)
     for (const py::object* o : {&step, &lr})
       if (THPVariable_Check(o->ptr()) && THPVariable_Unpack(o->ptr()).get_device() != key.second)

@@ -454,7 +454,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
         p = p (1 - lr wd) - lr / (1-b1^t) m / (sqrt(v or vmax) / sqrt(1-b2^t) + eps)
 
     params, grads   lists of contiguous float32 / float16 / bfloat16 CUDA tensors, pairwise of one type and size; arithmetic is float32, a
-                    16-bit parameter is rounded to nearest once a step (steps below half its spacing are lost)
+                    16-bit parameter is rounded to nearest once a step (steps below half its spacing are lost). What is written
+                    overlaps with nothing else that is written or read (a gradient may serve several parameters, or be its own)
     exp_avgs, exp_avg_sqs, max_exp_avg_sqs (amsgrad, or None)   float32 tensors of the same sizes
     step            t >= 1, or a one-element int64 CUDA tensor that already holds it; lr likewise a number or a one-element float32 CUDA
                     tensor. A captured step takes its count as a tensor only, and a learning rate given as a number stays that of the capture."""

@@ -524,6 +524,24 @@ def test_adamw_of_mixed_types_and_of_its_corners():
     ops.adamw_step([], [], [], [], step=1, lr=1.0)
 
 
+def test_adamw_refuses_gradients_in_what_it_writes():
+    from sleap_amd import ops
+
+    p, gr, m, v, _ = tensors(rng(35), [40, 40], torch.float32, False)
+    pool = torch.zeros(100, device=DEV)
+    for lists in (([p[0]], [p[1]], [m[0]], [p[1]]), (p, [gr[0], p[0]], m, v), (p, [m[1], gr[1]], m, v), (p, [gr[0], v[1]], m, v), ([pool[:40], p[1]], [gr[0], pool[39:79]], m, v),
+                  ([pool[40:80], p[1]], [gr[0], pool[1:41]], m, v)):
+        with pytest.raises(ValueError, match="a gradient overlaps"):
+            ops.adamw_step(*lists, step=1, lr=1e-3)
+    # two parameters of one gradient, neighbours in memory, and a parameter that is its own gradient, are whole
+    pool = normal(rng(36), 120, dtype=torch.float32)
+    args = ([pool[:40], pool[80:], p[0]], [pool[40:80], pool[40:80], p[0]], [*m, torch.zeros_like(m[0])], [*v, torch.zeros_like(v[0])])
+    alone = [[t.clone() for t in x] for x in args]
+    ops.adamw_step(*args, step=1, lr=1e-3)
+    ops.adamw_step(*alone, step=1, lr=1e-3)
+    assert all(torch.equal(a, b) for j in (0, 2, 3) for a, b in zip(args[j], alone[j]))
+
+
 def test_adamw_refuses_what_it_would_write_twice():
     from sleap_amd import ops
 
