@@ -30,12 +30,20 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group({**group, "params": params})
 
     def load_state_dict(self, state_dict):
-        """As torch's, but the states keep float32 (torch's casts them to their parameter's type)."""
+        """As torch's, but the states keep float32 (torch's casts them to their parameter's type). Takes what torch's Adam and AdamW saved
+        (their step is a tensor), unless they maximize or decay otherwise."""
+        for group in state_dict["param_groups"]:
+            if group.get("maximize"):
+                raise ValueError("AdamW: a state of an optimizer with maximize")
+            if group.get("weight_decay") and not group.get("decoupled_weight_decay", True):
+                raise ValueError("AdamW: a state of an optimizer whose weight decay is not decoupled")
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for p, i in zip((p for g in self.param_groups for p in g["params"]), saved):
             for name, value in state_dict["state"].get(i, {}).items():
-                if isinstance(value, torch.Tensor):
+                if name == "step":
+                    value = int(value)
+                elif isinstance(value, torch.Tensor):
                     value = value.detach().to(device=p.device, dtype=torch.float32, copy=True).contiguous()
                 self.state[p][name] = value
 

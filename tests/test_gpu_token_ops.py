@@ -649,6 +649,34 @@ def test_the_optimizer_keeps_float32_states_of_16_bit_parameters():
             opt.step()
 
 
+def test_the_optimizer_goes_on_from_a_state_of_torch():
+    """What torch's AdamW saved (a float32 tensor as step) continues: a step from it is `ops.adamw_step` with the next count; what this
+    optimizer would do otherwise is refused."""
+    from sleap_amd import ops
+    from sleap_amd.nn.optim import AdamW
+
+    g = rng(37)
+    p = torch.nn.Parameter(normal(g, 70, dtype=torch.float32))
+    theirs = torch.optim.AdamW([p], lr=1e-2, amsgrad=True)
+    for _ in range(3):
+        p.grad = normal(g, 70, dtype=torch.float32)
+        theirs.step()
+    saved = theirs.state_dict()
+    q, *states = (t.detach().clone() for t in (p, *(theirs.state[p][k] for k in ("exp_avg", "exp_avg_sq", "max_exp_avg_sq"))))
+    opt = AdamW([p])
+    opt.load_state_dict(saved)
+    opt.step()
+    assert opt.state[p]["step"] == 4 and isinstance(opt.state[p]["step"], int)
+    ops.adamw_step([q], [p.grad], *([t] for t in states[:2]), max_exp_avg_sqs=states[2:], step=4, lr=1e-2)
+    assert torch.equal(p.detach(), q) and all(torch.equal(opt.state[p][k], t) for k, t in zip(("exp_avg", "exp_avg_sq", "max_exp_avg_sq"), states))
+    for other, what in ((torch.optim.AdamW([p], maximize=True), "maximize"), (torch.optim.Adam([p], weight_decay=0.1), "decoupled")):
+        before = opt.state_dict()["param_groups"]
+        with pytest.raises(ValueError, match=what):
+            opt.load_state_dict(other.state_dict())
+        assert opt.state_dict()["param_groups"] == before
+    opt.load_state_dict(torch.optim.Adam([p]).state_dict())  # without decay both are one
+
+
 def test_the_fitting_commands_step_on_the_gpu():
     """tools/train_benchmark_model.py as it is started, three small steps of it: the fit runs and its losses stay finite."""
     import os
