@@ -751,8 +751,8 @@ int sa_cross_attention(const void* q, const void* k, const void* v, int dtype, i
                        float scale, void* out, float* lse, void* out_low, void* workspace, size_t workspace_bytes, sa_stream_t stream);
 
 /* Gradients of sa_cross_attention from its out, out_low (or NULL) and lse and from dout [B,Tq,Hq,D] (dout_strides: HOST, batch, token, head) ->
- * dq [B,Tq,Hq,D], dk and dv [B,Tk,Hkv,D], contiguous; shared heads are summed; hidden keys and rows that see none get zeros. No
- * atomics: the same call gives the same bits. workspace: sa_cross_attention_backward_workspace bytes. */
+ * dq [B,Tq,Hq,D], dk and dv [B,Tk,Hkv,D], contiguous; shared heads are summed; hidden keys and rows that see none get zeros. dq,
+ * or dk and dv together, may be NULL: not asked for, not computed. No atomics: the same call gives the same bits. workspace: sa_cross_attention_backward_workspace bytes. */
 size_t sa_cross_attention_backward_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D);
 int sa_cross_attention_backward(const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D,
                                 const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, const int64_t* mask_strides,

@@ -248,11 +248,16 @@ Attended attend(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Keys
 }
 
 std::array<Tensor, 3> attend_backward(const Tensor& dout_, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& out, const Tensor& lse,
-                                      const Tensor& low, const Keys& keys) {
+                                      const Tensor& low, const Keys& keys, bool want_q, bool want_kv) {
   const int64_t group = q_.size(2) / k_.size(2);
   const Laid q = laid_out(q_, 8, ROW_SPAN, group), k = laid_out(k_, 8, KEY_SPAN), v = laid_out(v_, 8, KEY_SPAN), dout = laid_out(dout_, 8, ROW_SPAN, group);
   const int B = (int)q.t.size(0), Tq = (int)q.t.size(1), H = (int)q.t.size(2), D = (int)q.t.size(3), Tk = (int)k.t.size(1), K = (int)k.t.size(2);
-  Tensor dq = at::empty({B, Tq, H, D}, q.t.options()), dk = at::empty({B, Tk, K, D}, q.t.options()), dv = at::empty({B, Tk, K, D}, q.t.options());
+  Tensor dq, dk, dv;
+  if (want_q) dq = at::empty({B, Tq, H, D}, q.t.options());
+  if (want_kv) {
+    dk = at::empty({B, Tk, K, D}, q.t.options());
+    dv = at::empty_like(dk);
+  }
   if (B == 0 || (Tq == 0 && Tk == 0)) return {dq, dk, dv};
   const size_t bytes = entry.backward_workspace(B, Tq, Tk, H, K, D);
   const Tensor ws = workspace(bytes, q.t);
@@ -260,8 +265,8 @@ std::array<Tensor, 3> attend_backward(const Tensor& dout_, const Tensor& q_, con
   const auto ms = keys.strides();
   const c10::OptionalDeviceGuard guard(q.t.device());
   check(entry.attention_backward(q.t.data_ptr(), k.t.data_ptr(), v.t.data_ptr(), type_of(q.t), B, Tq, Tk, H, K, D, strides, keys.n(), keys.m(),
-                               ms.data(), keys.scale, out.data_ptr(), low.defined() ? low.data_ptr() : nullptr, lse.data_ptr<float>(), dout.t.data_ptr(), dout.s.data(), dq.data_ptr(),
-                               dk.data_ptr(), dv.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q.t.device())),
+                               ms.data(), keys.scale, out.data_ptr(), low.defined() ? low.data_ptr() : nullptr, lse.data_ptr<float>(), dout.t.data_ptr(), dout.s.data(),
+                               want_q ? dq.data_ptr() : nullptr, want_kv ? dk.data_ptr() : nullptr, want_kv ? dv.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q.t.device())),
         "sa_cross_attention_backward");
   return {dq, dk, dv};
 }
@@ -280,10 +285,12 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     const auto saved = ctx->get_saved_variables();
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     const Keys keys = {saved[6], saved[7], (float)ctx->saved_data["scale"].toDouble()};
-    const auto [dq, dk, dv] = attend_backward(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], keys);
+    const auto [dq, dk, dv] = attend_backward(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], keys,
+                                            ctx->needs_input_grad(0), ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
     variable_list got = {dq, dk, dv};
     if (at::GradMode::is_enabled()) {  // create_graph: a second gradient has to fail, not to miss what these depend on
-      for (auto& t : got) t = t.detach().set_requires_grad(true);
+      for (auto& t : got)
+        if (t.defined()) t = t.detach().set_requires_grad(true);
       got = (*std::make_shared<torch::autograd::DelayedError>("cross_attention has first gradients only", 3))(std::move(got));
     }
     return {got[0], got[1], got[2], Tensor(), Tensor()};

@@ -238,6 +238,23 @@ def test_gradients_of_broadcast_inputs_are_summed():
     assert torch.equal(d, e.sum(0, keepdim=True))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ragged", ["none", "lengths+mask"])
+@pytest.mark.parametrize("B,Tq,Tk,H,K,D", [(2, 1, 64, 2, 2, 16), (3, 31, 700, 4, 2, 40), (1, 1100, 50, 2, 1, 64), (2, 190, 2300, 2, 2, 128), (1, 12, 9000, 1, 1, 72),
+                                           (2, 0, 9, 2, 2, 32), (2, 9, 0, 2, 2, 32)])
+def test_only_the_gradients_asked_for(dtype, ragged, B, Tq, Tk, H, K, D):
+    """A frozen map (q alone), given queries (k, v), and each of the three alone: cut otherwise than all together, as right."""
+    from sleap_amd import ops
+
+    q, k, v, dout, lengths, mask = make(rng(B + Tq * Tk + D), B, Tq, Tk, H, K, D, dtype, ragged)
+    want = oracle.attention(q, k, v, lengths, mask, None, dout)
+    for asked in ("q", "k", "v", "kv", "qv"):
+        inputs = {n: t.detach().requires_grad_(n in asked) for n, t in zip("qkv", (q, k, v))}
+        out = ops.cross_attention(*inputs.values(), key_lengths=lengths, key_mask=mask)
+        for n, x in zip(asked, torch.autograd.grad(out, [inputs[n] for n in asked], dout)):
+            assert x.shape == inputs[n].shape and oracle.worst(x, want["d" + n]) <= 1, (asked, n)
+
+
 def test_gradients_against_differences():
     """The 64-bit loss along a direction, by central differences, against the kernels' gradients along it."""
     from sleap_amd import ops

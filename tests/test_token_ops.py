@@ -87,6 +87,19 @@ def test_attention_entry_points_refuse():
     assert h.sa_cross_attention_workspace(0, 1, 1, 1, 1, 8) == 0 and h.sa_cross_attention_workspace(1, 4, 8, 3, 2, 8) == 0
 
 
+def test_attention_gradients_are_asked_for_in_pairs():
+    h = _lib.lib()
+
+    def call(dq, dk, dv, ws=0):
+        return h.sa_cross_attention_backward(256, 256, 256, 1, 1, 4, 8, 2, 2, 32, i64(*(64, 64, 32) * 3), None, None, None, 1.0, 256, None, 256, 256, i64(64, 64, 32), dq, dk, dv, 256, ws, None)
+
+    refused(call(256, 256, None), "null address")
+    refused(call(None, None, 256), "null address")
+    assert call(None, None, None) == 0  # nothing asked for
+    for asked in ((256, None, None), (None, 256, 256), (256, 256, 256)):
+        refused(call(*asked), "workspace")
+
+
 def test_adamw_entry_point_refuses():
     h = _lib.lib()
     row = i64(256, 256, 256, 256, 0, 10)
