@@ -39,7 +39,9 @@ constexpr float GROW = 8.0f;
 
 // LOW: weights are multiplied in two terms, rounded and what that left, and `low` is written. For gradients over few keys: rowsum(do * out)
 // has to cancel against w^T (do v^T) there, and the roundings of w and out alone made dq and dk over 3 keys 2.2 times as inexact as
-// their own rounding (600 keys: 1.5 times; from 4096 on it no longer shows).
+// their own rounding (600 keys: 1.5 times; from 4096 on it no longer shows). What counts are visible keys: FEW by the length, or the first FEW
+// that a mask leaves (shared out among the runs); further ones are multiplied once.
+constexpr int FEW = 2048;
 template <typename E, int DB, int NW, bool LOW>
 __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p) {
   constexpr int DP = DB == 3 ? 128 : DB * 32, KS = DB * 2;
@@ -93,6 +95,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
   for (int db = 0; db < DB; ++db) ot[db] = T::at_t(lane) ^ (db << 6);
 
   f32x16 o[DB] = {};
+  int few = length <= FEW ? 0x7FFFFFFF : mask ? FEW / (int)p.splits : 0;  // LOW: visible keys still to be multiplied twice
   float m = -INFINITY, l = 0.0f, shift = -Range<E>::LIFT;  // shift = c m - LIFT, of a maximum that is not -inf
   // A tile is copied while the one before is multiplied; the mask's bytes come one tile earlier still. (Three stages: slower by 5 to 15 %
   // at every head size, and workgroups of eight waves gain nothing either.)
@@ -150,15 +153,19 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
     for (int kk = 0; kk < 4; ++kk) {
       const f32x16& s = kk < 2 ? s0 : s1;
       const s16x8 w = pack8<E>(s, kk & 1);
-      s16x8 rest;
-      if constexpr (LOW) rest = pack8_rest<E>(s, kk & 1, w);
+      s16x8 v[DB];
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        const s16x8 v = read_t(vt, ot[db] + kk * 16 * T::ROW, 8 * T::ROW);
-        o[db] = Mfma<E>::run(v, w, o[db]);
-        if constexpr (LOW) o[db] = Mfma<E>::run(v, rest, o[db]);
+        v[db] = read_t(vt, ot[db] + kk * 16 * T::ROW, 8 * T::ROW);
+        o[db] = Mfma<E>::run(v[db], w, o[db]);
+      }
+      if (LOW && few > 0) {
+        const s16x8 rest = pack8_rest<E>(s, kk & 1, w);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] = Mfma<E>::run(v[db], rest, o[db]);
       }
     }
+    if (LOW) few -= __popcll(now);
   }
 
   l = sum_halves(l);

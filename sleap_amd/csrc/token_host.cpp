@@ -221,7 +221,8 @@ Tensor workspace(size_t bytes, const Tensor& like) {  // of one call: the alloca
   return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
-// Up to this many keys a forward pass that is to be differentiated keeps its output in two terms (attention.hip: LOW).
+// Up to this many keys, or where lengths or a mask may leave no more, a forward pass that is to be differentiated keeps its output in two
+// terms (attention.hip: LOW).
 constexpr int64_t FEW_KEYS = 2048;
 
 struct Attended {
@@ -273,7 +274,7 @@ std::array<Tensor, 3> attend_backward(const Tensor& dout_, const Tensor& q_, con
 
 struct CrossAttention : torch::autograd::Function<CrossAttention> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Keys& keys, bool want_lse) {
-    const auto [out, lse, low] = attend(q, k, v, keys, true, k.size(1) <= FEW_KEYS);
+    const auto [out, lse, low] = attend(q, k, v, keys, true, k.size(1) <= FEW_KEYS || keys.lengths.defined() || keys.mask.defined());
     ctx->save_for_backward({q, k, v, out, lse, low, keys.lengths, keys.mask});
     ctx->saved_data["scale"] = (double)keys.scale;
     ctx->set_materialize_grads(false);

@@ -442,7 +442,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, return
     scale        positive; default 1 / sqrt(D)
     return_lse   also the natural logarithm of the softmax's denominators, (B, H, Tq) float32, without a gradient
     A query that sees no key gives zeros (lse: -inf) and passes no gradient. Softmax and sums are float32, weights are rounded to q's
-    type before the product with v (a call that is to be differentiated, over 2048 keys at most, multiplies what the rounding leaves as well:
+    type before the product with v (a call that is to be differentiated, over 2048 visible keys at most, multiplies what the rounding leaves as well:
     its output is the more exact one); results do not depend on the order in which workgroups run. Differentiable in q, k and v, once: queries on a frozen map cost
     their own gradient only, and so do keys and values together."""
     return _token().cross_attention(q, k, v, key_lengths, key_mask, scale, return_lse)
