@@ -72,6 +72,14 @@ struct Range16<_Float16> {
   __device__ __forceinline__ float back() const { return 1.0f / up; }
 };
 
+// TWICE: w and ds are multiplied in two terms, rounded and what that left. Their rounding alone makes gradients 1.41 times as inexact as
+// their own rounding does where sums are long, up to 2.8 times where a few weights make them up, and dq of heads of up to 32 values 1.5 to 1.7
+// times at any size. So dq of such heads is multiplied twice always (2 x 2048 x 4096 x 8 x 16 bf16, both sides: 99 us with neither, 109 with dq,
+// 135 with all three), and all three are where it costs next to nothing: up to FREE multiply-adds a product, 30 us of kernel at most
+// beside the 40 to 75 that torch's engine takes on the host (3 x 417 x 1531 x 8 on 2 x 40 fp16, 0.9 FREE: 25.8 us of kernel, 22.6 without). 4096 x 8192 x 8
+// x 128 bf16 would take 629 us instead of 442.
+constexpr double FREE = 1024.0 * 1024 * 1024;
+
 template <typename E>
 __global__ __launch_bounds__(256) void attention_stats_kernel(const BwdParams p, uint32_t total) {
   const AttnShape& a = p.a;
@@ -127,7 +135,7 @@ __device__ __forceinline__ void copy_rows(char* lds, const Pieces<DP, NW>& at, c
 }
 
 // dk, dv: a wave owns 32 keys (k and v in registers) and walks rows in tiles of 64
-template <typename E, int DB, int NW>
+template <typename E, int DB, int NW, bool TWICE>
 __device__ __forceinline__ void keys_side(const BwdParams& p, uint32_t block, char* lds) {
   constexpr int DP = DB == 3 ? 128 : DB * 32, KS = DB * 2;
   using T = Tile<DP>;
@@ -207,8 +215,14 @@ __device__ __forceinline__ void keys_side(const BwdParams& p, uint32_t block, ch
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const s16x8 w = pack8<E>(s, s2);
+        s16x8 rest;
+        if constexpr (TWICE) rest = pack8_rest<E>(s, s2, w);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) dv[db] = Mfma<E>::run(read_t(dt, (at_ ^ (db << 6)) + s2 * 16 * T::ROW, 8 * T::ROW), w, dv[db]);
+        for (int db = 0; db < DB; ++db) {
+          const s16x8 f = read_t(dt, (at_ ^ (db << 6)) + s2 * 16 * T::ROW, 8 * T::ROW);
+          dv[db] = Mfma<E>::run(f, w, dv[db]);
+          if constexpr (TWICE) dv[db] = Mfma<E>::run(f, rest, dv[db]);
+        }
       }
       if (LATE) multiply_dp();
 #pragma unroll
@@ -221,8 +235,14 @@ __device__ __forceinline__ void keys_side(const BwdParams& p, uint32_t block, ch
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const s16x8 w = pack8<E>(dp, s2);
+        s16x8 rest;
+        if constexpr (TWICE) rest = pack8_rest<E>(dp, s2, w);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) dk[db] = Mfma<E>::run(read_t(qt, (at_ ^ (db << 6)) + s2 * 16 * T::ROW, 8 * T::ROW), w, dk[db]);
+        for (int db = 0; db < DB; ++db) {
+          const s16x8 f = read_t(qt, (at_ ^ (db << 6)) + s2 * 16 * T::ROW, 8 * T::ROW);
+          dk[db] = Mfma<E>::run(f, w, dk[db]);
+          if constexpr (TWICE) dk[db] = Mfma<E>::run(f, rest, dk[db]);
+        }
       }
     }
   }
@@ -249,7 +269,7 @@ __device__ __forceinline__ void keys_side(const BwdParams& p, uint32_t block, ch
 }
 
 // dq: a wave owns 32 rows (q and dout in registers) and walks keys in tiles of 64
-template <typename E, int DB, int NW>
+template <typename E, int DB, int NW, bool TWICE>
 __device__ __forceinline__ void rows_side(const BwdParams& p, uint32_t block, char* lds) {
   constexpr int DP = DB == 3 ? 128 : DB * 32, KS = DB * 2;
   using T = Tile<DP>;
@@ -336,8 +356,14 @@ __device__ __forceinline__ void rows_side(const BwdParams& p, uint32_t block, ch
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const s16x8 w = pack8<E>(dp, s2);
+        s16x8 rest;
+        if constexpr (TWICE) rest = pack8_rest<E>(dp, s2, w);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) dq[db] = Mfma<E>::run(read_t(kt, ot[db] + (blk * 2 + s2) * 16 * T::ROW, 8 * T::ROW), w, dq[db]);
+        for (int db = 0; db < DB; ++db) {
+          const s16x8 f = read_t(kt, ot[db] + (blk * 2 + s2) * 16 * T::ROW, 8 * T::ROW);
+          dq[db] = Mfma<E>::run(f, w, dq[db]);
+          if constexpr (TWICE) dq[db] = Mfma<E>::run(f, rest, dq[db]);
+        }
       }
     }
   }
@@ -355,11 +381,11 @@ __device__ __forceinline__ void rows_side(const BwdParams& p, uint32_t block, ch
 
 // Both sides in one launch: neither needs the other, and one's last workgroups fill up with the other's. Rows come first, their
 // walks are the longer ones where keys are many.
-template <typename E, int DB, int NW>
+template <typename E, int DB, int NW, bool TWICE>
 __global__ __launch_bounds__(NW * 64, 2) void attention_bwd_kernel(const BwdParams p) {
   extern __shared__ __align__(1024) char lds[];
-  if (blockIdx.x < p.rows.blocks) rows_side<E, DB, NW>(p, blockIdx.x, lds);
-  else keys_side<E, DB, NW>(p, blockIdx.x - p.rows.blocks, lds);
+  if (blockIdx.x < p.rows.blocks) rows_side<E, DB, NW, TWICE || DB == 1>(p, blockIdx.x, lds);
+  else keys_side<E, DB, NW, TWICE>(p, blockIdx.x - p.rows.blocks, lds);
 }
 
 // Adds the runs' gradients, in their order, of up to three tensors; a thread has 8 values of one.
@@ -425,16 +451,16 @@ Layout layout(int B, int Tq, int Tk, int Hq, int Hkv, int D, bool want_q, bool w
   return l;
 }
 
-template <typename E, int DB>
+template <typename E, int DB, bool TWICE>
 void launch_sides(const BwdParams& p, int waves, hipStream_t s) {
   constexpr size_t lds = 2 * (2 * Tile<DB == 3 ? 128 : DB * 32>::BYTES + 2 * TILE * 4);  // the keys' side, which has the rows' numbers beside its tiles
   auto go = [&](auto kernel) {
     if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     kernel<<<dim3(p.rows.blocks + p.kv.blocks), dim3(waves * 64), lds, s>>>(p);
   };
-  if (waves == 1) go(attention_bwd_kernel<E, DB, 1>);
-  else if (waves == 2) go(attention_bwd_kernel<E, DB, 2>);
-  else go(attention_bwd_kernel<E, DB, 4>);
+  if (waves == 1) go(attention_bwd_kernel<E, DB, 1, TWICE>);
+  else if (waves == 2) go(attention_bwd_kernel<E, DB, 2, TWICE>);
+  else go(attention_bwd_kernel<E, DB, 4, TWICE>);
 }
 
 template <typename E>
@@ -447,10 +473,14 @@ int launch(const BwdParams& p, int waves, hipStream_t s) {
     SA_LAUNCH_CHECK();
   }
   if (p.rows.blocks + p.kv.blocks == 0) return SA_OK;
-  if (db == 1) launch_sides<E, 1>(p, waves, s);
-  else if (db == 2) launch_sides<E, 2>(p, waves, s);
-  else if (db == 3) launch_sides<E, 3>(p, waves, s);
-  else launch_sides<E, 4>(p, waves, s);
+  auto sides = [&](auto twice) {
+    if (db == 1) launch_sides<E, 1, twice>(p, waves, s);
+    else if (db == 2) launch_sides<E, 2, twice>(p, waves, s);
+    else if (db == 3) launch_sides<E, 3, twice>(p, waves, s);
+    else launch_sides<E, 4, twice>(p, waves, s);
+  };
+  if ((double)p.heads * a.R * a.Tk * (db * 32) <= FREE) sides(std::true_type{});
+  else sides(std::false_type{});
   SA_LAUNCH_CHECK();
   AddParams add = {};
   uint32_t blocks = 0;

@@ -284,6 +284,26 @@ def test_few_visible_keys_of_many(dtype, by, n):
         assert e <= 1.2 * alone
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ragged", ["none", "lengths+mask"])
+@pytest.mark.parametrize("B,Tq,Tk,H,K,D", [(3, 1, 11, 2, 1, 48), (2, 18, 2, 1, 1, 72), (5, 2, 282, 8, 8, 16), (1, 300, 900, 4, 2, 128), (3, 400, 1500, 4, 2, 40), (4, 2000, 2000, 4, 4, 16)])
+def test_gradients_as_exact_as_their_type(dtype, ragged, B, Tq, Tk, H, K, D):
+    """Over up to 2048 keys, weights of the gradients multiplied in two terms (dq alone in the last of the sizes): what is left are terms of
+    2^-16 (bf16) and 2^-22 (fp16) beside the gradients' own rounding of 2^-8 and 2^-11, a tenth of it in the norm at most, and the float32
+    sums of dw and delta: a row that sees one key has dw = delta, dq = 0, and both sums are off by D 2^-24 of their terms."""
+    from sleap_amd import ops
+
+    q, k, v, dout, lengths, mask = make(rng(B + Tq * Tk + D), B, Tq, Tk, H, K, D, dtype, ragged, scale=1.5)
+    want = oracle.attention(q, k, v, lengths, mask, None, dout)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask), leaves, dout)
+    for name, x in zip(("dq", "dk", "dv"), grads):
+        if name == "dq" or Tq < 2000:
+            w = want[name][0]
+            sums = {"dq": want["sums"][0], "dk": want["sums"][1], "dv": torch.zeros(1)}[name]
+            assert (x.double() - w).norm() <= 1.1 * (w.to(dtype).double() - w).norm() + 1e-6 * w.norm() + sums.norm().item(), name
+
+
 def test_gradients_against_differences():
     """The 64-bit loss along a direction, by central differences, against the kernels' gradients along it."""
     from sleap_amd import ops

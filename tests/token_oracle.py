@@ -19,7 +19,7 @@ def visible(B, Tk, lengths, mask, device="cpu"):
 
 
 def attention(q, k, v, lengths=None, mask=None, scale=None, dout=None):
-    """-> dict of (value, allowance) pairs: out, lse and with dout dq, dk, dv; tensors as the operator takes them"""
+    """-> dict of (value, allowance) pairs: out, lse and with dout dq, dk, dv (and "sums": two parts of allowances); tensors as the operator takes them"""
     B, Tq, H, D = q.shape
     Tk, K = k.shape[1:3]
     G, u, tiny, dtype = H // K, UNIT[q.dtype], TINY[q.dtype], torch.float64
@@ -67,6 +67,8 @@ def attention(q, k, v, lengths=None, mask=None, scale=None, dout=None):
             e_dq = e_dq + 2.0 ** -37 * ds.abs().amax(-1, keepdim=True) * k_.abs().sum(2, keepdim=True) * scale
         for name, x, e in (("dq", dq, e_dq), ("dk", dk, e_dk), ("dv", dv, e_dv)):
             got[name] = (x, e + u * (x.abs() + e) + tiny)
+        # of the allowances of dq and dk, what the float32 sums in dw - delta alone make: all that is left where one key has the whole weight
+        got["sums"] = ((w * e_dw) @ k_.abs() * scale, share((w * e_dw).transpose(2, 3).contiguous() @ q_.abs()) * scale)
     return {n: (a.transpose(1, 2), b.transpose(1, 2)) if a.dim() == 4 else (a, b) for n, (a, b) in got.items()}
 
 
