@@ -509,6 +509,28 @@ def test_a_capture_on_top_of_a_living_graph_is_refused():
         ops.cross_attention(leaf * 3, k, v)  # built in the capture altogether
 
 
+def test_a_capture_over_two_streams():
+    """What an input hangs on may come from another stream of the same capture."""
+    from sleap_amd import ops
+
+    q, k, v, _, _, _ = make(rng(39), 1, 4, 6, 1, 1, 16, torch.float16)
+    leaf, side, graph = q.detach().requires_grad_(True), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    want = ops.cross_attention(q * 3, k, v)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            thrice = leaf * 3
+        torch.cuda.current_stream().wait_stream(side)
+        out = ops.cross_attention(thrice, k, v).detach()
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        # weights in one term (off by 2^-11 of v at most) and in two, both results rounded (2^-11 each)
+        assert (out.float() - want.float()).abs().max() <= 2.0 ** -11 * (v.float().abs().max() + 2 * want.float().abs().max()) * 1.01
+
+
 def test_two_calls_at_once_on_two_streams():
     """Calls with scratch, from two threads on streams of their own, do not meet."""
     import threading
