@@ -6,7 +6,8 @@
 // a head two workgroups a CU overlap one's products with the other's exponentials: 2 x 8 heads x 4096 x 16384 bf16 in 530 us = 1.04
 // PFLOP/s (a library product of 8192^3: 1.19), matrix pipes busy 0.53 of the time at the 1.85 GHz that the chip holds under that load. At 64
 // values the vector units are the limit (32 exponentials of 16 cycles a tile and lane beside 512 cycles of products): 0.70 to 0.77
-// PFLOP/s. Where rows are few the keys are cut into runs: 32 single tokens on 16384 keys x 2 heads x 128 read theirs at 4.7 TB/s.
+// PFLOP/s. Where rows are few, waves share the keys (52 queries x 8 heads x 32 on 1024 keys: 6.1 us) or the keys are cut
+// into runs: 32 single tokens on 16384 keys x 2 heads x 128 read theirs at 4.7 TB/s.
 #include "attention.h"
 
 namespace {
@@ -42,13 +43,19 @@ constexpr float GROW = 8.0f;
 // their own rounding (600 keys: 1.5 times; from 4096 on it no longer shows). What counts are visible keys: FEW by the length, or the first FEW
 // that a mask leaves (shared out among the runs); further ones are multiplied once.
 constexpr int FEW = 2048;
-template <typename E, int DB, int NW, bool LOW>
-__global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p) {
+//
+// KW: waves along the keys, each with the same 32 rows, a run of keys and tiles of its own, so that they need no barrier before their sums meet
+// in LDS: for few rows on few keys, where a second launch would join the runs otherwise.
+template <typename E, int DB, int NW, bool LOW, int KW>
+__global__ __launch_bounds__(NW * KW * 64, 2) void attention_kernel(const FwdParams p) {
+  static_assert(NW == 1 || KW == 1, "");
   constexpr int DP = DB == 3 ? 128 : DB * 32, KS = DB * 2;
   using T = Tile<DP>;
-  extern __shared__ __align__(1024) char lds[];  // [2 stages][k tile, v tile]
+  extern __shared__ __align__(1024) char lds_all[];  // [KW][2 stages][k tile, v tile]
   const AttnShape& a = p.a;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+  const int id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = KW > 1 ? 0 : id, part = KW > 1 ? id : 0;
+  const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+  char* lds = lds_all + part * 4 * T::BYTES;
   const Piece piece = piece_of(blockIdx.x, p.heads, p.row_tiles * p.splits, p.div_pieces);
   const uint32_t bh = piece.head, split = div_by(piece.at, p.div_tiles), tile = piece.at - split * p.row_tiles;
   const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv;
@@ -67,7 +74,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
   }
   int length = a.Tk;
   if (a.lengths) length = min(max(a.lengths[b], 0), a.Tk);
-  const int first = (int)split * p.split_keys, end = min(first + p.split_keys, length);
+  const int first = (int)(split * KW + part) * p.split_keys, end = min(first + p.split_keys, length);
   const int tiles = end > first ? (end - first + TILE - 1) / TILE : 0;
   const E* kbase = static_cast<const E*>(a.k) + (int64_t)b * a.kb + (int64_t)hk * a.kh;
   const E* vbase = static_cast<const E*>(a.v) + (int64_t)b * a.vb + (int64_t)hk * a.vh;
@@ -95,7 +102,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
   for (int db = 0; db < DB; ++db) ot[db] = T::at_t(lane) ^ (db << 6);
 
   f32x16 o[DB] = {};
-  int few = length <= FEW ? 0x7FFFFFFF : mask ? FEW / (int)p.splits : 0;  // LOW: visible keys still to be multiplied twice
+  int few = length <= FEW ? 0x7FFFFFFF : mask ? FEW / (int)(p.splits * KW) : 0;  // LOW: visible keys still to be multiplied twice
   float m = -INFINITY, l = 0.0f, shift = -Range<E>::LIFT;  // shift = c m - LIFT, of a maximum that is not -inf
   // A tile is copied while the one before is multiplied; the mask's bytes come one tile earlier still. (Three stages: slower by 5 to 15 %
   // at every head size, and workgroups of eight waves gain nothing either.)
@@ -107,7 +114,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
     next_mask = load_mask(1);
   }
   for (int i = 0; i < tiles; ++i) {
-    tile_barrier();
+    if constexpr (KW > 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the tiles are this wave's alone
+    else tile_barrier();
     const uint64_t now = seen;
     if (i + 1 < tiles) {
       seen = seen_of(i + 1, next_mask);
@@ -169,6 +177,46 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
   }
 
   l = sum_halves(l);
+  if constexpr (KW > 1) {
+    constexpr int STATS = DB * 4 * 1024;
+    if (part) {
+#pragma unroll
+      for (int j = 0; j < DB * 4; ++j)
+        *reinterpret_cast<f32x4*>(lds + (j * 64 + lane) * 16) = f32x4{o[j >> 2][4 * (j & 3)], o[j >> 2][4 * (j & 3) + 1], o[j >> 2][4 * (j & 3) + 2], o[j >> 2][4 * (j & 3) + 3]};
+      reinterpret_cast<float*>(lds + STATS)[lane] = shift;
+      reinterpret_cast<float*>(lds + STATS)[64 + lane] = l;
+    }
+    __syncthreads();
+    if (part) return;
+    float shifts[KW], sums[KW], top = l == 0.0f ? -INFINITY : shift;
+    shifts[0] = shift;
+    sums[0] = l;
+#pragma unroll
+    for (int w = 1; w < KW; ++w) {
+      const float* stats = reinterpret_cast<const float*>(lds + w * 4 * T::BYTES + STATS);
+      shifts[w] = stats[lane];
+      sums[w] = stats[64 + lane];
+      top = fmaxf(top, sums[w] == 0.0f ? -INFINITY : shifts[w]);
+    }
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      const float by = sums[w] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(shifts[w] - top);  // a run without a visible key: nothing
+      l += sums[w] * by;
+#pragma unroll
+      for (int j = 0; j < DB * 4; ++j) {
+        if (w == 0) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[j >> 2][4 * (j & 3) + e] *= by;
+        } else {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(lds + w * 4 * T::BYTES + (j * 64 + lane) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[j >> 2][4 * (j & 3) + e] += x[e] * by;
+        }
+      }
+    }
+    shift = top;
+  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   if (p.splits > 1) {
     if (!real) return;
@@ -178,7 +226,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const FwdParams p
     return;
   }
   if (p.lse && real && h == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = l == 0.0f ? -INFINITY : (shift + __log2f(l)) * LN2;
-  tile_barrier();  // the last tile has been read
+  if constexpr (KW == 1) tile_barrier();  // the last tile has been read
   auto row_of = [&](void* base) {
     return [=](int i) -> E* {
       const uint32_t r = row - n + i, t = div_by(r, a.div_g), g = r - t * a.G;
@@ -266,9 +314,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const FwdParams p, 
   *reinterpret_cast<u32x4*>(static_cast<E*>(p.low) + at) = u32x4{pack2<E>(acc[0], acc[1]), pack2<E>(acc[2], acc[3]), pack2<E>(acc[4], acc[5]), pack2<E>(acc[6], acc[7])};
 }
 
-// How a call is cut: waves of a workgroup (32 rows each) and runs of keys.
+// How a call is cut: waves of a workgroup (32 rows each, or along the keys) and runs of keys.
 struct Cut {
-  int waves;
+  int waves, key_waves;
   uint32_t row_tiles, splits;
   int split_keys;
 };
@@ -298,6 +346,23 @@ Cut cut(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
       }
     }
   }
+  // Few rows on few keys: four waves of a workgroup along the keys and one launch, as long as every workgroup has a place (64 KB of
+  // tiles at up to 32 values a head, 128 KB above) and the longer runs cost less than a second launch and the runs' results, written
+  // and read: in microseconds, a tile of a lone wave 0.45 + 0.01 D, 1.5 for the launch, 4 bytes a value twice at 4 TB/s. (52 queries x 8 heads x 32 on
+  // 640 keys: 5.3 us, 8.5 in two launches; on 1024: 6.1 and 7.9; on 2048, in two launches: 8.4, 9.0 in one. 2 x 416 x 8 x 32 on 1536: 7.8 and 13.1.)
+  c.key_waves = 1;
+  const uint64_t narrow = (R + 31) / 32 * B * Hkv, along = (key_tiles + 3) / 4;
+  if (key_tiles >= 3 && D <= 64 && narrow <= (D <= 32 ? 512 : 256)) {
+    const double longer = (double)along - (double)((key_tiles + splits - 1) / splits);
+    if (splits == 1 || longer * (0.45 + 0.01 * D) <= 1.5 + (double)splits * R * B * Hkv * D * 8 / 4e6) {
+      c.waves = 1;
+      c.key_waves = 4;
+      c.row_tiles = (uint32_t)((R + 31) / 32);
+      c.splits = 1;
+      c.split_keys = (int)along * TILE;
+      return c;
+    }
+  }
   const uint32_t per = key_tiles ? (uint32_t)((key_tiles + splits - 1) / splits) : 1;
   c.split_keys = (int)per * TILE;
   c.splits = key_tiles ? (key_tiles + per - 1) / per : 1;
@@ -305,26 +370,34 @@ Cut cut(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
 }
 
 template <typename E, int DB, bool LOW>
-void launch_low(const FwdParams& p, int waves, hipStream_t s) {
+void launch_low(const FwdParams& p, const Cut& c, hipStream_t s) {
   constexpr size_t lds = 4 * Tile<DB == 3 ? 128 : DB * 32>::BYTES;
-  if (waves == 1) attention_kernel<E, DB, 1, LOW><<<dim3(p.blocks), dim3(64), lds, s>>>(p);
-  else if (waves == 2) attention_kernel<E, DB, 2, LOW><<<dim3(p.blocks), dim3(128), lds, s>>>(p);
-  else attention_kernel<E, DB, 4, LOW><<<dim3(p.blocks), dim3(256), lds, s>>>(p);
+  if constexpr (DB <= 2) {
+    if (c.key_waves > 1) {
+      const auto kernel = attention_kernel<E, DB, 1, LOW, 4>;
+      if (4 * lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)(4 * lds));
+      kernel<<<dim3(p.blocks), dim3(256), 4 * lds, s>>>(p);
+      return;
+    }
+  }
+  if (c.waves == 1) attention_kernel<E, DB, 1, LOW, 1><<<dim3(p.blocks), dim3(64), lds, s>>>(p);
+  else if (c.waves == 2) attention_kernel<E, DB, 2, LOW, 1><<<dim3(p.blocks), dim3(128), lds, s>>>(p);
+  else attention_kernel<E, DB, 4, LOW, 1><<<dim3(p.blocks), dim3(256), lds, s>>>(p);
 }
 
 template <typename E, int DB>
-void launch(const FwdParams& p, int waves, hipStream_t s) {
-  if (p.low) launch_low<E, DB, true>(p, waves, s);
-  else launch_low<E, DB, false>(p, waves, s);
+void launch(const FwdParams& p, const Cut& c, hipStream_t s) {
+  if (p.low) launch_low<E, DB, true>(p, c, s);
+  else launch_low<E, DB, false>(p, c, s);
 }
 
 template <typename E>
-void launch_e(const FwdParams& p, int waves, hipStream_t s) {
+void launch_e(const FwdParams& p, const Cut& c, hipStream_t s) {
   const int db = (p.a.D + 31) / 32;
-  if (db == 1) launch<E, 1>(p, waves, s);
-  else if (db == 2) launch<E, 2>(p, waves, s);
-  else if (db == 3) launch<E, 3>(p, waves, s);
-  else launch<E, 4>(p, waves, s);
+  if (db == 1) launch<E, 1>(p, c, s);
+  else if (db == 2) launch<E, 2>(p, c, s);
+  else if (db == 3) launch<E, 3>(p, c, s);
+  else launch<E, 4>(p, c, s);
   if (p.splits > 1) {
     const uint32_t rows = p.heads * p.a.R;
     uint32_t log2 = 0;
@@ -408,8 +481,8 @@ extern "C" int sa_cross_attention(const void* q, const void* k, const void* v, i
   p.heads = (uint32_t)B * Hkv;
   p.div_pieces = fast_div(c.row_tiles * c.splits);
   p.div_heads = fast_div(Hkv);
-  if (dtype == SA_F16) launch_e<_Float16>(p, c.waves, (hipStream_t)stream);
-  else launch_e<__bf16>(p, c.waves, (hipStream_t)stream);
+  if (dtype == SA_F16) launch_e<_Float16>(p, c, (hipStream_t)stream);
+  else launch_e<__bf16>(p, c, (hipStream_t)stream);
   SA_LAUNCH_CHECK();
   return SA_OK;
 }

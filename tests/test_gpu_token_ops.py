@@ -186,6 +186,26 @@ def test_attention_of_many_tiles(dtype, B, Tq, Tk, H, K, D):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ragged", ["none", "lengths+mask"])
+@pytest.mark.parametrize("B,Tq,Tk,H,K,D", [(1, 52, 1024, 8, 8, 32), (3, 33, 129, 2, 1, 8), (3, 20, 192, 4, 4, 64), (2, 1, 193, 2, 2, 40), (1, 800, 1537, 8, 8, 64), (3, 410, 1500, 8, 8, 32),
+                                           (16, 500, 320, 1, 1, 32), (16, 513, 320, 1, 1, 32), (8, 1000, 500, 1, 1, 48), (8, 1025, 500, 1, 1, 48)])
+def test_attention_of_waves_along_the_keys(dtype, ragged, B, Tq, Tk, H, K, D):
+    """Few rows on few keys, four waves a workgroup along the keys: waves whose run is short, empty or hidden, and the last sizes that are cut so."""
+    check(*make(rng(B + Tq * Tk + D), B, Tq, Tk, H, K, D, dtype, ragged))
+
+
+def test_waves_whose_keys_are_hidden():
+    """Of four runs of 128 keys, each alone visible, and each alone hidden."""
+    q, k, v, dout, _, _ = make(rng(40), 1, 40, 512, 2, 2, 32, torch.float16)
+    for run in range(4):
+        mask = torch.zeros((1, 512), dtype=torch.bool, device=DEV)
+        mask[:, 128 * run:128 * run + 128] = True
+        for seen in (mask, ~mask):
+            hidden = ~seen[:, :, None, None]
+            check(q, k.masked_fill(hidden, float("nan")), v.masked_fill(hidden, float("inf")), dout, None, seen)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("spread", [0.0, 8.0, 40.0])
 def test_attention_of_flat_and_of_steep_scores(dtype, spread):
     """From uniform weights to a weight of one; the largest score comes first, last and in the middle of the keys."""
