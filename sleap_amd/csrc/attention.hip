@@ -43,7 +43,7 @@ constexpr float GROW = 8.0f;
 // their own rounding (600 keys: 1.5 times; from 4096 on it no longer shows). What counts are visible keys: FEW by the length, or the first FEW
 // that a mask leaves (shared out among the runs); further ones are multiplied once.
 constexpr int FEW = 2048;
-//
+
 // KW: waves along the keys, each with the same 32 rows, a run of keys and tiles of its own, so that they need no barrier before their sums meet
 // in LDS: for few rows on few keys, where a second launch would join the runs otherwise.
 template <typename E, int DB, int NW, bool LOW, int KW>
