@@ -40,9 +40,8 @@ SOURCES = [
     ("network.hip", []),
     # token operators
     ("rotary.hip", []),
-    # -fno-honor-nans: a maximum is one instruction (else each carries two that quiet signalling NaNs); NaNs still pass the arithmetic
-    ("attention.hip", ["-fno-honor-nans"]),
-    ("attention_bwd.hip", ["-fno-honor-nans"]),
+    ("attention.hip", []),
+    ("attention_bwd.hip", []),
     ("adamw.hip", []),
 ]
 # No packed float32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results now and then on this chip. Same

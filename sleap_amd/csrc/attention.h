@@ -82,11 +82,15 @@ __device__ __forceinline__ s16x8 pack8_rest(const f32x16& c, int s, s16x8 rounde
   return pack8<E>(x, 0);
 }
 
+// The larger of two, NaN if one of them is: v_maximum3_f32, two of them in one instruction. (fmaxf would need another for each operand that
+// an arithmetic instruction did not write, to quiet a signalling NaN.)
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // the two half-waves' values of the same column
 __device__ __forceinline__ float max_halves(float v) {
   const uint32_t u = __float_as_uint(v);
   const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  return larger(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float sum_halves(float v) {
   const uint32_t u = __float_as_uint(v);

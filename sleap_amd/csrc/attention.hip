@@ -135,12 +135,12 @@ __global__ __launch_bounds__(NW * KW * 64, 2) void attention_kernel(const FwdPar
       hide(s0, (uint32_t)now, h);
       hide(s1, (uint32_t)(now >> 32), h);
     }
-    float top = fmaxf(s0[0], s1[0]);
+    float top = larger(s0[0], s1[0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, s0[i]), s1[i]);
+    for (int i = 1; i < 16; ++i) top = larger(larger(top, s0[i]), s1[i]);
     top = max_halves(top);
     if (__any((top - m) * a.c > GROW)) {
-      const float grown = fmaxf(m, top), at = grown == -INFINITY ? 0.0f : grown;
+      const float grown = larger(m, top), at = grown == -INFINITY ? 0.0f : grown;
       const float keep = __builtin_amdgcn_exp2f((m - at) * a.c);
       m = grown;
       shift = at * a.c - Range<E>::LIFT;
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(NW * KW * 64, 2) void attention_kernel(const FwdPar
       const float* stats = reinterpret_cast<const float*>(lds + w * 4 * T::BYTES + STATS);
       shifts[w] = stats[lane];
       sums[w] = stats[64 + lane];
-      top = fmaxf(top, sums[w] == 0.0f ? -INFINITY : shifts[w]);
+      top = larger(top, sums[w] == 0.0f ? -INFINITY : shifts[w]);
     }
     l = 0.0f;
 #pragma unroll
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const FwdParams p, 
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (s0 + k * groups >= p.splits || l[k] == -INFINITY) continue;  // a run without a visible key
-      const float top = fmaxf(m, l[k]), keep = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(l[k] - top);
+      const float top = larger(m, l[k]), keep = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(l[k] - top);
       m = top;
       sum = sum * keep + w;
 #pragma unroll
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const FwdParams p, 
     if (group) return;
     for (uint32_t g = 1; g < groups; ++g) {
       const float* other = sums[threadIdx.x + 16 * g];
-      const float top = fmaxf(m, other[0]);
+      const float top = larger(m, other[0]);
       if (other[1] == 0.0f) continue;
       const float keep = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(other[0] - top);
       m = top;

@@ -58,7 +58,7 @@ struct Range16<_Float16> {
   __device__ __forceinline__ void follow(f32x16& ds, f32x16* acc, int n) {
     float top = fabsf(ds[0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, fabsf(ds[i]));
+    for (int i = 1; i < 16; ++i) top = larger(top, fabsf(ds[i]));
     top = max_halves(top);
     if (__any(top * up > 0x1p15f)) {
       const int e = __builtin_amdgcn_frexp_expf(top);  // top < 2^e

@@ -585,6 +585,44 @@ def test_two_calls_at_once_on_two_streams():
     assert not bad
 
 
+NAN_SHAPES = [(2, 40, 100, 4, 2, 32), (1, 52, 1024, 2, 2, 32), (1, 3, 9000, 2, 2, 64), (2, 300, 900, 2, 1, 128)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", NAN_SHAPES)
+def test_a_nan_goes_where_it_is_used(dtype, shape):
+    """In q: its row, and through it the keys of its head; in a visible key: all rows of its heads; in a value: its place in them; in dout: its
+    row's dq and its head's keys. Workgroups along rows, along keys, and runs that are joined."""
+    from sleap_amd import ops
+
+    B, Tq, Tk, H, K, D = shape
+    G = H // K
+    for what in ("q", "k", "v", "dout"):
+        q, k, v, dout, _, _ = make(rng(49), *shape, dtype)
+        t = {"q": q, "k": k, "v": v, "dout": dout}[what]
+        at = (B - 1, t.shape[1] - 2, t.shape[2] - 1, 5)
+        t[at] = float("nan")
+        leaves = [x.requires_grad_(True) for x in (q, k, v)]
+        out, lse = ops.cross_attention(*leaves, return_lse=True)
+        dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+        plain = ops.cross_attention(*(x.detach() for x in leaves))
+        want = {n: torch.zeros_like(x, dtype=torch.bool) for n, x in (("out", out), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv))}
+        b, row, h, d = at
+        heads = slice(h * G, h * G + G) if what in "kv" else h
+        key = h if what in "kv" else h // G
+        if what == "q":
+            want["out"][b, row, h], want["lse"][b, h, row], want["dq"][b, row, h], want["dk"][b, :, key], want["dv"][b, :, key] = (True,) * 5
+        if what == "k":
+            want["out"][b, :, heads], want["lse"][b, heads], want["dq"][b, :, heads], want["dk"][b, :, key], want["dv"][b, :, key] = (True,) * 5
+        if what == "v":
+            want["out"][b, :, heads, d], want["dq"][b, :, heads], want["dk"][b, :, key] = (True,) * 3
+        if what == "dout":
+            want["dq"][b, row, h], want["dk"][b, :, key], want["dv"][b, :, key, d] = (True,) * 3
+        for n, x in (("out", out), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
+            assert torch.equal(torch.isnan(x), want[n]), (what, n)
+        assert torch.equal(torch.isnan(plain), want["out"]), what
+
+
 # --------------------------------------------------------------------------------------------------
 # AdamW
 # --------------------------------------------------------------------------------------------------
