@@ -740,7 +740,7 @@ int sa_rotary_axes(const void* x, int dtype, int B, int T, int H, int D, const i
  *   key_lengths  [B] or NULL: keys j >= key_lengths[b] are hidden (values outside 0 .. Tk count as the nearer of the two)
  *   key_mask     [B,Tk] bytes or NULL, 0 hides a key (mask_strides: HOST, batch, token); what hidden keys and values hold is not read
  *                into a result, NaN and infinities included
- *   out          [B,Tq,Hq,D] contiguous; zeros where no key is visible
+ *   out          [B,Tq,Hq,D] contiguous; zeros where no key is visible; NaN (lse too) where all visible ones score -inf
  *   lse          [B,Hq,Tq] natural logarithm of the softmax's denominator (-inf where no key is visible), or NULL
  *   out_low      like out: out + out_low is the result with about twice the bits of its type (for the gradients of few keys; half as many
  *                products again; over more than 2048 visible keys the weights are multiplied in one term only), or NULL

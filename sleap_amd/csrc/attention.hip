@@ -38,6 +38,16 @@ struct Range<_Float16> {
 };
 constexpr float GROW = 8.0f;
 
+// A sum of zero has two causes: no visible key (the row is zeros), or visible keys that all score -inf (it is NaN: their softmax is
+// undefined). The logarithm of the first is -inf and of the second the lowest finite number, which no run of a finite score goes below.
+constexpr float LOWEST = -3.4028234663852886e38f;
+__device__ __forceinline__ float of_sum(float sum, float log, float value) {
+  return sum != 0.0f ? value : log == LOWEST ? __builtin_nanf("") : 0.0f;
+}
+__device__ __forceinline__ float lse_of_sum(float sum, float log) {
+  return sum != 0.0f ? (log + __log2f(sum)) * LN2 : log == LOWEST ? __builtin_nanf("") : -INFINITY;
+}
+
 // LOW: weights are multiplied in two terms, rounded and what that left, and `low` is written. For gradients over few keys: rowsum(do * out)
 // has to cancel against w^T (do v^T) there, and the roundings of w and out alone made dq and dk over 3 keys 2.2 times as inexact as
 // their own rounding (600 keys: 1.5 times; from 4096 on it no longer shows). What counts are visible keys: FEW by the length, or the first FEW
@@ -106,7 +116,7 @@ __global__ __launch_bounds__(NW * KW * 64, 2) void attention_kernel(const FwdPar
   float m = -INFINITY, l = 0.0f, shift = -Range<E>::LIFT;  // shift = c m - LIFT, of a maximum that is not -inf
   // A tile is copied while the one before is multiplied; the mask's bytes come one tile earlier still. (Three stages: slower by 5 to 15 %
   // at every head size, and workgroups of eight waves gain nothing either.)
-  uint64_t seen = 0;
+  uint64_t seen = 0, any = 0;
   uint8_t next_mask = 1;
   if (tiles) {
     seen = seen_of(0, load_mask(0));
@@ -123,6 +133,7 @@ __global__ __launch_bounds__(NW * KW * 64, 2) void attention_kernel(const FwdPar
       next_mask = load_mask(i + 2);
     }
     if (now == 0) continue;
+    any |= now;
     const char* kt = lds + (i & 1) * 2 * T::BYTES;
     const char* vt = kt + T::BYTES;
     f32x16 s0 = {}, s1 = {};
@@ -177,6 +188,7 @@ __global__ __launch_bounds__(NW * KW * 64, 2) void attention_kernel(const FwdPar
   }
 
   l = sum_halves(l);
+  if (l == 0.0f) shift = any ? LOWEST : -INFINITY;
   if constexpr (KW > 1) {
     constexpr int STATS = DB * 4 * 1024;
     if (part) {
@@ -188,7 +200,7 @@ __global__ __launch_bounds__(NW * KW * 64, 2) void attention_kernel(const FwdPar
     }
     __syncthreads();
     if (part) return;
-    float shifts[KW], sums[KW], top = l == 0.0f ? -INFINITY : shift;
+    float shifts[KW], sums[KW], top = shift;
     shifts[0] = shift;
     sums[0] = l;
 #pragma unroll
@@ -196,12 +208,12 @@ __global__ __launch_bounds__(NW * KW * 64, 2) void attention_kernel(const FwdPar
       const float* stats = reinterpret_cast<const float*>(lds + w * 4 * T::BYTES + STATS);
       shifts[w] = stats[lane];
       sums[w] = stats[64 + lane];
-      top = larger(top, sums[w] == 0.0f ? -INFINITY : shifts[w]);
+      top = larger(top, shifts[w]);
     }
     l = 0.0f;
 #pragma unroll
     for (int w = 0; w < KW; ++w) {
-      const float by = sums[w] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(shifts[w] - top);  // a run without a visible key: nothing
+      const float by = sums[w] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(shifts[w] - top);  // a run without weight: nothing
       l += sums[w] * by;
 #pragma unroll
       for (int j = 0; j < DB * 4; ++j) {
@@ -217,15 +229,15 @@ __global__ __launch_bounds__(NW * KW * 64, 2) void attention_kernel(const FwdPar
     }
     shift = top;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   if (p.splits > 1) {
     if (!real) return;
     const int64_t at = ((int64_t)bh * p.splits + split) * a.R + row;
-    if (h == 0) p.part_lse[at] = l == 0.0f ? -INFINITY : shift + __log2f(l);
-    store_part(p.part + at * a.D, o, a.D, h, inv);
+    if (h == 0) p.part_lse[at] = l == 0.0f ? shift : shift + __log2f(l);
+    store_part(p.part + at * a.D, o, a.D, h, l == 0.0f ? 0.0f : 1.0f / l);
     return;
   }
-  if (p.lse && real && h == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = l == 0.0f ? -INFINITY : (shift + __log2f(l)) * LN2;
+  const float inv = of_sum(l, shift, 1.0f / l);
+  if (p.lse && real && h == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = lse_of_sum(l, shift);
   if constexpr (KW == 1) tile_barrier();  // the last tile has been read
   auto row_of = [&](void* base) {
     return [=](int i) -> E* {
@@ -302,8 +314,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const FwdParams p, 
   }
   if (!real) return;
   const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv, t = div_by(row, a.div_g), g = row - t * a.G;
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (p.lse && d == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = sum == 0.0f ? -INFINITY : (m + __log2f(sum)) * LN2;
+  if (m == LOWEST) sum = 0.0f;
+  const float inv = of_sum(sum, m, 1.0f / sum);
+  if (p.lse && d == 0) p.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Tq + t] = lse_of_sum(sum, m);
   const int64_t at = (((int64_t)b * a.Tq + t) * a.Hq + hk * a.G + g) * a.D + d;
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] *= inv;

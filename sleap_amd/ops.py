@@ -438,8 +438,9 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, return
     q            (B, Tq, H, D) float16 or bfloat16; D a multiple of 8, at most 128; any strides (unaligned ones cost a copy)
     k, v         (B, Tk, K, D) of q's type; H a multiple of K: head h reads key head h // (H // K)
     key_lengths  (B,) int32 / int64: keys from key_lengths[b] on are hidden (padding)
-    key_mask     (B, Tk) or (1, Tk) bool: False hides a key. What hidden keys and values hold (NaN, infinities) reaches no result;
-                 an infinity in a visible one comes out as infinity or NaN
+    key_mask     (B, Tk) or (1, Tk) bool: False hides a key. What hidden keys and values hold (NaN, infinities) reaches no result.
+                 What visible ones hold does as in the formula: a NaN makes all NaN that it is part of, an infinite value infinity or
+                 NaN, a score of infinity (or beyond float32) NaN; one of -infinity has no weight, and a query all of whose scores are is NaN
     scale        positive; default 1 / sqrt(D)
     return_lse   also the natural logarithm of the softmax's denominators, (B, H, Tq) float32, without a gradient
     A query that sees no key gives zeros (lse: -inf) and passes no gradient. Softmax and sums are float32, weights are rounded to q's

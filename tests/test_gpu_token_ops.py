@@ -623,6 +623,35 @@ def test_a_nan_goes_where_it_is_used(dtype, shape):
         assert torch.equal(torch.isnan(plain), want["out"]), what
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", NAN_SHAPES)
+def test_scores_of_minus_infinity(dtype, shape):
+    """A visible key that scores -inf has no weight; where all that a query sees do, its softmax is undefined: NaN, not the zeros of a query without a
+    key. The one visible key with a finite score comes first, last, and in a run of its own."""
+    from sleap_amd import ops
+
+    B, Tq, Tk, H, K, D = shape
+    q, k, v, dout, _, _ = make(rng(50), *shape, dtype)
+    q[..., 0] = q[..., 0].abs() + 0.25
+    low = k.clone()
+    low[..., 0] = float("-inf")
+    for at in (0, Tk // 2, Tk - 1):
+        kk = low.clone()
+        kk[0, at] = k[0, at]
+        for grad in (False, True):
+            out, lse = ops.cross_attention(q.clone().requires_grad_(grad), kk, v, return_lse=True)
+            want = v[:1, at].repeat_interleave(H // K, 1)[:, None].expand(1, Tq, H, D)
+            assert torch.equal(out[:1], want) and torch.isfinite(lse[:1]).all()
+            if B > 1:
+                assert torch.isnan(out[1:]).all() and torch.isnan(lse[1:]).all()
+    leaves = [t.requires_grad_(True) for t in (q, low, v)]
+    out, lse = ops.cross_attention(*leaves, return_lse=True)
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
+    assert all(torch.isnan(x).all() for x in torch.autograd.grad(out, leaves, dout))
+    out, lse = ops.cross_attention(q, low, v, key_lengths=torch.zeros(B, dtype=torch.int32, device=DEV), return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
 # --------------------------------------------------------------------------------------------------
 # AdamW
 # --------------------------------------------------------------------------------------------------
