@@ -50,8 +50,9 @@ __device__ __forceinline__ float lse_of_sum(float sum, float log) {
 
 // LOW: weights are multiplied in two terms, rounded and what that left, and `low` is written. For gradients over few keys: rowsum(do * out)
 // has to cancel against w^T (do v^T) there, and the roundings of w and out alone made dq and dk over 3 keys 2.2 times as inexact as
-// their own rounding (600 keys: 1.5 times; from 4096 on it no longer shows). What counts are visible keys: FEW by the length, or the first FEW
-// that a mask leaves (shared out among the runs); further ones are multiplied once.
+// their own rounding (600 keys: 1.5 times; from 4096 on it no longer shows). What counts are visible keys: FEW by the length, or, under
+// a mask, the first FEW of each run, since they may all lie in one (a share of FEW each is 4 to 15 % faster where runs are long, 125 us instead of 140
+// for 8 x 8 heads x 192 x 16384 x 64, but then 2000 visible keys that lie together are 1.36 times as far off); further ones are multiplied once.
 constexpr int FEW = 2048;
 
 // KW: waves along the keys, each with the same 32 rows, a run of keys and tiles of its own, so that they need no barrier before their sums meet
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(NW * KW * 64, 2) void attention_kernel(const FwdPar
   for (int db = 0; db < DB; ++db) ot[db] = T::at_t(lane) ^ (db << 6);
 
   f32x16 o[DB] = {};
-  int few = length <= FEW ? 0x7FFFFFFF : mask ? FEW / (int)(p.splits * KW) : 0;  // LOW: visible keys still to be multiplied twice
+  int few = length <= FEW ? 0x7FFFFFFF : mask ? FEW : 0;  // LOW: visible keys still to be multiplied twice
   float m = -INFINITY, l = 0.0f, shift = -Range<E>::LIFT;  // shift = c m - LIFT, of a maximum that is not -inf
   // A tile is copied while the one before is multiplied; the mask's bytes come one tile earlier still. (Three stages: slower by 5 to 15 %
   // at every head size, and workgroups of eight waves gain nothing either.)

@@ -443,10 +443,11 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, return
                  NaN, a score of infinity (or beyond float32) NaN; one of -infinity has no weight, and a query all of whose scores are is NaN
     scale        positive; default 1 / sqrt(D)
     return_lse   also the natural logarithm of the softmax's denominators, (B, H, Tq) float32, without a gradient
-    A query that sees no key gives zeros (lse: -inf) and passes no gradient. Softmax and sums are float32, weights are rounded to q's
-    type before the product with v (a call that is to be differentiated, over 2048 visible keys at most, multiplies what the rounding leaves as well:
-    its output is the more exact one); results do not depend on the order in which workgroups run. Differentiable in q, k and v, once: queries on a frozen map cost
-    their own gradient only, and so do keys and values together."""
+    A query that sees no key gives zeros (lse: -inf) and passes no gradient. Softmax and sums are float32. Weights are rounded to q's type ahead of
+    their products, which makes results about 1.4 times as inexact as their own rounding; what the rounding leaves is multiplied as well (and
+    results are as exact as their type) in a call that is to be differentiated over at most 2048 visible keys, and in its gradients up to 2^30
+    multiply-adds a product. Results do not depend on the order in which workgroups run. Differentiable in q, k and v, once: queries on a
+    frozen map cost their own gradient only, and so do keys and values together."""
     return _token().cross_attention(q, k, v, key_lengths, key_mask, scale, return_lse)
 
 

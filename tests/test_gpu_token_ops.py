@@ -305,6 +305,35 @@ def test_few_visible_keys_of_many(dtype, by, n):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,Tq,Tk,n", [(2, 150, 20000, 2000), (1, 30, 3000, 700), (1, 5, 40000, 600)])
+def test_visible_keys_that_lie_together(dtype, B, Tq, Tk, n):
+    """As above, for keys that one run or wave has all of."""
+    from sleap_amd import ops
+
+    g = rng(51 + n)
+    q, k, v, dout, _, _ = make(g, B, Tq, n, 2, 2, 32, dtype, scale=0.3)
+    want = oracle.attention(q, k, v, None, None, None, dout)
+    for start in (0, 64 * 11, Tk - n):
+        many = [torch.full((B, Tk, 2, 32), float("nan"), device=DEV, dtype=dtype) for _ in range(2)]
+        for x, y in zip(many, (k, v)):
+            x[:, start:start + n] = y
+        mask = torch.zeros((1, Tk), dtype=torch.bool, device=DEV)
+        mask[:, start:start + n] = True
+
+        def errors(k, v, mask=None):
+            leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+            out = ops.cross_attention(*leaves, key_mask=mask)
+            grads = torch.autograd.grad(out, leaves, dout)
+            if mask is not None:
+                grads = [grads[0], *(x[:, start:start + n] for x in grads[1:])]
+            return [(x.double() - want[name][0]).norm().item() for name, x in zip(("out", "dq", "dk", "dv"), [out.detach(), *grads])]
+
+        a, b = errors(*many, mask), errors(k, v)
+        print(dtype, B, Tq, Tk, n, start, ["%.3f" % (x / y) for x, y in zip(a, b)], flush=True)
+        assert all(x <= 1.2 * y for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("ragged", ["none", "lengths+mask"])
 @pytest.mark.parametrize("B,Tq,Tk,H,K,D", [(3, 1, 11, 2, 1, 48), (2, 18, 2, 1, 1, 72), (5, 2, 282, 8, 8, 16), (1, 300, 900, 4, 2, 128), (3, 400, 1500, 4, 2, 40), (4, 2000, 2000, 4, 4, 16)])
 def test_gradients_as_exact_as_their_type(dtype, ragged, B, Tq, Tk, H, K, D):
