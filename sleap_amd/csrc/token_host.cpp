@@ -144,8 +144,9 @@ struct Turn {
   bool shared, interleaved, inverse;
 };
 
-Tensor turn(const Tensor& x_, const Tensor& positions, const Turn& how) {
+Tensor turn(const Tensor& x_, const Tensor& positions_, const Turn& how) {
   const Laid x = laid_out(x_, how.interleaved ? 2 : 1);
+  const Tensor positions = positions_.resolve_neg();
   const int64_t B = x.t.size(0), T = x.t.size(1), H = x.t.size(2), D = x.t.size(3);
   Tensor y = at::empty({B, T, H, D}, x.t.options());
   if (B == 0 || T == 0) return y;
@@ -328,7 +329,7 @@ py::object cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
     if ((kind != at::kInt && kind != at::kLong) || keys.lengths.dim() != 1 || keys.lengths.size(0) != B)
       bad_value(who, ": key_lengths must be (", B, ",) int32 or int64: got ", keys.lengths.sizes(), " ", kind);
     if (kind == at::kLong) keys.lengths = keys.lengths.clamp(0, Tk).to(at::kInt);
-    keys.lengths = keys.lengths.contiguous();
+    keys.lengths = keys.lengths.resolve_neg().contiguous();
   }
   if (keys.mask.defined() && (keys.mask.scalar_type() != at::kBool || keys.mask.dim() != 2 || (keys.mask.size(0) != B && keys.mask.size(0) != 1) || keys.mask.size(1) != Tk))
     bad_value(who, ": key_mask must be (", B, ", ", Tk, ") bool, True where a key is visible: got ", keys.mask.sizes(), " ", keys.mask.scalar_type());

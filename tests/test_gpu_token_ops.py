@@ -94,6 +94,17 @@ def test_rotary_refusals():
             ops.rotary_axes(**{**dict(x=x, positions=p, sections=(4, 4)), **bad})
 
 
+def test_rotary_reads_negated_views():
+    """The imaginary part of a conjugated tensor is a float view that torch holds with the other sign."""
+    from sleap_amd import ops
+
+    z = torch.randn((7, 2), generator=rng(43), device=DEV, dtype=torch.complex64) * 50
+    p = z.conj().imag
+    assert p.is_neg()
+    x = normal(rng(44), 1, 7, 2, 16, dtype=torch.float32)
+    assert oracle.worst(ops.rotary_axes(x, p, (4, 4)), oracle.rotary(x, p.resolve_neg(), (4, 4))) <= 1
+
+
 def test_attention_refusals():
     from sleap_amd import ops
 
