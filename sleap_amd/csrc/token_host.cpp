@@ -72,7 +72,14 @@ int type_of(const Tensor& t) {
   }
 }
 
+// forward-mode derivatives (torch.autograd.forward_ad) would be lost without a word: a kernel reads a tensor's values alone
+void no_tangent(const char* who, const char* name, const Tensor& t) {
+  if (t._fw_grad(/*level=*/0).defined()) throw std::runtime_error(text(who, ": ", name, " carries a forward-mode derivative: there are none"));
+}
+
 void on_one_gpu(const char* who, std::initializer_list<std::pair<const char*, const Tensor*>> tensors) {
+  for (const auto& [name, t] : tensors)
+    if (t->defined()) no_tangent(who, name, *t);
   const Tensor* first = nullptr;
   for (const auto& [name, t] : tensors) {
     if (!t->defined()) continue;
@@ -372,6 +379,7 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
   for (const auto& [tensor, kind, what] : {std::tuple(&step, at::kLong, "a step tensor is one int64"), std::tuple(&lr, at::kFloat, "a learning rate tensor is one float32")})
     if (THPVariable_Check(tensor->ptr())) {
       const Tensor& x = THPVariable_Unpack(tensor->ptr());
+      no_tangent(who, "a step or learning rate tensor", x);
       if (x.scalar_type() != kind || x.numel() != 1 || !x.is_cuda()) bad_value(who, ": ", what, " on the GPU of the parameters");
     }
   if (n == 0) return;
@@ -388,6 +396,7 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
     for (int j = 0; j < lists; ++j) {
       if (!THPVariable_Check(items[j][i])) bad_value(who, ": lists of CUDA tensors: ", names[j], "[", i, "] is none");
       x[j] = &THPVariable_Unpack(items[j][i]);
+      no_tangent(who, names[j], *x[j]);
       if (!x[j]->is_cuda() || x[j]->get_device() != x[0]->get_device())
         bad_value(who, ": CUDA tensors, a parameter, its gradient and its states on one GPU (there is no CPU fallback): ", names[j], "[", i, "] is on ", x[j]->device());
       if (x[j]->layout() != at::kStrided || !x[j]->is_contiguous()) bad_value(who, ": ", names[j], "[", i, "] must be contiguous");

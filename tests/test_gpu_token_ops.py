@@ -105,6 +105,26 @@ def test_rotary_reads_negated_views():
     assert oracle.worst(ops.rotary_axes(x, p, (4, 4)), oracle.rotary(x, p.resolve_neg(), (4, 4))) <= 1
 
 
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+
+    from sleap_amd import ops
+
+    x, p = normal(rng(45), 1, 5, 2, 16, dtype=torch.float32), torch.zeros((5, 2), device=DEV)
+    q, k, v, _, _, _ = make(rng(46), 1, 5, 9, 2, 2, 16, torch.float16)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: ops.rotary_axes(dual(x), p, (4, 4)), lambda: ops.rotary_axes(x, dual(p), (4, 4)), lambda: ops.cross_attention(dual(q), k, v),
+                     lambda: ops.cross_attention(q, dual(k), v), lambda: ops.cross_attention(q, k, dual(v))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        one = [torch.ones(3, device=DEV) for _ in range(4)]
+        for j in range(4):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ops.adamw_step(*[[dual(t) if i == j else t] for i, t in enumerate(one)], step=1, lr=1e-3)
+        ops.rotary_axes(x, p, (4, 4))  # without a tangent: as ever
+
+
 def test_attention_refusals():
     from sleap_amd import ops
 

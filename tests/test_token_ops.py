@@ -143,6 +143,23 @@ def test_host_tensors_are_refused():
         AdamW([], lr=-1.0)
 
 
+def test_tangents_are_refused():
+    """Forward-mode derivatives would be dropped silently; refused ahead of the device."""
+    import torch.autograd.forward_ad as fw
+
+    x, p = torch.zeros((1, 2, 1, 8)), torch.zeros((2, 1))
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t, torch.ones_like(t))
+
+        h = x.half()
+        for call in (lambda: ops.rotary_axes(dual(x), p, (2,)), lambda: ops.rotary_axes(x, dual(p), (2,)), lambda: ops.cross_attention(dual(h), h, h),
+                     lambda: ops.cross_attention(h, dual(h), h), lambda: ops.cross_attention(h, h, dual(h)), lambda: ops.adamw_step([dual(x)], [x], [x], [x], step=1, lr=1e-3),
+                     lambda: ops.adamw_step([x], [x], [x], [x], step=1, lr=dual(torch.ones(1)))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
 def test_oracle_gradients_against_differences():
     """The formulas of the attention oracle by central differences in 64 bits."""
     g = torch.Generator().manual_seed(0)
