@@ -381,6 +381,7 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
       const Tensor& x = THPVariable_Unpack(tensor->ptr());
       no_tangent(who, "a step or learning rate tensor", x);
       if (x.scalar_type() != kind || x.numel() != 1 || !x.is_cuda()) bad_value(who, ": ", what, " on the GPU of the parameters");
+      if (x.is_neg()) bad_value(who, ": ", what, ", not a negated view");
     }
   if (n == 0) return;
 
@@ -400,6 +401,7 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
       if (!x[j]->is_cuda() || x[j]->get_device() != x[0]->get_device())
         bad_value(who, ": CUDA tensors, a parameter, its gradient and its states on one GPU (there is no CPU fallback): ", names[j], "[", i, "] is on ", x[j]->device());
       if (x[j]->layout() != at::kStrided || !x[j]->is_contiguous()) bad_value(who, ": ", names[j], "[", i, "] must be contiguous");
+      if (x[j]->is_neg()) bad_value(who, ": ", names[j], "[", i, "] is a negated view");  // its memory has the other sign
       if (x[j]->numel() != x[0]->numel()) bad_value(who, ": ", names[j], "[", i, "] differs in size from its parameter");
       if (j >= 2 && x[j]->scalar_type() != at::kFloat) bad_type(who, ": the states must be float32");
     }

@@ -797,6 +797,20 @@ def test_adamw_refuses_what_it_would_write_twice():
         ops.adamw_step(p, gr, m, v, step=0, lr=1e-3)
 
 
+def test_adamw_refuses_negated_views():
+    from sleap_amd import ops
+
+    z = torch.ones((1,), device=DEV, dtype=torch.complex64)
+    neg = z.conj().imag
+    assert neg.is_neg() and neg.is_contiguous()
+    one = [torch.ones(1, device=DEV) for _ in range(4)]
+    for j in range(4):
+        with pytest.raises(ValueError, match="negated"):
+            ops.adamw_step(*[[neg if i == j else t] for i, t in enumerate(one)], step=1, lr=1e-3)
+    with pytest.raises(ValueError, match="negated"):
+        ops.adamw_step(*[[t] for t in one], step=1, lr=neg)
+
+
 def test_an_adamw_step_is_noticed_by_graphs():
     from sleap_amd import ops
 
