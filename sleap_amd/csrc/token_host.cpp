@@ -77,6 +77,12 @@ void no_tangent(const char* who, const char* name, const Tensor& t) {
   if (t._fw_grad(/*level=*/0).defined()) throw std::runtime_error(text(who, ": ", name, " carries a forward-mode derivative: there are none"));
 }
 
+// The step has no gradient: a graph that it would cut, with what it leaves behind of it, is refused. (A parameter that is a leaf has none.)
+void no_graph(const char* what, const Tensor& t, bool leaf) {
+  if (at::GradMode::is_enabled() && t.requires_grad() && !(leaf && t.is_leaf()))
+    throw std::runtime_error(text("adamw_step: there is no gradient through a step (", what, " requires one): call it under torch.no_grad()"));
+}
+
 void on_one_gpu(const char* who, std::initializer_list<std::pair<const char*, const Tensor*>> tensors) {
   for (const auto& [name, t] : tensors)
     if (t->defined()) no_tangent(who, name, *t);
@@ -380,6 +386,7 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
     if (THPVariable_Check(tensor->ptr())) {
       const Tensor& x = THPVariable_Unpack(tensor->ptr());
       no_tangent(who, "a step or learning rate tensor", x);
+      no_graph("a step or learning rate tensor", x, false);
       if (x.scalar_type() != kind || x.numel() != 1 || !x.is_cuda()) bad_value(who, ": ", what, " on the GPU of the parameters");
       if (x.is_neg()) bad_value(who, ": ", what, ", not a negated view");
     }
@@ -398,6 +405,7 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
       if (!THPVariable_Check(items[j][i])) bad_value(who, ": lists of CUDA tensors: ", names[j], "[", i, "] is none");
       x[j] = &THPVariable_Unpack(items[j][i]);
       no_tangent(who, names[j], *x[j]);
+      no_graph(names[j], *x[j], j == 0);
       if (!x[j]->is_cuda() || x[j]->get_device() != x[0]->get_device())
         bad_value(who, ": CUDA tensors, a parameter, its gradient and its states on one GPU (there is no CPU fallback): ", names[j], "[", i, "] is on ", x[j]->device());
       if (x[j]->layout() != at::kStrided || !x[j]->is_contiguous()) bad_value(who, ": ", names[j], "[", i, "] must be contiguous");

@@ -811,6 +811,23 @@ def test_adamw_refuses_negated_views():
         ops.adamw_step(*[[t] for t in one], step=1, lr=neg)
 
 
+def test_adamw_refuses_to_cut_a_graph():
+    from sleap_amd import ops
+
+    def sets():
+        return [torch.ones(4, device=DEV) for _ in range(4)]
+
+    for j in range(4):
+        one = sets()
+        one[j] = one[j].requires_grad_(True) * 2
+        with pytest.raises(RuntimeError, match="no gradient"):
+            ops.adamw_step(*[[t] for t in one], step=1, lr=1e-3)
+        with torch.no_grad():
+            ops.adamw_step(*[[t] for t in one], step=1, lr=1e-3)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.adamw_step(*[[t] for t in sets()], step=1, lr=torch.ones(1, device=DEV).requires_grad_(True))
+
+
 def test_an_adamw_step_is_noticed_by_graphs():
     from sleap_amd import ops
 
