@@ -140,12 +140,13 @@ struct Laid {
 };
 Laid laid_out(Tensor t, int64_t elements, int64_t limit = 0, int64_t group = 0) {
   t = t.resolve_neg();
+  if (t.numel() == 0) return {std::move(t), {}};  // nothing to step over, whatever its strides say
   for (int turn = 0;; ++turn) {
     std::array<int64_t, 3> s;
     for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
     const bool fits = (t.size(3) == 1 || t.stride(3) == 1) && s[0] % elements == 0 && s[1] % elements == 0 && s[2] % elements == 0 &&
                       reinterpret_cast<uintptr_t>(t.data_ptr()) % (elements * t.element_size()) == 0 && (!limit || 64 * s[1] + group * s[2] < limit);
-    if (fits || turn || t.numel() == 0) return {std::move(t), s};
+    if (fits || turn) return {std::move(t), s};
     t = t.clone(at::MemoryFormat::Contiguous);
   }
 }

@@ -277,6 +277,16 @@ def test_attention_takes_any_layout():
     check(q, packed[:, :, 0], packed[:, :, 1], dout, lengths=torch.tensor([[90, 1], [17, 1]], device=DEV)[:, 0])  # int64, strided
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_of_empty_views(dtype):
+    """No keys, and no queries, cut from a layout whose strides the kernels do not take."""
+    g = rng(47)
+    q, wide = normal(g, 2, 4, 3, 8, dtype=dtype), normal(g, 2, 5, 3, 9, dtype=dtype)
+    none = wide[..., :8][:, :0]
+    check(q, none, none, q)
+    check(none, q, q, none)
+
+
 def test_gradients_of_broadcast_inputs_are_summed():
     from sleap_amd import ops
 
