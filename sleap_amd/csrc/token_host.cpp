@@ -219,7 +219,7 @@ Tensor rotary_axes(const Tensor& x, const Tensor& positions, const std::vector<i
     bad_value(who, ": positions ", positions.sizes(), " for ", B, " x ", T, " tokens and ", A, " axes");
   if (ladder != "axis" && ladder != "shared") bad_value(who, ": ladder '", ladder, "': 'axis' or 'shared'");
   if (!(theta > 0 && theta < 1e30)) bad_value(who, ": theta ", theta);
-  if (positions.requires_grad()) bad_value(who, ": there is no gradient for positions");
+  if (positions.requires_grad() && at::GradMode::is_enabled()) bad_value(who, ": there is no gradient for positions");
   const Turn how = {{sections.begin(), sections.end()}, theta, ladder == "shared", interleaved, inverse};
   if (!x.requires_grad() || !at::GradMode::is_enabled()) return turn(x, positions, how);
   not_held_elsewhere(who, {&x});

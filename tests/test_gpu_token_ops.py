@@ -125,6 +125,15 @@ def test_tangents_are_refused():
         ops.rotary_axes(x, p, (4, 4))  # without a tangent: as ever
 
 
+def test_rotary_of_positions_that_are_learned_elsewhere():
+    from sleap_amd import ops
+
+    x, p = normal(rng(48), 1, 5, 2, 16, dtype=torch.float32), torch.rand((5, 2), device=DEV)
+    want = ops.rotary_axes(x, p, (4, 4))
+    with torch.no_grad():
+        assert torch.equal(ops.rotary_axes(x, p.requires_grad_(True), (4, 4)), want)
+
+
 def test_attention_refusals():
     from sleap_amd import ops
 
