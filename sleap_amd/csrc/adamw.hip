@@ -151,7 +151,7 @@ int step_all(AdamwParams<AMS>& a, const sa_adamw_tensor* tensors, int n, int dty
         a.high[k][a.n] = (uint16_t)((uintptr_t)address[k] >> 32);
       }
       const uint32_t pieces = (uint32_t)((t.n + CHUNK - 1) / CHUNK);
-      if (a.n && (uint64_t)a.blocks + pieces >= (1ull << 31)) break;  // a launch's workgroups
+      if (a.n && (uint64_t)a.blocks + pieces >= (1ull << 24)) break;  // a launch has less than 2^32 threads
       a.tail[a.n] = (uint16_t)(t.n - (int64_t)(pieces - 1) * CHUNK);
       a.first[a.n++] = a.blocks;
       a.blocks += pieces;

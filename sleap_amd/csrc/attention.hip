@@ -67,7 +67,9 @@ __global__ __launch_bounds__(NW * KW * 64, 2) void attention_kernel(const FwdPar
   const int id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = KW > 1 ? 0 : id, part = KW > 1 ? id : 0;
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   char* lds = lds_all + part * 4 * T::BYTES;
-  const Piece piece = piece_of(blockIdx.x, p.heads, p.row_tiles * p.splits, p.div_pieces);
+  const uint32_t block = workgroup();
+  if (block >= p.blocks) return;
+  const Piece piece = piece_of(block, p.heads, p.row_tiles * p.splits, p.div_pieces);
   const uint32_t bh = piece.head, split = div_by(piece.at, p.div_tiles), tile = piece.at - split * p.row_tiles;
   const uint32_t b = div_by(bh, p.div_heads), hk = bh - b * a.Hkv;
 
@@ -264,7 +266,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const FwdParams p, 
   __shared__ float sums[256][10];
   const AttnShape& a = p.a;
   const uint32_t groups = 1u << groups_log2, lane = threadIdx.x & 15, unit = threadIdx.x >> 4, group = unit & (groups - 1);
-  const uint32_t br = blockIdx.x * (16 >> groups_log2) + (unit >> groups_log2), d = lane * 8;
+  const uint32_t block = workgroup();
+  if ((uint64_t)block * (16 >> groups_log2) >= rows) return;
+  const uint32_t br = block * (16 >> groups_log2) + (unit >> groups_log2), d = lane * 8;
   const bool real = br < rows && d < (uint32_t)a.D;
   const uint32_t bh = div_by(min(br, rows - 1), div_rows), row = min(br, rows - 1) - bh * a.R;
   const float* lse = p.part_lse + (int64_t)bh * p.splits * a.R + row;
@@ -390,13 +394,13 @@ void launch_low(const FwdParams& p, const Cut& c, hipStream_t s) {
     if (c.key_waves > 1) {
       const auto kernel = attention_kernel<E, DB, 1, LOW, 4>;
       if (4 * lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)(4 * lds));
-      kernel<<<dim3(p.blocks), dim3(256), 4 * lds, s>>>(p);
+      kernel<<<grid_of(p.blocks), dim3(256), 4 * lds, s>>>(p);
       return;
     }
   }
-  if (c.waves == 1) attention_kernel<E, DB, 1, LOW, 1><<<dim3(p.blocks), dim3(64), lds, s>>>(p);
-  else if (c.waves == 2) attention_kernel<E, DB, 2, LOW, 1><<<dim3(p.blocks), dim3(128), lds, s>>>(p);
-  else attention_kernel<E, DB, 4, LOW, 1><<<dim3(p.blocks), dim3(256), lds, s>>>(p);
+  if (c.waves == 1) attention_kernel<E, DB, 1, LOW, 1><<<grid_of(p.blocks), dim3(64), lds, s>>>(p);
+  else if (c.waves == 2) attention_kernel<E, DB, 2, LOW, 1><<<grid_of(p.blocks), dim3(128), lds, s>>>(p);
+  else attention_kernel<E, DB, 4, LOW, 1><<<grid_of(p.blocks), dim3(256), lds, s>>>(p);
 }
 
 template <typename E, int DB>
@@ -417,7 +421,7 @@ void launch_e(const FwdParams& p, const Cut& c, hipStream_t s) {
     uint32_t log2 = 0;
     while (log2 < 4 && (4u << log2) < p.splits) ++log2;  // four runs a group
     const uint32_t per = 16 >> log2;
-    attention_join_kernel<E><<<dim3((rows + per - 1) / per), dim3(256), 0, s>>>(p, fast_div(p.a.R), log2, rows);
+    attention_join_kernel<E><<<grid_of((rows + per - 1) / per), dim3(256), 0, s>>>(p, fast_div(p.a.R), log2, rows);
   }
 }
 

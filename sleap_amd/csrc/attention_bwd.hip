@@ -83,7 +83,9 @@ constexpr double FREE = 1024.0 * 1024 * 1024;
 template <typename E>
 __global__ __launch_bounds__(256) void attention_stats_kernel(const BwdParams p, uint32_t total) {
   const AttnShape& a = p.a;
-  const uint32_t i = blockIdx.x * 16 + (threadIdx.x >> 4);  // 16 lanes of 8 values a row
+  const uint32_t block = workgroup();
+  if ((uint64_t)block * 16 >= total) return;
+  const uint32_t i = block * 16 + (threadIdx.x >> 4);  // 16 lanes of 8 values a row
   const uint32_t ic = min(i, total - 1);
   const uint32_t bt = div_by(ic, p.div_hq), hh = ic - bt * a.Hq;
   const uint32_t b = bt / a.Tq, t = bt - b * a.Tq;
@@ -384,8 +386,9 @@ __device__ __forceinline__ void rows_side(const BwdParams& p, uint32_t block, ch
 template <typename E, int DB, int NW, bool TWICE>
 __global__ __launch_bounds__(NW * 64, 2) void attention_bwd_kernel(const BwdParams p) {
   extern __shared__ __align__(1024) char lds[];
-  if (blockIdx.x < p.rows.blocks) rows_side<E, DB, NW, TWICE || DB == 1>(p, blockIdx.x, lds);
-  else keys_side<E, DB, NW, TWICE>(p, blockIdx.x - p.rows.blocks, lds);
+  const uint32_t block = workgroup();
+  if (block < p.rows.blocks) rows_side<E, DB, NW, TWICE || DB == 1>(p, block, lds);
+  else if (block < p.rows.blocks + p.kv.blocks) keys_side<E, DB, NW, TWICE>(p, block - p.rows.blocks, lds);
 }
 
 // Adds the runs' gradients, in their order, of up to three tensors; a thread has 8 values of one.
@@ -395,11 +398,14 @@ struct AddParams {
   int64_t n[3];
   int splits[3];
   uint32_t first[3];  // first workgroup of each
+  uint32_t blocks;
 };
 template <typename E>
 __global__ __launch_bounds__(256) void attention_add_kernel(const AddParams p) {
-  const int k = blockIdx.x >= p.first[2] ? 2 : blockIdx.x >= p.first[1] ? 1 : 0;
-  const int64_t i = ((int64_t)(blockIdx.x - p.first[k]) * 256 + threadIdx.x) * 8, n = p.n[k];
+  const uint32_t block = workgroup();
+  if (block >= p.blocks) return;
+  const int k = block >= p.first[2] ? 2 : block >= p.first[1] ? 1 : 0;
+  const int64_t i = ((int64_t)(block - p.first[k]) * 256 + threadIdx.x) * 8, n = p.n[k];
   if (i >= n) return;
   f32x4 x = {}, y = {};
 #pragma unroll 4
@@ -456,7 +462,7 @@ void launch_sides(const BwdParams& p, int waves, hipStream_t s) {
   constexpr size_t lds = 2 * (2 * Tile<DB == 3 ? 128 : DB * 32>::BYTES + 2 * TILE * 4);  // the keys' side, which has the rows' numbers beside its tiles
   auto go = [&](auto kernel) {
     if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    kernel<<<dim3(p.rows.blocks + p.kv.blocks), dim3(waves * 64), lds, s>>>(p);
+    kernel<<<grid_of((uint64_t)p.rows.blocks + p.kv.blocks), dim3(waves * 64), lds, s>>>(p);
   };
   if (waves == 1) go(attention_bwd_kernel<E, DB, 1, TWICE>);
   else if (waves == 2) go(attention_bwd_kernel<E, DB, 2, TWICE>);
@@ -469,7 +475,7 @@ int launch(const BwdParams& p, int waves, hipStream_t s) {
   const int db = (a.D + 31) / 32;
   if (a.R) {
     const uint32_t rows = p.heads * a.R;
-    attention_stats_kernel<E><<<dim3((rows + 15) / 16), dim3(256), 0, s>>>(p, rows);
+    attention_stats_kernel<E><<<grid_of(((uint64_t)rows + 15) / 16), dim3(256), 0, s>>>(p, rows);
     SA_LAUNCH_CHECK();
   }
   if (p.rows.blocks + p.kv.blocks == 0) return SA_OK;
@@ -497,7 +503,8 @@ int launch(const BwdParams& p, int waves, hipStream_t s) {
   sum(1, p.part_dv, p.dv, a.Tk, p.kv.splits);
   sum(2, p.part_dq, p.dq, a.R, p.rows.splits);
   if (blocks) {
-    attention_add_kernel<E><<<dim3(blocks), dim3(256), 0, s>>>(add);
+    add.blocks = blocks;
+    attention_add_kernel<E><<<grid_of(blocks), dim3(256), 0, s>>>(add);
     SA_LAUNCH_CHECK();
   }
   return SA_OK;

@@ -24,7 +24,7 @@ struct RotaryParams {
   int64_t xb, xt, xh;      // strides of x, in elements
   int64_t pb, pt, pa;      // strides of the positions
   int T, H, D, P, tok;     // tokens, heads, head size, pairs, tokens of a workgroup
-  uint32_t tiles;          // workgroups of a batch entry
+  uint32_t tiles, blocks;  // workgroups of a batch entry, of the launch
   FastDiv div_tiles, div_g, div_h, div_p;
   int G;                   // pieces of a head: P / V (or 2P / V) rotated ones, then the ones that pass
   int rot;                 // how many of them are rotated
@@ -47,8 +47,10 @@ __device__ __forceinline__ double position(const RotaryParams& p, int64_t i) {
 template <typename T, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
   extern __shared__ float2 cs[];  // [tok][P]
-  const uint32_t b = div_by(blockIdx.x, p.div_tiles);
-  const int t0 = (int)(blockIdx.x - b * p.tiles) * p.tok;
+  const uint32_t block = workgroup();
+  if (block >= p.blocks) return;
+  const uint32_t b = div_by(block, p.div_tiles);
+  const int t0 = (int)(block - b * p.tiles) * p.tok;
   const int nt = min(p.tok, p.T - t0);
   for (uint32_t i = threadIdx.x; i < (uint32_t)(nt * p.P); i += 256) {
     const uint32_t t = div_by(i, p.div_p), j = i - t * p.P;
@@ -98,19 +100,19 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
 }
 
 template <typename T, int V>
-void launch_v(const RotaryParams& p, bool interleaved, uint32_t blocks, size_t lds, hipStream_t s) {
-  if (!interleaved) rotary_kernel<T, V, false><<<dim3(blocks), dim3(256), lds, s>>>(p);
-  else if constexpr (V > 1) rotary_kernel<T, V, true><<<dim3(blocks), dim3(256), lds, s>>>(p);
+void launch_v(const RotaryParams& p, bool interleaved, size_t lds, hipStream_t s) {
+  if (!interleaved) rotary_kernel<T, V, false><<<grid_of(p.blocks), dim3(256), lds, s>>>(p);
+  else if constexpr (V > 1) rotary_kernel<T, V, true><<<grid_of(p.blocks), dim3(256), lds, s>>>(p);
 }
 
 template <typename T>
-void launch(const RotaryParams& p, int V, bool interleaved, uint32_t blocks, size_t lds, hipStream_t s) {
-  if (V * sizeof(T) == 16) return launch_v<T, 16 / sizeof(T)>(p, interleaved, blocks, lds, s);
+void launch(const RotaryParams& p, int V, bool interleaved, size_t lds, hipStream_t s) {
+  if (V * sizeof(T) == 16) return launch_v<T, 16 / sizeof(T)>(p, interleaved, lds, s);
   if constexpr (sizeof(T) == 2) {
-    if (V == 4) return launch_v<T, 4>(p, interleaved, blocks, lds, s);
+    if (V == 4) return launch_v<T, 4>(p, interleaved, lds, s);
   }
-  if (V == 2) return launch_v<T, 2>(p, interleaved, blocks, lds, s);
-  launch_v<T, 1>(p, interleaved, blocks, lds, s);
+  if (V == 2) return launch_v<T, 2>(p, interleaved, lds, s);
+  launch_v<T, 1>(p, interleaved, lds, s);
 }
 
 }  // namespace
@@ -179,11 +181,12 @@ extern "C" int sa_rotary_axes(const void* x, int dtype, int B, int T, int H, int
   p.div_g = fast_div(p.G);
   p.div_h = fast_div(H);
   p.div_p = fast_div(P);
+  p.blocks = (uint32_t)blocks;
   const size_t lds = sizeof(float2) * tok * P;
   const hipStream_t s = (hipStream_t)stream;
-  if (dtype == SA_F32) launch<float>(p, V, interleaved, (uint32_t)blocks, lds, s);
-  else if (dtype == SA_F16) launch<_Float16>(p, V, interleaved, (uint32_t)blocks, lds, s);
-  else launch<__bf16>(p, V, interleaved, (uint32_t)blocks, lds, s);
+  if (dtype == SA_F32) launch<float>(p, V, interleaved, lds, s);
+  else if (dtype == SA_F16) launch<_Float16>(p, V, interleaved, lds, s);
+  else launch<__bf16>(p, V, interleaved, lds, s);
   SA_LAUNCH_CHECK();
   return SA_OK;
 }

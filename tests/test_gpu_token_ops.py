@@ -134,6 +134,15 @@ def test_rotary_of_positions_that_are_learned_elsewhere():
         assert torch.equal(ops.rotary_axes(x, p.requires_grad_(True), (4, 4)), want)
 
 
+def test_rotary_of_more_workgroups_than_a_grid_row():
+    """2^24 single tokens: more threads than one dimension of a launch has."""
+    from sleap_amd import ops
+
+    g, B = rng(54), (1 << 24) + 5
+    x, p = normal(g, B, 1, 1, 4, dtype=torch.float16), torch.rand((B, 1, 1), generator=g, device=DEV) * 100
+    assert oracle.worst(ops.rotary_axes(x, p, (2,)), oracle.rotary(x, p, (2,))) <= 1
+
+
 def test_attention_refusals():
     from sleap_amd import ops
 
@@ -485,6 +494,31 @@ def test_keys_beyond_32_bit_offsets():
     near = ops.cross_attention(q, k.contiguous(), v.contiguous())
     far = ops.cross_attention(q, k, v)
     assert torch.equal(near, far)
+
+
+@pytest.mark.parametrize("B,Tq", [((1 << 26) + 9, 1), (1, (1 << 28) + 17)])
+def test_attention_of_more_workgroups_than_a_grid_row(B, Tq):
+    """2^26 images of one query, and 2^28 queries (row statistics have 16 threads each), on two keys of equal weight and small whole values:
+    all results are exact. With the gradients of whichever side is as large."""
+    from sleap_amd import ops
+
+    def whole(*shape, step=1):
+        return (torch.randint(-2, 3, shape, generator=rng(sum(shape)), device=DEV, dtype=torch.int8) * step).half()
+
+    q, k, v, dout = torch.zeros((B, Tq, 1, 8), device=DEV, dtype=torch.float16), whole(B, 2, 1, 8), whole(B, 2, 1, 8, step=2), whole(B, Tq, 1, 8)
+    leaves = [q.requires_grad_(True), k.requires_grad_(B > 1), v.requires_grad_(B > 1)]
+    out = ops.cross_attention(*leaves, scale=1.0)
+    grads = torch.autograd.grad(out, leaves if B > 1 else leaves[:1], dout)
+    with torch.no_grad():
+        for rows in torch.arange(max(B, Tq), device=DEV).split(1 << 24):
+            b, t = (slice(int(rows[0]), int(rows[-1]) + 1), slice(None)) if B > 1 else (slice(None), slice(int(rows[0]), int(rows[-1]) + 1))
+            kk, vv, do = k[b].float(), v[b].float(), dout[b, t].float()
+            mean = vv.mean(1, keepdim=True)
+            assert torch.equal(out[b, t].float(), mean.expand(do.shape))
+            ds = 0.5 * (do * (vv[:, :1] - mean)).sum(-1, keepdim=True)  # of the first key; the second has the opposite
+            assert torch.equal(grads[0][b, t].float(), ds * (kk[:, :1] - kk[:, 1:]))
+            if B > 1:
+                assert (grads[1][b] == 0).all() and torch.equal(grads[2][b].float(), (0.5 * do).expand(vv.shape))
 
 
 def test_attention_on_another_stream():
