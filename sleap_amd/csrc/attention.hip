@@ -266,9 +266,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const FwdParams p, 
   __shared__ float sums[256][10];
   const AttnShape& a = p.a;
   const uint32_t groups = 1u << groups_log2, lane = threadIdx.x & 15, unit = threadIdx.x >> 4, group = unit & (groups - 1);
-  const uint32_t block = workgroup();
-  if ((uint64_t)block * (16 >> groups_log2) >= rows) return;
-  const uint32_t br = block * (16 >> groups_log2) + (unit >> groups_log2), d = lane * 8;
+  const uint32_t br = workgroup() * (16 >> groups_log2) + (unit >> groups_log2), d = lane * 8;
   const bool real = br < rows && d < (uint32_t)a.D;
   const uint32_t bh = div_by(min(br, rows - 1), div_rows), row = min(br, rows - 1) - bh * a.R;
   const float* lse = p.part_lse + (int64_t)bh * p.splits * a.R + row;

@@ -83,9 +83,7 @@ constexpr double FREE = 1024.0 * 1024 * 1024;
 template <typename E>
 __global__ __launch_bounds__(256) void attention_stats_kernel(const BwdParams p, uint32_t total) {
   const AttnShape& a = p.a;
-  const uint32_t block = workgroup();
-  if ((uint64_t)block * 16 >= total) return;
-  const uint32_t i = block * 16 + (threadIdx.x >> 4);  // 16 lanes of 8 values a row
+  const uint32_t i = workgroup() * 16 + (threadIdx.x >> 4);  // 16 lanes of 8 values a row
   const uint32_t ic = min(i, total - 1);
   const uint32_t bt = div_by(ic, p.div_hq), hh = ic - bt * a.Hq;
   const uint32_t b = bt / a.Tq, t = bt - b * a.Tq;

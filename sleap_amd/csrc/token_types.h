@@ -29,8 +29,7 @@ inline FastDiv fast_div(uint32_t d) {
 __device__ __forceinline__ uint32_t div_by(uint32_t n, const FastDiv& f) { return (__umulhi(n, f.m) + n) >> f.s; }
 
 // A grid dimension has less than 2^32 threads; a launch of more runs some of them and reports no error. Workgroups (256 threads at most) are
-// counted along rows of 2^23.
-// A kernel returns where its workgroup's number is not below the launch's.
+// counted along rows of 2^23; a kernel returns, or stores nothing, where its workgroup's number is not below the launch's.
 constexpr uint32_t GRID_ROW = 1u << 23;
 inline dim3 grid_of(uint64_t blocks) {
   return blocks <= GRID_ROW ? dim3((uint32_t)blocks) : dim3(GRID_ROW, (uint32_t)((blocks + GRID_ROW - 1) / GRID_ROW));
