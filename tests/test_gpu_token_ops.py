@@ -236,6 +236,54 @@ def test_attention_of_many_tiles(dtype, B, Tq, Tk, H, K, D):
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("ragged", ["none", "lengths+mask"])
+@pytest.mark.parametrize("B,Tq,Tk,H,K,D", [(2300, 30, 31, 8, 8, 40), (600, 60, 64, 8, 8, 64), (2, 1100, 1300, 8, 8, 64), (4, 1100, 1300, 8, 8, 48), (1, 1700, 1701, 4, 4, 96),
+                                           (3, 900, 1001, 8, 4, 72), (1, 1500, 1501, 4, 4, 128), (2, 2500, 999, 4, 1, 104)])
+def test_gradients_multiplied_once(dtype, ragged, B, Tq, Tk, H, K, D):
+    """Just above 2^30 multiply-adds a product: the kernels of long training calls, in all their widths, with one, two and four waves."""
+    assert B * H * Tq * Tk * -(-D // 32) * 32 > 2 ** 30
+    check(*make(rng(B + Tq * Tk + D), B, Tq, Tk, H, K, D, dtype, ragged))
+
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ragged", ["none", "lengths+mask"])
+@pytest.mark.parametrize("B,Tq,Tk,H,K,D", [(13, 130, 8000, 20, 20, 64), (13, 300, 500, 20, 20, 64), (3, 1500, 2100, 24, 12, 128), (9, 1100, 2300, 8, 8, 24)])
+def test_more_workgroups_than_places(dtype, ragged, B, Tq, Tk, H, K, D):
+    """More than 512 workgroups of 128 rows, where runs of keys even out the last round and where they do not pay."""
+    assert B * K * -(-Tq * (H // K) // 128) > 512
+    check(*make(rng(B + Tq * Tk + D), B, Tq, Tk, H, K, D, dtype, ragged))
+
+
+
+def test_layouts_that_span_too_far_are_copied():
+    """Tokens of q, k, v and dout so far apart that the kernels' 32-bit offsets do not reach over a tile; and keys that they just reach over."""
+    g = rng(41)
+    for step in (1 << 24, (1 << 23) - 8):
+        held = torch.empty((72, step), dtype=torch.bfloat16, device=DEV)
+        held[:, :256] = normal(g, 72, 256, dtype=torch.bfloat16)
+        q, k, v, dout = (held[:n, a:a + 64].view(1, n, 2, 32) for n, a in ((40, 0), (70, 64), (70, 128), (40, 192)))
+        check(q, k, v, dout)
+
+
+
+def test_gradients_of_keys_beyond_32_bit_offsets():
+    """Keys 128 Ki elements apart: the last lie 4.3 GB behind the first. (The copies are contiguous, the order of sums is the same.)"""
+    from sleap_amd import ops
+
+    g, Tk, step = rng(42), 16500, 1 << 17
+    held = torch.empty((Tk, step), dtype=torch.bfloat16, device=DEV)
+    held[:, :64] = normal(g, Tk, 64, dtype=torch.bfloat16)
+    far = [held[:, :32].view(1, Tk, 1, 32), held[:, 32:64].view(1, Tk, 1, 32)]
+    q, dout = normal(g, 1, 3, 2, 32, dtype=torch.bfloat16), normal(g, 1, 3, 2, 32, dtype=torch.bfloat16)
+    got = []
+    for k, v in (far, [t.contiguous() for t in far]):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        got.append(torch.autograd.grad(ops.cross_attention(*leaves), leaves, dout))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ragged", ["none", "lengths+mask"])
 @pytest.mark.parametrize("B,Tq,Tk,H,K,D", [(1, 52, 1024, 8, 8, 32), (3, 33, 129, 2, 1, 8), (3, 20, 192, 4, 4, 64), (2, 1, 193, 2, 2, 40), (1, 800, 1537, 8, 8, 64), (3, 410, 1500, 8, 8, 32),
                                            (16, 500, 320, 1, 1, 32), (16, 513, 320, 1, 1, 32), (8, 1000, 500, 1, 1, 48), (8, 1025, 500, 1, 1, 48)])
 def test_attention_of_waves_along_the_keys(dtype, ragged, B, Tq, Tk, H, K, D):
