@@ -181,7 +181,7 @@ extern "C" int sa_adamw_step(const sa_adamw_tensor* tensors, int n, int dtype, i
                "sa_adamw_step: tensor %d has a negative size or a null address", i);
     SA_REQUIRE((((uintptr_t)t.param | (uintptr_t)t.grad | (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq | (uintptr_t)(amsgrad ? t.max_exp_avg_sq : nullptr)) >> 48) == 0,
                "sa_adamw_step: tensor %d: addresses have 48 bits", i);
-    SA_REQUIRE((t.n + CHUNK - 1) / CHUNK < (1ll << 24), "sa_adamw_step: tensor %d has more than 2^36 values", i);
+    SA_REQUIRE(t.n <= (1ll << 36) - CHUNK, "sa_adamw_step: tensor %d has more than 2^36 values", i);
   }
   auto go = [&](auto& a) {
     a.lr = (float)lr;

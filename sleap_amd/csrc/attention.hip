@@ -343,7 +343,7 @@ Cut cut(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
   c.row_tiles = (uint32_t)((R + c.waves * 32 - 1) / (c.waves * 32));
   const uint64_t blocks = (uint64_t)c.row_tiles * B * Hkv;
   const uint64_t want = 2048 / c.waves;  // eight waves a CU
-  const uint32_t key_tiles = (uint32_t)((Tk + TILE - 1) / TILE);
+  const uint32_t key_tiles = (uint32_t)(((int64_t)Tk + TILE - 1) / TILE);
   uint64_t splits = blocks ? want / blocks : 1;
   const uint64_t most = key_tiles / 4;   // a run of at least four tiles
   if (splits > most) splits = most;

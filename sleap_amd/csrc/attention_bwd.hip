@@ -531,7 +531,8 @@ extern "C" int sa_cross_attention_backward(const void* q, const void* k, const v
   SA_REQUIRE((((uintptr_t)out | (uintptr_t)out_low | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) & 15) == 0, "%s: addresses are multiples of 16", who);
   for (int i = 0; i < 3; ++i) SA_REQUIRE(dout_strides[i] >= 0 && dout_strides[i] % 8 == 0, "%s: strides are multiples of 8 elements", who);
   const int64_t G = Hq / Hkv, far = 1ll << 30;
-  SA_REQUIRE(TILE * strides[1] + G * strides[2] < far && TILE * dout_strides[1] + G * dout_strides[2] < far,
+  auto near = [&](const int64_t* s) { return s[1] < far && s[2] < far && TILE * s[1] + G * s[2] < far; };
+  SA_REQUIRE(near(strides) && near(dout_strides),
              "%s: 64 tokens and the heads on one key head span less than 2^30 elements of q and of dout", who);
   const Layout l = layout(B, Tq, Tk, Hq, Hkv, D, dq, dk);
   SA_REQUIRE((uint64_t)l.kv.blocks + l.rows.blocks < (1ull << 31) && (uint64_t)B * Hq * Tq < (1ull << 31) - 1024 && (uint64_t)B * Hkv < (1ull << 31), "%s: too many rows", who);

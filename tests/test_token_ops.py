@@ -123,6 +123,16 @@ def test_adamw_entry_point_refuses():
     assert call(n=0, table=None) == 0 and call(table=i64(0, 0, 0, 0, 0, 0)) == 0
 
 
+def test_sizes_beyond_64_bits_are_refused():
+    """Counts and strides whose products do not fit 64 bits are not taken for small ones."""
+    h = _lib.lib()
+    refused(h.sa_adamw_step(i64(256, 256, 256, 256, 0, 2 ** 63 - 1), 1, 0, 0, 1e-3, None, 0.9, 0.999, 1e-8, 0.0, 1, None, None), "2^36")
+    near, far = (64, 64, 32), (64, 1 << 58, 32)  # 64 tokens of 2^58 elements: 2^64
+    for q, dout in ((far, near), (near, far), ((64, 64, 1 << 62), near), (near, (64, 64, 1 << 62))):
+        refused(h.sa_cross_attention_backward(256, 256, 256, 1, 1, 4, 8, 8, 2, 32, i64(*q, *near, *near), None, None, None, 1.0, 256, None, 256, 256, i64(*dout), 256, 256, 256, 256,
+                                              1 << 40, None), "span")
+
+
 def test_host_tensors_are_refused():
     x = torch.zeros((1, 2, 1, 8))
     with pytest.raises(ValueError, match="CUDA"):
