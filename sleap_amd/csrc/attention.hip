@@ -434,6 +434,7 @@ int attention_shape(const char* who, AttnShape* a, const void* q, const void* k,
   SA_REQUIRE(dtype == SA_F16 || dtype == SA_BF16, "%s: 16-bit types only (%d)", who, dtype);
   SA_REQUIRE(scale > 0 && scale <= 1e30f, "%s: scale must be positive and finite", who);
   SA_REQUIRE(Tk <= (1 << 30) && (uint64_t)Tq * (Hq / Hkv) < (1ull << 31) - 1024 && (uint64_t)B * Hq < (1ull << 31), "%s: too many rows", who);
+  SA_REQUIRE(strides, "%s: null address of strides", who);
   for (int i = 0; i < 9; ++i) SA_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, "%s: strides are multiples of 8 elements", who);
   for (int i = 3; i < 9; i += 3) SA_REQUIRE(strides[i + 1] < (1ll << 23), "%s: token strides of keys and values are below 2^23 elements", who);
   SA_REQUIRE(!mask || mask_strides, "%s: a mask needs its strides", who);

@@ -529,6 +529,7 @@ extern "C" int sa_cross_attention_backward(const void* q, const void* k, const v
   SA_REQUIRE((Tq == 0 || (out && lse && dout)) && (Tk == 0 || !dk == !dv), "%s: null address", who);
   if (!dq && !dk) return SA_OK;
   SA_REQUIRE((((uintptr_t)out | (uintptr_t)out_low | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) & 15) == 0, "%s: addresses are multiples of 16", who);
+  SA_REQUIRE(dout_strides, "%s: null address of strides", who);
   for (int i = 0; i < 3; ++i) SA_REQUIRE(dout_strides[i] >= 0 && dout_strides[i] % 8 == 0, "%s: strides are multiples of 8 elements", who);
   const int64_t G = Hq / Hkv, far = 1ll << 30;
   auto near = [&](const int64_t* s) { return s[1] < far && s[2] < far && TILE * s[1] + G * s[2] < far; };

@@ -126,6 +126,7 @@ extern "C" int sa_rotary_axes(const void* x, int dtype, int B, int T, int H, int
   SA_REQUIRE(pos_type == SA_POS_I32 || pos_type == SA_POS_I64 || pos_type == SA_POS_F32, "sa_rotary_axes: bad position type %d", pos_type);
   SA_REQUIRE(n_axes >= 1 && n_axes <= MAX_AXES, "sa_rotary_axes: 1 to %d axes", MAX_AXES);
   SA_REQUIRE(theta > 0 && theta < 1e30, "sa_rotary_axes: theta must be positive and finite");
+  SA_REQUIRE(x_strides && pos_strides && sections, "sa_rotary_axes: null address of strides or sections");
   int P = 0;
   for (int a = 0; a < n_axes; ++a) {
     SA_REQUIRE(sections[a] >= 0 && sections[a] <= MAX_PAIRS, "sa_rotary_axes: bad section %d", sections[a]);

@@ -133,6 +133,16 @@ def test_sizes_beyond_64_bits_are_refused():
                                               1 << 40, None), "span")
 
 
+def test_null_host_arrays_are_refused():
+    h = _lib.lib()
+    xs, ps, sections, strides = i64(8, 8, 8), i64(0, 1, 1), (C.c_int * 1)(2), i64(*(64, 64, 32) * 3)
+    for a, b, c in ((None, ps, sections), (xs, None, sections), (xs, ps, None)):
+        refused(h.sa_rotary_axes(256, 0, 1, 1, 1, 8, a, 256, 0, b, 1, c, 1e4, 0, 0, 0, 256, None), "null")
+    refused(h.sa_cross_attention(256, 256, 256, 1, 1, 4, 8, 2, 2, 32, None, None, None, None, 1.0, 256, None, None, 256, 0, None), "null")
+    for a, b in ((None, xs), (strides, None)):
+        refused(h.sa_cross_attention_backward(256, 256, 256, 1, 1, 4, 8, 2, 2, 32, a, None, None, None, 1.0, 256, None, 256, 256, b, 256, 256, 256, 256, 1 << 40, None), "null")
+
+
 def test_host_tensors_are_refused():
     x = torch.zeros((1, 2, 1, 8))
     with pytest.raises(ValueError, match="CUDA"):
