@@ -18,7 +18,7 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=False):
         if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas)):
             raise ValueError(f"AdamW: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=amsgrad))
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=amsgrad, decoupled_weight_decay=True))  # (the last: what a saved state says of itself)
 
     def add_param_group(self, group):
         params = [group["params"]] if isinstance(group["params"], torch.Tensor) else list(group["params"])
@@ -31,13 +31,16 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but the states keep float32 (torch's casts them to their parameter's type). Takes what torch's Adam and AdamW saved
-        (their step is a tensor), unless they maximize or decay otherwise."""
+        (their step is a tensor), unless they maximize or decay otherwise. A state with decay that does not say how it decays (no
+        `decoupled_weight_decay` in its groups: older releases of torch, Adam as well as AdamW) is refused until the key is added."""
         for group in state_dict["param_groups"]:
             if group.get("maximize"):
                 raise ValueError("AdamW: a state of an optimizer with maximize")
-            if group.get("weight_decay") and not group.get("decoupled_weight_decay", True):
-                raise ValueError("AdamW: a state of an optimizer whose weight decay is not decoupled")
+            if group.get("weight_decay") and not group.get("decoupled_weight_decay", False):
+                raise ValueError("AdamW: a state of an optimizer whose weight decay is not decoupled, or that does not say that it is (decoupled_weight_decay=True in its groups)")
         super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            group["decoupled_weight_decay"] = True  # whatever a state without decay said
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for p, i in zip((p for g in self.param_groups for p in g["params"]), saved):
             for name, value in state_dict["state"].get(i, {}).items():

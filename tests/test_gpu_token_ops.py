@@ -1044,6 +1044,23 @@ def test_the_optimizer_goes_on_from_a_state_of_torch():
     opt.load_state_dict(torch.optim.Adam([p]).state_dict())  # without decay both are one
 
 
+def test_the_optimizer_refuses_states_of_unknown_decay():
+    from sleap_amd.nn.optim import AdamW
+
+    p = torch.nn.Parameter(normal(rng(52), 9, dtype=torch.float32))
+    old = torch.optim.Adam([p], weight_decay=0.1).state_dict()
+    del old["param_groups"][0]["decoupled_weight_decay"]
+    opt = AdamW([p])
+    with pytest.raises(ValueError, match="decoupled"):
+        opt.load_state_dict(old)
+    opt.load_state_dict(AdamW([p], weight_decay=0.3).state_dict())
+    assert opt.param_groups[0]["weight_decay"] == 0.3
+    opt.load_state_dict(torch.optim.Adam([p]).state_dict())
+    opt.param_groups[0]["weight_decay"] = 0.2
+    AdamW([p]).load_state_dict(opt.state_dict())  # decays decoupled from here on, and says so
+    torch.optim.AdamW([p]).load_state_dict(opt.state_dict())
+
+
 def test_the_fitting_commands_step_on_the_gpu():
     """tools/train_benchmark_model.py as it is started, three small steps of it: the fit runs and its losses stay finite."""
     import os
