@@ -24,6 +24,8 @@ class AdamW(torch.optim.Optimizer):
         params = [group["params"]] if isinstance(group["params"], torch.Tensor) else list(group["params"])
         if len({id(p) for p in params}) != len(params):
             raise ValueError("AdamW: the same parameter twice in a group")
+        if group.get("maximize") or not group.get("decoupled_weight_decay", True):
+            raise ValueError("AdamW: a group that maximizes, or whose weight decay is not decoupled")
         for p in params:
             if not isinstance(p, torch.Tensor) or not p.is_cuda or p.dtype not in (torch.float32, torch.float16, torch.bfloat16) or not p.is_contiguous():
                 raise ValueError("AdamW: parameters are contiguous float32, float16 or bfloat16 CUDA tensors (there is no CPU fallback)")
@@ -32,7 +34,8 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As torch's, but the states keep float32 (torch's casts them to their parameter's type). Takes what torch's Adam and AdamW saved
         (their step is a tensor), unless they maximize or decay otherwise. A state with decay that does not say how it decays (no
-        `decoupled_weight_decay` in its groups: older releases of torch, Adam as well as AdamW) is refused until the key is added."""
+        `decoupled_weight_decay` in its groups: older releases of torch, Adam as well as AdamW, and of this class) is refused until the key is
+        added."""
         for group in state_dict["param_groups"]:
             if group.get("maximize"):
                 raise ValueError("AdamW: a state of an optimizer with maximize")

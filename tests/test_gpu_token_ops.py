@@ -1061,6 +1061,15 @@ def test_the_optimizer_refuses_states_of_unknown_decay():
     torch.optim.AdamW([p]).load_state_dict(opt.state_dict())
 
 
+def test_the_optimizer_refuses_groups_that_it_would_step_otherwise():
+    from sleap_amd.nn.optim import AdamW
+
+    p = torch.nn.Parameter(normal(rng(52), 9, dtype=torch.float32))
+    for more, what in ((dict(maximize=True), "maximize"), (dict(decoupled_weight_decay=False, weight_decay=0.1), "decoupled")):
+        with pytest.raises(ValueError, match=what):
+            AdamW([dict(params=[p], **more)])
+
+
 def test_the_fitting_commands_step_on_the_gpu():
     """tools/train_benchmark_model.py as it is started, three small steps of it: the fit runs and its losses stay finite."""
     import os
