@@ -36,22 +36,35 @@ class AdamW(torch.optim.Optimizer):
         (their step is a tensor), unless they maximize or decay otherwise. A state with decay that does not say how it decays (no
         `decoupled_weight_decay` in its groups: older releases of torch, Adam as well as AdamW, and of this class) is refused until the key is
         added."""
-        for group in state_dict["param_groups"]:
-            if group.get("maximize"):
-                raise ValueError("AdamW: a state of an optimizer with maximize")
-            if group.get("weight_decay") and not group.get("decoupled_weight_decay", False):
-                raise ValueError("AdamW: a state of an optimizer whose weight decay is not decoupled, or that does not say that it is (decoupled_weight_decay=True in its groups)")
-        super().load_state_dict(state_dict)
-        for group in self.param_groups:
-            group["decoupled_weight_decay"] = True  # whatever a state without decay said
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for p, i in zip((p for g in self.param_groups for p in g["params"]), saved):
-            for name, value in state_dict["state"].get(i, {}).items():
-                if name == "step":
-                    value = int(value)
-                elif isinstance(value, torch.Tensor):
-                    value = value.detach().to(device=p.device, dtype=torch.float32, copy=True).contiguous()
-                self.state[p][name] = value
+        loaded = {}
+
+        def look(_, saved):
+            for group in saved["param_groups"]:
+                if group.get("maximize"):
+                    raise ValueError("AdamW: a state of an optimizer with maximize")
+                if group.get("weight_decay") and not group.get("decoupled_weight_decay", False):
+                    raise ValueError("AdamW: a state of an optimizer whose weight decay is not decoupled, or that does not say that it is (decoupled_weight_decay=True in its groups)")
+            loaded.update(saved)
+
+        def keep(_):
+            for group in self.param_groups:
+                group["decoupled_weight_decay"] = True  # whatever a state without decay said
+            saved = [i for g in loaded["param_groups"] for i in g["params"]]
+            for p, i in zip((p for g in self.param_groups for p in g["params"]), saved):
+                for name, value in loaded["state"].get(i, {}).items():
+                    if name == "step":
+                        value = int(value)
+                    elif isinstance(value, torch.Tensor):
+                        value = value.detach().to(device=p.device, dtype=torch.float32, copy=True).contiguous()
+                    self.state[p][name] = value
+
+        # behind the hooks that may change the state, ahead of those that may read what was loaded
+        hooks = self.register_load_state_dict_pre_hook(look), self.register_load_state_dict_post_hook(keep, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
 
     @torch.no_grad()
     def step(self, closure=None):

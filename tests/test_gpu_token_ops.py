@@ -1070,6 +1070,25 @@ def test_the_optimizer_refuses_groups_that_it_would_step_otherwise():
             AdamW([dict(params=[p], **more)])
 
 
+def test_the_optimizer_loads_what_hooks_leave():
+    """A hook that changes the state ahead of its loading is heard, one that looks at what was loaded sees float32."""
+    from sleap_amd.nn.optim import AdamW
+
+    p = torch.nn.Parameter(normal(rng(53), 9, dtype=torch.bfloat16))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p])
+    opt.step()
+
+    def half(_, saved):
+        return {**saved, "state": {i: {n: x / 2 if torch.is_tensor(x) else x for n, x in s.items()} for i, s in saved["state"].items()}}
+
+    twin, seen = AdamW([p]), []
+    twin.register_load_state_dict_pre_hook(half)
+    twin.register_load_state_dict_post_hook(lambda o: seen.append(o.state[p]["exp_avg"].dtype))
+    twin.load_state_dict(opt.state_dict())
+    assert torch.equal(twin.state[p]["exp_avg"], opt.state[p]["exp_avg"] / 2) and seen == [torch.float32]
+
+
 def test_the_fitting_commands_step_on_the_gpu():
     """tools/train_benchmark_model.py as it is started, three small steps of it: the fit runs and its losses stay finite."""
     import os
