@@ -7,6 +7,7 @@
 // sleap_amd/ops.py, from the library build that the rest of the package uses.
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
@@ -72,20 +73,23 @@ int type_of(const Tensor& t) {
   }
 }
 
-// forward-mode derivatives (torch.autograd.forward_ad) would be lost without a word: a kernel reads a tensor's values alone
+// Forward-mode derivatives (torch.autograd.forward_ad) would be lost without a word: a kernel reads a tensor's values alone. Tensors carry them
+// within a level only; outside of one they are not asked, since each answer takes a lock (448 tensors of an optimizer step: 50 us).
+bool may_carry_tangents() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 void no_tangent(const char* who, const char* name, const Tensor& t) {
   if (t._fw_grad(/*level=*/0).defined()) throw std::runtime_error(text(who, ": ", name, " carries a forward-mode derivative: there are none"));
 }
 
 // The step has no gradient: a graph that it would cut, with what it leaves behind of it, is refused. (A parameter that is a leaf has none.)
 void no_graph(const char* what, const Tensor& t, bool leaf) {
-  if (at::GradMode::is_enabled() && t.requires_grad() && !(leaf && t.is_leaf()))
+  if (t.requires_grad() && !(leaf && t.is_leaf()))
     throw std::runtime_error(text("adamw_step: there is no gradient through a step (", what, " requires one): call it under torch.no_grad()"));
 }
 
 void on_one_gpu(const char* who, std::initializer_list<std::pair<const char*, const Tensor*>> tensors) {
-  for (const auto& [name, t] : tensors)
-    if (t->defined()) no_tangent(who, name, *t);
+  if (may_carry_tangents())
+    for (const auto& [name, t] : tensors)
+      if (t->defined()) no_tangent(who, name, *t);
   const Tensor* first = nullptr;
   for (const auto& [name, t] : tensors) {
     if (!t->defined()) continue;
@@ -361,7 +365,7 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
                 const py::object& max_exp_avg_sqs, const py::object& step, const py::object& lr, std::pair<double, double> betas, double eps,
                 double weight_decay) {
   const char* who = "adamw_step";
-  const bool ams = !max_exp_avg_sqs.is_none();
+  const bool ams = !max_exp_avg_sqs.is_none(), tangents = may_carry_tangents(), recording = at::GradMode::is_enabled();
   const int lists = ams ? 5 : 4;
   const char* names[5] = {"params", "grads", "exp_avgs", "exp_avg_sqs", "max_exp_avg_sqs"};
   const py::object given[5] = {params, grads, exp_avgs, exp_avg_sqs, max_exp_avg_sqs};
@@ -386,8 +390,8 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
   for (const auto& [tensor, kind, what] : {std::tuple(&step, at::kLong, "a step tensor is one int64"), std::tuple(&lr, at::kFloat, "a learning rate tensor is one float32")})
     if (THPVariable_Check(tensor->ptr())) {
       const Tensor& x = THPVariable_Unpack(tensor->ptr());
-      no_tangent(who, "a step or learning rate tensor", x);
-      no_graph("a step or learning rate tensor", x, false);
+      if (tangents) no_tangent(who, "a step or learning rate tensor", x);
+      if (recording) no_graph("a step or learning rate tensor", x, false);
       if (x.scalar_type() != kind || x.numel() != 1 || !x.is_cuda()) bad_value(who, ": ", what, " on the GPU of the parameters");
       if (x.is_neg()) bad_value(who, ": ", what, ", not a negated view");
     }
@@ -405,8 +409,8 @@ void adamw_step(const py::sequence& params, const py::sequence& grads, const py:
     for (int j = 0; j < lists; ++j) {
       if (!THPVariable_Check(items[j][i])) bad_value(who, ": lists of CUDA tensors: ", names[j], "[", i, "] is none");
       x[j] = &THPVariable_Unpack(items[j][i]);
-      no_tangent(who, names[j], *x[j]);
-      no_graph(names[j], *x[j], j == 0);
+      if (tangents) no_tangent(who, names[j], *x[j]);
+      if (recording) no_graph(names[j], *x[j], j == 0);
       if (!x[j]->is_cuda() || x[j]->get_device() != x[0]->get_device())
         bad_value(who, ": CUDA tensors, a parameter, its gradient and its states on one GPU (there is no CPU fallback): ", names[j], "[", i, "] is on ", x[j]->device());
       if (x[j]->layout() != at::kStrided || !x[j]->is_contiguous()) bad_value(who, ": ", names[j], "[", i, "] must be contiguous");
