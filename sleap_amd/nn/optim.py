@@ -90,7 +90,7 @@ class AdamW(torch.optim.Optimizer):
                         s[name] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 sets.setdefault(s["step"] + 1, []).append((p, s))
             for count, items in sets.items():
-                grads = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _ in items]
+                grads = [p.grad if p.grad.is_contiguous() and not p.grad.is_neg() else p.grad.resolve_neg().contiguous() for p, _ in items]
                 m, v, *w = ([s[name] for _, s in items] for name in names)
                 ops.adamw_step([p for p, _ in items], grads, m, v, max_exp_avg_sqs=w[0] if w else None, step=count, lr=group["lr"],
                                betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"])

@@ -1016,6 +1016,19 @@ def test_the_optimizer_keeps_float32_states_of_16_bit_parameters():
             opt.step()
 
 
+def test_the_optimizer_reads_negated_gradients():
+    """What the backward pass of a conjugation may leave: a view that torch holds with the other sign."""
+    from sleap_amd.nn.optim import AdamW
+
+    for n in (1, 5):
+        z = torch.randn(n, generator=rng(55), device=DEV, dtype=torch.complex64)
+        params = [torch.nn.Parameter(torch.ones(n, device=DEV)) for _ in range(2)]
+        params[0].grad, params[1].grad = z.conj().imag, -z.imag
+        assert params[0].grad.is_neg()
+        AdamW(params).step()
+        assert torch.equal(*params)
+
+
 def test_the_optimizer_goes_on_from_a_state_of_torch():
     """What torch's AdamW saved (a float32 tensor as step) continues: a step from it is `ops.adamw_step` with the next count; what this
     optimizer would do otherwise is refused."""
