@@ -8,6 +8,10 @@ import torch
 from .. import ops
 
 
+def _taken(p):
+    return isinstance(p, torch.Tensor) and p.is_cuda and p.dtype in (torch.float32, torch.float16, torch.bfloat16) and p.is_contiguous()
+
+
 class AdamW(torch.optim.Optimizer):
     """m, v (and the running maximum of v with `amsgrad`) are float32 whatever the parameter's type; see `ops.adamw_step`.
 
@@ -27,7 +31,7 @@ class AdamW(torch.optim.Optimizer):
         if group.get("maximize") or not group.get("decoupled_weight_decay", True):
             raise ValueError("AdamW: a group that maximizes, or whose weight decay is not decoupled")
         for p in params:
-            if not isinstance(p, torch.Tensor) or not p.is_cuda or p.dtype not in (torch.float32, torch.float16, torch.bfloat16) or not p.is_contiguous():
+            if not _taken(p):
                 raise ValueError("AdamW: parameters are contiguous float32, float16 or bfloat16 CUDA tensors (there is no CPU fallback)")
         super().add_param_group({**group, "params": params})
 
@@ -100,8 +104,9 @@ class AdamW(torch.optim.Optimizer):
 
 
 def adam(params, lr):
-    """What the fitting commands step with: `AdamW` without decay, which is Adam, on a GPU; torch's Adam on the CPU."""
+    """What the fitting commands step with: `AdamW` without decay, which is Adam, on a GPU; torch's Adam on the CPU and
+    for parameters that `AdamW` does not take (another type or layout)."""
     params = list(params)
-    if all(p.is_cuda for p in params):
+    if all(_taken(p) for p in params):
         return AdamW(params, lr=lr, weight_decay=0.0)
     return torch.optim.Adam(params, lr=lr)

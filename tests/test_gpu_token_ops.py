@@ -1029,6 +1029,18 @@ def test_the_optimizer_reads_negated_gradients():
         assert torch.equal(*params)
 
 
+def test_what_the_fitting_commands_step_with():
+    from sleap_amd.nn.optim import AdamW, adam
+
+    kernel = normal(rng(56), 8, 4, 3, 3, dtype=torch.float32)
+    for p, kind in ((kernel, AdamW), (kernel.to(memory_format=torch.channels_last), torch.optim.Adam), (kernel.double(), torch.optim.Adam), (kernel.cpu(), torch.optim.Adam)):
+        p = torch.nn.Parameter(p)
+        p.grad = torch.ones_like(p)
+        opt = adam([p], 1e-2)
+        assert type(opt) is kind
+        opt.step()
+
+
 def test_the_optimizer_goes_on_from_a_state_of_torch():
     """What torch's AdamW saved (a float32 tensor as step) continues: a step from it is `ops.adamw_step` with the next count; what this
     optimizer would do otherwise is refused."""
