@@ -743,7 +743,8 @@ int sa_rotary_axes(const void* x, int dtype, int B, int T, int H, int D, const i
  *   out          [B,Tq,Hq,D] contiguous; zeros where no key is visible; NaN (lse too) where all visible ones score -inf
  *   lse          [B,Hq,Tq] natural logarithm of the softmax's denominator (-inf where no key is visible), or NULL
  *   out_low      like out: out + out_low is the result with about twice the bits of its type (for the gradients of few keys; half as many
- *                products again; over more than 2048 visible keys the weights are multiplied in one term only), or NULL
+ *                products again; over up to 2048 visible keys all weights are multiplied in two terms, over more at least a part of them
+ *                in one), or NULL
  *   workspace    sa_cross_attention_workspace bytes (0: none): runs of keys that several workgroups work on */
 size_t sa_cross_attention_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D);
 int sa_cross_attention(const void* q, const void* k, const void* v, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D,

@@ -1,7 +1,7 @@
 // Host side of the token operators: checks, layouts, workspaces, streams and gradients of `ops.rotary_axes`, `ops.cross_attention` and
 // `ops.adamw_step` over the C ABI of include/sleap_amd.h. In C++ because these calls are small beside what Python charges for them: a
-// rotary call of a frame's queries runs 3.5 us on the GPU and cost its host 13 us through ctypes, the gradients of an attention 130 us
-// (now what torch's engine itself takes), the checks of 448 tensors of an optimizer step 600 us (now 40).
+// rotary call of a frame's queries runs 3.5 us on the GPU and cost its host 13 us through ctypes (now 5), an attention with its gradients 155 us
+// (now 70, of which torch's engine alone takes 27), the step of 448 tensors 600 us (now 50, its four launches among them).
 //
 // Plain torch C++ on raw tensors: device memory, streams and the autograd graph. The entry points are handed over as addresses by
 // sleap_amd/ops.py, from the library build that the rest of the package uses.

@@ -1,5 +1,5 @@
 """AdamW for the commands that fit models (tools/train_benchmark_model.py, tools/train_config_models.py) and for networks of token
-operators: torch's optimizer interface (parameter groups, schedulers, state_dict) over `ops.adamw_step`, one launch per 128 tensors.
+operators: torch's optimizer interface (parameter groups, schedulers, state_dict) over `ops.adamw_step`, one launch per 128 tensors (108 with amsgrad).
 
 The reference fits with tf.keras.optimizers.Adam(amsgrad=True) (sleap/nn/config/optimization.py, sleap/nn/training.py); without
 weight decay this is Adam, with `amsgrad=True` its running maximum."""

@@ -401,8 +401,8 @@ def optical_flow_pyr_lk(prev: "FlowPyramid", nxt: "FlowPyramid", points, max_cou
 
 # --------------------------------------------------------------------------------------------------
 # token operators (csrc/rotary.hip, attention.hip, attention_bwd.hip, adamw.hip): keypoint queries and feature-map tokens. Unlike the
-# layer wrappers above they take any torch layout, check their arguments, run on the device of their tensors and have gradients; their
-# host side is C++ (csrc/token_host.cpp), which calls the same C ABI.
+# layer wrappers above they take any torch layout, check their arguments (forward-mode derivatives are refused), run on the device of their
+# tensors and have gradients; their host side is C++ (csrc/token_host.cpp), which calls the same C ABI.
 # --------------------------------------------------------------------------------------------------
 _token_host = None
 
@@ -444,7 +444,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, return
     scale        positive; default 1 / sqrt(D)
     return_lse   also the natural logarithm of the softmax's denominators, (B, H, Tq) float32, without a gradient
     A query that sees no key gives zeros (lse: -inf) and passes no gradient. Softmax and sums are float32. Weights are rounded to q's type ahead of
-    their products, which makes results about 1.4 times as inexact as their own rounding; what the rounding leaves is multiplied as well (and
+    their products, which makes results 1.4 times as inexact as their own rounding (up to 2.8 times where a few weights make them up); what the rounding leaves is multiplied as well (and
     results are as exact as their type) in a call that is to be differentiated over at most 2048 visible keys, and in its gradients up to 2^30
     multiply-adds a product. Results do not depend on the order in which workgroups run. Differentiable in q, k and v, once: queries on a
     frozen map cost their own gradient only, and so do keys and values together."""
@@ -452,7 +452,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, return
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_exp_avg_sqs=None):
-    """One AdamW step over many tensors, in place, a launch for up to 128 of one type and device:
+    """One AdamW step over many tensors, in place, a launch for up to 128 (with max_exp_avg_sqs 108) of one type and device:
 
         m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  [vmax = max(vmax, v)]
         p = p (1 - lr wd) - lr / (1-b1^t) m / (sqrt(v or vmax) / sqrt(1-b2^t) + eps)
@@ -462,5 +462,6 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
                     overlaps with nothing else that is written or read (a gradient may serve several parameters, or be its own)
     exp_avgs, exp_avg_sqs, max_exp_avg_sqs (amsgrad, or None)   float32 tensors of the same sizes
     step            t >= 1, or a one-element int64 CUDA tensor that already holds it; lr likewise a number or a one-element float32 CUDA
-                    tensor. A captured step takes its count as a tensor only, and a learning rate given as a number stays that of the capture."""
+                    tensor. A captured step takes its count as a tensor only, and a learning rate given as a number stays that of the capture.
+    There is no gradient through a step: in grad mode parameters are leaves and nothing else requires a gradient."""
     _token().adamw_step(params, grads, exp_avgs, exp_avg_sqs, max_exp_avg_sqs, step, lr, betas, eps, weight_decay)
