@@ -3,7 +3,7 @@
 //     S^T [keys x rows] = k q^T        P^T = exp2(c S^T - m)        O^T [d x rows] += v^T P^T
 //
 // A wave has 32 rows, a workgroup of one, two or four waves a tile of 64 keys and values in LDS, the next one on its way. At 128 values
-// a head two workgroups a CU overlap one's products with the other's exponentials: 2 x 8 heads x 4096 x 16384 bf16 in 530 us = 1.04
+// a head two workgroups a CU overlap one's products with the other's exponentials: 2 x 8 heads x 4096 x 16384 bf16 in 523 us = 1.05
 // PFLOP/s (a library product of 8192^3: 1.19), matrix pipes busy 0.53 of the time at the 1.85 GHz that the chip holds under that load. At 64
 // values the vector units are the limit (32 exponentials of 16 cycles a tile and lane beside 512 cycles of products): 0.70 to 0.77
 // PFLOP/s. Where rows are few, waves share the keys (52 queries x 8 heads x 32 on 1024 keys: 6.1 us) or the keys are cut

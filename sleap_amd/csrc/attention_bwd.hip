@@ -6,7 +6,7 @@
 // atomics or a float32 dq read and written once per tile of keys. Shared heads are rows like any others (attention.h): dk and dv sum
 // over them by themselves. Where one side owns little, runs of what it walks go to several workgroups, and a last
 // kernel adds their float32 sums in order. A side whose gradients nobody asks for (a frozen map, given queries) is not run: forward and
-// backward of 4096 x 8192 x 8 x 128 take 593 us, for dq alone 349, for dk and dv alone 405.
+// backward of 4096 x 8192 x 8 x 128 take 574 us, for dq alone 335, for dk and dv alone 387.
 //
 // Measured: 8 heads x 4096 x 8192 x 128 bf16 430 us for both sides = 1.12 PFLOP/s of seven products (the rate of a large library product);
 // 8 x 8 heads x 192 x 4096 x 64 68 us, 0.66 PFLOP/s: three tiles of rows a workgroup, so that what it reads first and writes last weighs.
