@@ -104,18 +104,20 @@ bool capturing(const at::Device& d) {
   return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
 }
 
-// whether a stream is the current one or another that the capture has taken in (the default stream can not be, and is not asked)
-bool captured(const c10::Stream& s) {
+// whether a stream is the current one or another that the capture has taken in, or, of a leaf's node, can take in and gives back by itself (the
+// engine joins the streams of leaves when a backward pass ends). The default stream can not be captured, and is not asked.
+bool captured(const c10::Stream& s, bool leaf) {
   const auto now = c10::hip::getCurrentHIPStream(s.device_index());
   if (s.id() == now.id()) return true;
   const hipStream_t other = c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, c10::Stream(c10::Stream::UNSAFE, now.unwrap().device(), s.id())).stream();
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  return other && hipStreamIsCapturing(other, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+  return other && (leaf || (hipStreamIsCapturing(other, &status) == hipSuccess && status == hipStreamCaptureStatusActive));
 }
 
 // A graph that was built outside of a capture and still lives holds the gradient nodes of its leaves, and with them the stream that it was
 // built on: a captured backward pass that reaches one of its nodes would pull that stream into the capture, where torch's engine ends the
-// process. Refused before it starts; everything that the inputs hang on is looked at, while capturing only.
+// process. Refused before it starts; everything that the inputs hang on is looked at, while capturing only. (Leaves whose graph was
+// built on a stream of its own, as a warm-up ahead of a capture is, are fine.)
 void not_held_elsewhere(const char* who, std::initializer_list<const Tensor*> tensors) {
   if (!capturing((*tensors.begin())->device())) return;
   std::vector<std::shared_ptr<torch::autograd::Node>> todo;
@@ -129,7 +131,7 @@ void not_held_elsewhere(const char* who, std::initializer_list<const Tensor*> te
     const auto node = std::move(todo.back());
     todo.pop_back();
     const auto held = node->stream();
-    if (held && !captured(*held))
+    if (held && !captured(*held, node->next_edges().empty()))
       throw std::runtime_error(text(who, ": captured while a graph from outside of the capture holds the same leaf: delete that graph first (or capture a detached leaf)"));
     for (const auto& edge : node->next_edges()) meet(edge.function);
   }

@@ -402,7 +402,9 @@ def optical_flow_pyr_lk(prev: "FlowPyramid", nxt: "FlowPyramid", points, max_cou
 # --------------------------------------------------------------------------------------------------
 # token operators (csrc/rotary.hip, attention.hip, attention_bwd.hip, adamw.hip): keypoint queries and feature-map tokens. Unlike the
 # layer wrappers above they take any torch layout, check their arguments (forward-mode derivatives are refused), run on the device of their
-# tensors and have gradients; their host side is C++ (csrc/token_host.cpp), which calls the same C ABI.
+# tensors and have gradients; their host side is C++ (csrc/token_host.cpp), which calls the same C ABI. They can be captured into graphs, gradients
+# included, as torch's own capture of callables does; refused are inputs that hang on a graph from outside of the capture, and leaves that such a
+# graph, built on the default stream, still holds (a warm-up belongs on a stream of its own).
 # --------------------------------------------------------------------------------------------------
 _token_host = None
 

@@ -712,6 +712,77 @@ def test_a_capture_over_two_streams():
         assert (out.float() - want.float()).abs().max() <= 2.0 ** -11 * (v.float().abs().max() + 2 * want.float().abs().max()) * 1.01
 
 
+def test_callables_graphed_by_torch():
+    """torch's own capture of a function and its gradients, which keeps its warm-up's graph (on a stream of its own) while it captures."""
+    from sleap_amd import ops
+
+    p = torch.rand((30, 2), generator=rng(57), device=DEV) * 50
+
+    def data(seed):
+        g = rng(seed)
+        return [normal(g, 2, n, 4, 32).requires_grad_(True) for n in (30, 700, 700)]
+
+    def step(q, k, v):
+        return ops.cross_attention(ops.rotary_axes(q, p, (8, 8)), k, v)
+
+    graphed = torch.cuda.make_graphed_callables(step, tuple(data(58)))
+    for seed in (59, 60, 61):
+        one, two, dout = data(seed), data(seed), normal(rng(seed + 10), 2, 30, 4, 32)
+        got, want = (f(*x) for f, x in ((graphed, one), (step, two)))
+        for a, b in zip((got, *torch.autograd.grad(got, one, dout)), (want, *torch.autograd.grad(want, two, dout))):
+            assert torch.equal(a, b)
+
+
+def test_a_captured_fit_after_a_warm_up_that_lives():
+    """Warm-up on a side stream whose graph is still held, then forward, backward and optimizer step in one graph; replayed on new inputs against
+    the same steps made one by one."""
+    from sleap_amd import ops
+
+    g = rng(62)
+    q0, w0 = normal(g, 1, 20, 2, 32, dtype=torch.float32), normal(g, 64, 64, dtype=torch.float32, scale=0.1)
+    x, target = normal(g, 3, 500, 64, dtype=torch.float32), normal(g, 3, 20, 2, 32, dtype=torch.float32)
+    place = torch.rand((20, 2), generator=g, device=DEV) * 9
+
+    def make_fit():
+        leaves = [t.clone().requires_grad_(True) for t in (q0, w0)]
+        states = [[torch.zeros_like(t) for t in leaves] for _ in range(2)]
+        count, rate = torch.zeros(1, dtype=torch.int64, device=DEV), torch.full((1,), 1e-2, device=DEV)
+
+        def fit(update=True):
+            for t in leaves:
+                t.grad = None
+            kv = (x @ leaves[1]).half().view(3, 500, 2, 32)
+            q = ops.rotary_axes(leaves[0].half().expand(3, 20, 2, 32), place, (8, 8))
+            loss = ((ops.cross_attention(q, kv, kv).float() - target) ** 2).mean()
+            loss.backward()
+            if update:
+                with torch.no_grad():
+                    count.add_(1)
+                    ops.adamw_step(leaves, [t.grad for t in leaves], *states, step=count, lr=rate)
+            return loss
+
+        return leaves, fit
+
+    (leaves, fit), (twins, twin) = make_fit(), make_fit()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        held = fit(update=False)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = fit()
+    for turn in range(3):
+        x.copy_(normal(rng(70 + turn), 3, 500, 64, dtype=torch.float32))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = twin()
+        assert torch.equal(loss.detach(), want.detach())
+        for a, b in zip(leaves, twins):
+            assert torch.equal(a.grad, b.grad) and torch.equal(a, b)
+    assert torch.isfinite(held)
+
+
 def test_two_calls_at_once_on_two_streams():
     """Calls with scratch, from two threads on streams of their own, do not meet."""
     import threading
